@@ -56,6 +56,48 @@ class HkAttnDesc(C.Structure):
     ]
 
 
+class HkPrefixAttnDesc(C.Structure):
+    _fields_ = [
+        ("Q", C.c_void_p), ("KP", C.c_void_p), ("VP", C.c_void_p), ("K", C.c_void_p), ("V", C.c_void_p), ("O", C.c_void_p),
+        ("key_bias", C.c_void_p), ("ws", C.c_void_p), ("ws_bytes", C.c_size_t),
+        ("B", C.c_int32), ("H", C.c_int32), ("Nq", C.c_int32), ("P", C.c_int32), ("Nk", C.c_int32), ("head_dim", C.c_int32),
+        ("ldq", C.c_int64), ("bsq", C.c_int64), ("ldkp", C.c_int64), ("ldvp", C.c_int64), ("ldk", C.c_int64), ("bsk", C.c_int64),
+        ("ldv", C.c_int64), ("bsv", C.c_int64), ("ldo", C.c_int64), ("bso", C.c_int64), ("bias_bs", C.c_int64),
+    ]
+
+
+class HkStepWeightsDesc(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("k_cache", C.c_void_p), ("v_cache", C.c_void_p), ("key_bias", C.c_void_p), ("w_in", C.c_void_p),
+        ("w_out", C.c_void_p), ("out", C.c_void_p), ("ws", C.c_void_p), ("ws_bytes", C.c_size_t),
+        ("B", C.c_int32), ("H", C.c_int32), ("head_dim", C.c_int32), ("n_keys", C.c_int32),
+        ("cache_rows", C.c_int64), ("bias_bs", C.c_int64), ("bias_hs", C.c_int64), ("wi_bs", C.c_int64), ("wi_hs", C.c_int64),
+        ("wo_bs", C.c_int64), ("wo_hs", C.c_int64),
+    ]
+
+
+class HkKeyWeightsDesc(C.Structure):
+    _fields_ = [
+        ("Q", C.c_void_p), ("K", C.c_void_p), ("key_bias", C.c_void_p), ("w_in", C.c_void_p), ("w_out", C.c_void_p),
+        ("ws", C.c_void_p), ("ws_bytes", C.c_size_t),
+        ("B", C.c_int32), ("H", C.c_int32), ("Nq", C.c_int32), ("Nk", C.c_int32), ("head_dim", C.c_int32), ("causal", C.c_int32),
+        ("ldq", C.c_int64), ("bsq", C.c_int64), ("ldk", C.c_int64), ("bsk", C.c_int64), ("bias_bs", C.c_int64),
+        ("wi_bs", C.c_int64), ("wi_hs", C.c_int64), ("wo_bs", C.c_int64), ("wo_hs", C.c_int64),
+    ]
+
+
+class HkCacheEvictDesc(C.Structure):
+    _fields_ = [
+        ("K", C.c_void_p), ("V", C.c_void_p), ("k_out", C.c_void_p), ("v_out", C.c_void_p), ("weight", C.c_void_p),
+        ("weight_out", C.c_void_p), ("key_bias", C.c_void_p), ("key_bias_out", C.c_void_p), ("kept", C.c_void_p),
+        ("B", C.c_int32), ("H", C.c_int32), ("head_dim", C.c_int32), ("n_keys", C.c_int32), ("budget", C.c_int32), ("recent", C.c_int32),
+        ("ldk", C.c_int64), ("bsk", C.c_int64), ("ldv", C.c_int64), ("bsv", C.c_int64),
+        ("ldko", C.c_int64), ("bsko", C.c_int64), ("ldvo", C.c_int64), ("bsvo", C.c_int64),
+        ("w_bs", C.c_int64), ("w_hs", C.c_int64), ("wo_bs", C.c_int64), ("wo_hs", C.c_int64),
+        ("b_bs", C.c_int64), ("b_hs", C.c_int64), ("bo_bs", C.c_int64), ("bo_hs", C.c_int64),
+    ]
+
+
 class HkTransposeJob(C.Structure):
     _fields_ = [("x", C.c_void_p), ("out", C.c_void_p), ("ld", C.c_int64), ("ldo", C.c_int64),
                 ("R", C.c_int32), ("C", C.c_int32), ("tile0", C.c_int32), ("pad_", C.c_int32)]
@@ -114,6 +156,12 @@ SYMBOLS = {
     "hk_decode_attn_rope_bf16": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p,
                                            C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int64,
                                            C.c_int64, C.c_int32, C.c_float, C.c_int32, C.c_void_p, C.c_void_p]),
+    "hk_prefix_attn_bf16": (C.c_int, [C.POINTER(HkPrefixAttnDesc), C.c_void_p]),
+    "hk_prefix_attn_ws": (C.c_size_t, [C.c_int32] * 6),
+    "hk_decode_attn_weights_bf16": (C.c_int, [C.POINTER(HkStepWeightsDesc), C.c_void_p]),
+    "hk_decode_attn_weights_ws": (C.c_size_t, [C.c_int32] * 4),
+    "hk_attn_key_weights_bf16": (C.c_int, [C.POINTER(HkKeyWeightsDesc), C.c_void_p]),
+    "hk_cache_evict_bf16": (C.c_int, [C.POINTER(HkCacheEvictDesc), C.c_void_p]),
     "hk_argmax_f32": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int64, C.c_void_p]),
     "hk_silu_mul_bf16": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p]),
     "hk_rmsnorm_add_parts": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64,

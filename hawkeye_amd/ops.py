@@ -488,6 +488,222 @@ def decode_attn_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, po
     return out
 
 
+# ---------------------------------------------------------------- a shared prefix; caches cut by attention weight
+def _strides(t: torch.Tensor, name: str, H: int, hd: int):
+    """(token stride, batch stride) of a bf16 [B, N, H, hd] view whose last two dims are dense; of a dim of size 1 the stride is free."""
+    _need(t, torch.bfloat16, name)
+    if t.dim() != 4 or t.shape[2] != H or t.shape[3] != hd or t.stride(3) != 1 or (H > 1 and t.stride(2) != hd):
+        raise RuntimeError(f"{name} must be [B,N,{H},{hd}] with dense (H,{hd}) dims, got {tuple(t.shape)} strides {t.stride()}")
+    return (t.stride(1) if t.shape[1] > 1 else H * hd), (t.stride(0) if t.shape[0] > 1 else H * hd * t.shape[1])
+
+
+def _one_device(what: str, *ts):
+    dev = ts[0].device
+    for t in ts:
+        if t is not None and t.device != dev:
+            raise RuntimeError(f"{what}: tensors on {dev} and {t.device}")
+    return dev
+
+
+def _per_key(t: Optional[torch.Tensor], name: str, B: int, H: int, n: int, per_head: bool):
+    """(batch stride, head stride) of an fp32 [B, H, >= n] tensor (or [B, >= n] where one row serves all heads)."""
+    if t is None:
+        return 0, 0
+    _need(t, torch.float32, name)
+    shared = t.dim() == 2 and not per_head
+    if not shared and t.dim() != 3 or t.shape[0] != B or (not shared and t.shape[1] != H) or t.shape[-1] < n or (n > 1 and t.stride(-1) != 1):
+        raise RuntimeError(f"{name} must be fp32 [{B}, {H}, >= {n}]{'' if per_head else f' or [{B}, >= {n}]'} with unit key stride, got {tuple(t.shape)}")
+    return (t.stride(0) if B > 1 else H * t.shape[-1]), 0 if shared else (t.stride(1) if H > 1 else t.shape[-1])
+
+
+def _span(t: torch.Tensor):
+    a = t.data_ptr()
+    return a, a + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() if t.numel() else a
+
+
+def _no_overlap(what: str, out: torch.Tensor, *ins):
+    a0, a1 = _span(out)
+    for t in ins:
+        if t is not None:
+            b0, b1 = _span(t)
+            if a0 < b1 and b0 < a1:
+                raise RuntimeError(f"{what}: the output overlaps an input")
+
+
+def prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                     key_bias: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                     ws: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of a batch whose sequences share a prefix: q [B,Nq,H,hd] (pre-scaled by scale*log2(e)) over the prefix's keys
+    k_prefix / v_prefix [P,H,hd] (P >= 0, one copy for all sequences, all visible) and the sequences' own k / v [B,Nk,H,hd]
+    (Nk >= Nq >= 1, causal: query i sees own keys <= i + Nk - Nq).  bf16 views, hd 64 or 128, last two dims dense; returns
+    [B,Nq,H,hd] bf16.  key_bias: optional fp32 [B, >= Nk] of the own keys (natural-log units); -1e4 or less removes the key.  A row that sees
+    no key gives zeros.  ws: uint8 of at least prefix_attention_ws(...) bytes (default: allocated), for this call alone."""
+    if q.dim() != 4 or q.shape[3] not in (64, 128):
+        raise RuntimeError("prefix_attention: q must be [B,Nq,H,hd], head size 64 or 128")
+    B, Nq, H, hd = q.shape
+    if k_prefix.dim() != 3 or v_prefix.dim() != 3 or k_prefix.shape != v_prefix.shape:
+        raise RuntimeError("prefix_attention: k_prefix and v_prefix must be [P,H,hd]")
+    if k.dim() != 4 or k.shape != v.shape or k.shape[0] != B:
+        raise RuntimeError("prefix_attention: k and v must be [B,Nk,H,hd]")
+    P, Nk = k_prefix.shape[0], k.shape[1]
+    if Nq < 1 or Nk < Nq:
+        raise RuntimeError(f"prefix_attention: {Nq} queries need at least as many own keys, got {Nk}")
+    dev = _one_device("prefix_attention", q, k_prefix, v_prefix, k, v, key_bias, out, ws)
+    ldq, bsq = _strides(q, "q", H, hd)
+    ldkp, _ = _strides(k_prefix[None], "k_prefix", H, hd)
+    ldvp, _ = _strides(v_prefix[None], "v_prefix", H, hd)
+    ldk, bsk = _strides(k, "k", H, hd)
+    ldv, bsv = _strides(v, "v", H, hd)
+    bias_bs = 0
+    if key_bias is not None:
+        if key_bias.dim() != 2:
+            raise RuntimeError("prefix_attention: key_bias must be fp32 [B, >= Nk]")
+        bias_bs, _ = _per_key(key_bias, "key_bias", B, 1, Nk, False)
+    if out is None:
+        out = torch.empty((B, Nq, H, hd), dtype=torch.bfloat16, device=dev)
+    if out.shape != q.shape:
+        raise RuntimeError(f"prefix_attention: out must be {tuple(q.shape)}")
+    ldo, bso = _strides(out, "out", H, hd)
+    _no_overlap("prefix_attention", out, k_prefix, v_prefix, k, v, key_bias, ws)
+    lib = L.load()
+    need = prefix_attention_ws(B, H, Nq, P, Nk, hd)
+    with torch.cuda.device(dev):
+        if ws is None:
+            ws = torch.empty((need,), dtype=torch.uint8, device=dev)
+        _need(ws, torch.uint8, "ws")
+        d = L.HkPrefixAttnDesc(q.data_ptr(), k_prefix.data_ptr(), v_prefix.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(key_bias),
+                               ws.data_ptr(), ws.numel(), B, H, Nq, P, Nk, hd, ldq, bsq, ldkp, ldvp, ldk, bsk, ldv, bsv, ldo, bso, bias_bs)
+        L.check(lib.hk_prefix_attn_bf16(C.byref(d), _stream()), "hk_prefix_attn_bf16")
+    return out
+
+
+def prefix_attention_ws(B: int, H: int, Nq: int, P: int, Nk: int, head_dim: int) -> int:
+    """Workspace bytes of one prefix_attention call."""
+    need = L.load().hk_prefix_attn_ws(B, H, Nq, P, Nk, head_dim)
+    if need == 0:
+        raise RuntimeError(f"prefix_attention: shape B={B} H={H} Nq={Nq} P={P} Nk={Nk} head size {head_dim} is not supported")
+    return need
+
+
+def decode_attn_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, n_keys: int, H: int, head_dim: int,
+                        weight: Optional[torch.Tensor], key_bias: Optional[torch.Tensor] = None,
+                        weight_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """decode_attn (one query row per (sequence, head) over cache rows [0, n_keys): bf16 [B, H*hd]) that also adds the row's softmax weights
+    to what the keys have collected: weight_out[..., :n_keys] = weight[..., :n_keys] + p, fp32 [B, H, >= n_keys] (weight_out None: in
+    place; weight None: zeros).  key_bias: optional fp32 [B, >= n_keys] or, once heads keep different rows, [B, H, >= n_keys]; -1e4 or
+    less removes the key.  A sequence without a key gives zeros and adds nothing."""
+    _need(q, torch.bfloat16, "q")
+    _need(k_cache, torch.bfloat16, "k_cache")
+    _need(v_cache, torch.bfloat16, "v_cache")
+    if weight_out is None:
+        weight_out = weight
+    if weight_out is None:
+        raise RuntimeError("decode_attn_weights: weight and weight_out are both None")
+    B, D = q.shape[0], H * head_dim
+    if tuple(q.shape) != (B, D) or not q.is_contiguous() or k_cache.shape != v_cache.shape or k_cache.dim() != 3 or k_cache.shape[0] != B \
+            or k_cache.shape[2] != D or not k_cache.is_contiguous() or not v_cache.is_contiguous():
+        raise RuntimeError("decode_attn_weights: q contiguous [B, H*hd], caches contiguous [B, rows, H*hd]")
+    if not 1 <= n_keys <= k_cache.shape[1]:
+        raise RuntimeError(f"decode_attn_weights: n_keys={n_keys} must be 1..{k_cache.shape[1]}")
+    dev = _one_device("decode_attn_weights", q, k_cache, v_cache, weight, weight_out, key_bias)
+    wi_bs, wi_hs = _per_key(weight, "weight", B, H, n_keys, True)
+    wo_bs, wo_hs = _per_key(weight_out, "weight_out", B, H, n_keys, True)
+    bias_bs, bias_hs = _per_key(key_bias, "key_bias", B, H, n_keys, False)
+    same = weight is not None and weight.data_ptr() == weight_out.data_ptr()
+    _no_overlap("decode_attn_weights", weight_out, q, k_cache, v_cache, key_bias, None if same else weight)
+    lib = L.load()
+    with torch.cuda.device(dev):
+        out = torch.empty_like(q)
+        need = lib.hk_decode_attn_weights_ws(B, H, head_dim, n_keys)
+        ws = torch.empty((max(need, 16),), dtype=torch.uint8, device=dev)
+        d = L.HkStepWeightsDesc(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _ptr(key_bias), _ptr(weight), weight_out.data_ptr(),
+                                out.data_ptr(), ws.data_ptr(), ws.numel(), B, H, head_dim, n_keys, k_cache.shape[1], bias_bs, bias_hs,
+                                wi_bs, wi_hs, wo_bs, wo_hs)
+        L.check(lib.hk_decode_attn_weights_bf16(C.byref(d), _stream()), "hk_decode_attn_weights_bf16")
+    return out
+
+
+def attn_key_weights(q: torch.Tensor, k: torch.Tensor, key_bias: Optional[torch.Tensor] = None, causal: bool = True,
+                     weight: Optional[torch.Tensor] = None, weight_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The attention weight every key collects from the queries of a prompt (or of its last Nq tokens): the sum over the rows of q
+    [B,Nq,H,hd] (pre-scaled) of their softmax weights over k [B,Nk,H,hd] -> fp32 [B,H,Nk]; causal: query i sees keys <= i + Nk - Nq.
+    weight fp32 [B,H,>=Nk]: added to it, in place unless weight_out (of the same kind) is given; both None: a new tensor.
+    key_bias fp32 [B, >= Nk] (-1e4 or less removes the key).  A query that sees no key adds nothing."""
+    if q.dim() != 4 or k.dim() != 4 or q.shape[3] not in (64, 128) or k.shape[0] != q.shape[0]:
+        raise RuntimeError("attn_key_weights: q [B,Nq,H,hd] and k [B,Nk,H,hd], head size 64 or 128")
+    B, Nq, H, hd = q.shape
+    Nk = k.shape[1]
+    if Nq < 1 or Nk < 1 or (causal and Nk < Nq):
+        raise RuntimeError(f"attn_key_weights: Nq={Nq}, Nk={Nk} (at least one each; causal needs Nk >= Nq)")
+    dev = _one_device("attn_key_weights", q, k, key_bias, weight, weight_out)
+    ldq, bsq = _strides(q, "q", H, hd)
+    ldk, bsk = _strides(k, "k", H, hd)
+    bias_bs = 0
+    if key_bias is not None:
+        if key_bias.dim() != 2:
+            raise RuntimeError("attn_key_weights: key_bias must be fp32 [B, >= Nk]")
+        bias_bs, _ = _per_key(key_bias, "key_bias", B, 1, Nk, False)
+    with torch.cuda.device(dev):
+        if weight_out is None:
+            weight_out = weight if weight is not None else torch.empty((B, H, Nk), dtype=torch.float32, device=dev)
+        wi_bs, wi_hs = _per_key(weight, "weight", B, H, Nk, True)
+        wo_bs, wo_hs = _per_key(weight_out, "weight_out", B, H, Nk, True)
+        same = weight is not None and weight.data_ptr() == weight_out.data_ptr()
+        _no_overlap("attn_key_weights", weight_out, q, k, key_bias, None if same else weight)
+        ws = torch.empty((B * H * Nq,), dtype=torch.float32, device=dev)
+        d = L.HkKeyWeightsDesc(q.data_ptr(), k.data_ptr(), _ptr(key_bias), _ptr(weight), weight_out.data_ptr(), ws.data_ptr(), ws.numel() * 4,
+                               B, H, Nq, Nk, hd, 1 if causal else 0, ldq, bsq, ldk, bsk, bias_bs, wi_bs, wi_hs, wo_bs, wo_hs)
+        L.check(L.load().hk_attn_key_weights_bf16(C.byref(d), _stream()), "hk_attn_key_weights_bf16")
+    return weight_out
+
+
+def cache_evict(k: torch.Tensor, v: torch.Tensor, weight: torch.Tensor, n_keys: int, budget: int, recent: int = 0,
+                key_bias: Optional[torch.Tensor] = None, out=None) -> torch.Tensor:
+    """Cut a cache to `budget` rows by accumulated attention weight: for every (sequence, head) the last `recent` of rows [0, n_keys) of
+    k / v [B,rows,H,hd] and, of the rest, those with the largest weight [B,H,>=n_keys] (equal: the lowest index; removed keys, key_bias -1e4
+    or less, rank below all; NaN below numbers) move, in ascending order, to rows [0, budget), with their weights and biases.
+    Returns kept int32 [B,H,budget], the rows they came from.  1 <= budget <= n_keys, 0 <= recent <= budget.
+    out None: in place (weights and biases of rows [budget, n_keys) become 0); out = (k_out, v_out, weight_out, key_bias_out or None):
+    other tensors that overlap no input, rows behind budget left alone.  key_bias fp32 [B,H,>=n_keys]: per head, as heads keep different rows."""
+    if k.dim() != 4 or k.shape != v.shape:
+        raise RuntimeError("cache_evict: k and v must be [B,rows,H,hd]")
+    B, rows, H, hd = k.shape
+    if not (1 <= budget <= n_keys <= rows and 0 <= recent <= budget):
+        raise RuntimeError(f"cache_evict: n_keys={n_keys} of {rows} rows, budget={budget}, recent={recent} "
+                           "(1 <= budget <= n_keys <= rows, 0 <= recent <= budget)")
+    inplace = out is None
+    ko, vo, wo, bo = (k, v, weight, key_bias) if inplace else out
+    if (bo is None) != (key_bias is None):
+        raise RuntimeError("cache_evict: key_bias and its output come together")
+    dev = _one_device("cache_evict", k, v, weight, key_bias, ko, vo, wo, bo)
+    ldk, bsk = _strides(k, "k", H, hd)
+    ldv, bsv = _strides(v, "v", H, hd)
+    w_bs, w_hs = _per_key(weight, "weight", B, H, n_keys, True)
+    b_bs, b_hs = _per_key(key_bias, "key_bias", B, H, n_keys, True)
+    if inplace:
+        pairs = [(k, v), (k, weight), (v, weight)] + ([(key_bias, t) for t in (k, v, weight)] if key_bias is not None else [])
+        for a, b in pairs:
+            _no_overlap("cache_evict", a, b)
+        ldko, bsko, ldvo, bsvo, wo_bs, wo_hs, bo_bs, bo_hs = ldk, bsk, ldv, bsv, w_bs, w_hs, b_bs, b_hs
+    else:
+        if ko.dim() != 4 or vo.dim() != 4 or ko.shape[0] != B or vo.shape[0] != B or ko.shape[1] < budget or vo.shape[1] < budget:
+            raise RuntimeError(f"cache_evict: k_out and v_out must be [{B},>= {budget},{H},{hd}]")
+        ldko, bsko = _strides(ko, "k_out", H, hd)
+        ldvo, bsvo = _strides(vo, "v_out", H, hd)
+        wo_bs, wo_hs = _per_key(wo, "weight_out", B, H, budget, True)
+        bo_bs, bo_hs = _per_key(bo, "key_bias_out", B, H, budget, True)
+        outs = [t for t in (ko, vo, wo, bo) if t is not None]
+        for i, t in enumerate(outs):
+            _no_overlap("cache_evict", t, k, v, weight, key_bias, *outs[i + 1:])
+    with torch.cuda.device(dev):
+        kept = torch.empty((B, H, budget), dtype=torch.int32, device=dev)
+        d = L.HkCacheEvictDesc(k.data_ptr(), v.data_ptr(), ko.data_ptr(), vo.data_ptr(), weight.data_ptr(), wo.data_ptr(), _ptr(key_bias), _ptr(bo),
+                               kept.data_ptr(), B, H, hd, n_keys, budget, recent, ldk, bsk, ldv, bsv, ldko, bsko, ldvo, bsvo,
+                               w_bs, w_hs, wo_bs, wo_hs, b_bs, b_hs, bo_bs, bo_hs)
+        L.check(L.load().hk_cache_evict_bf16(C.byref(d), _stream()), "hk_cache_evict_bf16")
+    return kept
+
+
 def argmax(logits: torch.Tensor) -> torch.Tensor:
     """fp32 [rows, V] -> int64 [rows], the lowest index of the largest value."""
     _need(logits, torch.float32, "logits")

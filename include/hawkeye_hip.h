@@ -420,6 +420,95 @@ int hk_qformer_embed_gather(const float* query_tokens, const float* word_emb, co
 int hk_qformer_embed_bwd(const float* dz, const int64_t* input_ids, float* dquery, float* dword, float* dpos,
                          int32_t B, int32_t nq, int32_t Lt, int32_t d, int32_t vocab, void* stream);
 
+/* Attention of a batch whose sequences share one prefix (several questions about one clip: the same system text, video tokens
+ * and instruction, tasks/test.py:79-97, and then a question each): for every query row i of sequence b
+ *   O = softmax over the P prefix keys, all visible, and the sequence's own keys j <= i + (Nk - Nq)      (Nk >= Nq >= 1, P >= 0)
+ * The prefix's K and V exist once and are read once for the rows of all sequences.  Prompts (Nq > 1: the questions) and single tokens
+ * (Nq = 1: the decode step) alike.  bf16 in and out, fp32 softmax.
+ *   Q [B,Nq,H,hd] carries softmax_scale * log2(e); KP / VP [P,H,hd]; K / V [B,Nk,H,hd]; O [B,Nq,H,hd]: token strides ld*, batch strides
+ *   bs* in elements, head h at column h * hd.  key_bias: optional fp32, own key j of sequence b adds key_bias[b * bias_bs + j] (natural-log
+ *   units); a key whose bias is -1e4 or less (hk_qformer_key_bias's mask value, -inf) is removed: its K and V rows may hold anything.
+ *   A row that sees no key gives zeros.
+ * ws: hk_prefix_attn_ws bytes of the caller's, 16-byte aligned, for this call alone (calls in flight together need one each).
+ * Bit-reproducible: chunks are joined in index order. */
+typedef struct hk_prefix_attn_desc {
+    const void* Q;
+    const void* KP;
+    const void* VP;
+    const void* K;
+    const void* V;
+    void* O;
+    const float* key_bias;
+    void* ws;
+    size_t ws_bytes;
+    int32_t B, H, Nq, P, Nk, head_dim;
+    int64_t ldq, bsq, ldkp, ldvp, ldk, bsk, ldv, bsv, ldo, bso, bias_bs;
+} hk_prefix_attn_desc;
+int hk_prefix_attn_bf16(const hk_prefix_attn_desc* d, void* stream);
+size_t hk_prefix_attn_ws(int32_t B, int32_t H, int32_t Nq, int32_t P, int32_t Nk, int32_t head_dim); /* 0: refused shape */
+
+/* One decode step's attention (hk_decode_attn_bf16's operator) that also adds its softmax weights to what every key has collected:
+ *   p_j = softmax_j(q . k_j + bias_j) over cache rows [0, n_keys),  out = sum_j p_j v_j,  w_out[b][h][j] = w_in[b][h][j] + p_j
+ * for hk_cache_evict.  q bf16 [B, H*hd] pre-scaled, caches bf16 [B, cache_rows, H*hd], out bf16 [B, H*hd]; w_in (NULL: zeros) and w_out
+ * fp32 with strides (wi_bs, wi_hs), (wo_bs, wo_hs), may be one array; key_bias[b * bias_bs + h * bias_hs + j] optional, as in
+ * hk_prefix_attn_desc (bias_hs = 0: one row for all heads).  A sequence without a key gives zeros and adds nothing.  ws as above. */
+typedef struct hk_step_weights_desc {
+    const void* q;
+    const void* k_cache;
+    const void* v_cache;
+    const float* key_bias;
+    const float* w_in;
+    float* w_out;
+    void* out;
+    void* ws;
+    size_t ws_bytes;
+    int32_t B, H, head_dim, n_keys;
+    int64_t cache_rows, bias_bs, bias_hs, wi_bs, wi_hs, wo_bs, wo_hs;
+} hk_step_weights_desc;
+int hk_decode_attn_weights_bf16(const hk_step_weights_desc* d, void* stream);
+size_t hk_decode_attn_weights_ws(int32_t B, int32_t H, int32_t head_dim, int32_t n_keys); /* 0: refused shape */
+
+/* The attention weight every key collects from the queries of a prompt (or of a window of it), for hk_cache_evict:
+ *   w_out[b][h][j] = w_in[b][h][j] + sum over i of softmax_j(q_i . k_j + bias_j),   causal: query i sees keys <= i + (Nk - Nq)
+ * Q [B,Nq,H,hd] (carrying softmax_scale * log2(e)) and K [B,Nk,H,hd] bf16 through strides as in hk_attn_desc; weights fp32 with strides
+ * (*_bs, *_hs), w_in NULL = zeros, may be w_out; key_bias[b * bias_bs + j] as in hk_prefix_attn_desc; a query that sees no key adds nothing.
+ * ws: B * H * Nq floats of the caller's (the rows' log2 sums).  Two launches: row sums, then weights; bit-reproducible. */
+typedef struct hk_key_weights_desc {
+    const void* Q;
+    const void* K;
+    const float* key_bias;
+    const float* w_in;
+    float* w_out;
+    void* ws;
+    size_t ws_bytes;
+    int32_t B, H, Nq, Nk, head_dim, causal;
+    int64_t ldq, bsq, ldk, bsk, bias_bs, wi_bs, wi_hs, wo_bs, wo_hs;
+} hk_key_weights_desc;
+int hk_attn_key_weights_bf16(const hk_key_weights_desc* d, void* stream);
+
+/* Eviction by accumulated attention weight: for every (sequence, head) the last `recent` of n_keys cache rows and, of the rest, the
+ * budget - recent with the largest weight (equal weights: the lowest index) move, in ascending order, to rows [0, budget) of the output:
+ * their K and V pieces (head_dim values), weights and biases; kept[b][h][i] (int32, dense) = the row they come from.
+ * Removed keys (bias -1e4 or less) rank below all others, NaN weights below numbers; -0 equals 0.  0 <= recent <= budget <= n_keys, budget >= 1.
+ * The output is the input itself (every pointer and stride the same; weights and biases of rows [budget, n_keys) become 0, K and V
+ * there keep what they held) or other memory that overlaps none of it (rows behind budget are left alone).
+ * K / V [B, rows, H, hd] through strides ld*, bs*; weights [B, H, rows] through (w_bs, w_hs) in and (wo_bs, wo_hs) out; biases, which
+ * are per head here because heads keep different rows, through (b_bs, b_hs) and (bo_bs, bo_hs), or both NULL. */
+typedef struct hk_cache_evict_desc {
+    const void* K;
+    const void* V;
+    void* k_out;
+    void* v_out;
+    const float* weight;
+    float* weight_out;
+    const float* key_bias;
+    float* key_bias_out;
+    int32_t* kept;
+    int32_t B, H, head_dim, n_keys, budget, recent;
+    int64_t ldk, bsk, ldv, bsv, ldko, bsko, ldvo, bsvo, w_bs, w_hs, wo_bs, wo_hs, b_bs, b_hs, bo_bs, bo_hs;
+} hk_cache_evict_desc;
+int hk_cache_evict_bf16(const hk_cache_evict_desc* d, void* stream);
+
 /* Measurement aid, no reference counterpart (SURVEY.md §8d asks for a register-resident MFMA-peak probe):
  * `grid` workgroups of 4 waves each issue `iters` x 8 independent v_mfma_f32_16x16x32_bf16 (kind 0) or
  * `iters` x 4 v_mfma_f32_32x32x16_bf16 (kind 1) on fragments loaded once from seed_bf16_2048 (2048 bf16 values);
