@@ -16,6 +16,7 @@
 // K goes from memory straight to the A operand's registers, V through 32 keys of LDS that belong to the wave (no barrier in
 // the loop).  The next tile's K is requested as soon as this one's scores stand, its V as soon as this one's is in LDS: a
 // wave keeps about 16 KB in flight, 8 waves per CU.
+#include <type_traits>
 #include "hk_common.h"
 
 namespace {
@@ -25,18 +26,22 @@ constexpr float M_NONE = -1.0e30f;   // running maximum of a row that has met no
 constexpr int TK = 32;               // keys per tile
 constexpr int NWV = 4;               // waves per workgroup
 constexpr int MAX_CHUNK = 1024;      // keys per chunk at most: the chunk's bias lives in LDS
+#ifndef HK_PREFIX_WANT
+#define HK_PREFIX_WANT 1024          // workgroups per launch the chunks are cut for
+#endif
 
 struct PrefixParams {
     const __bf16 *Q, *KP, *VP, *K, *V;
     __bf16* O;
     const float* bias;               // own keys: bias[b * bias_bs + h * bias_hs + j]
-    float* part_o;                   // [slot][row][head][HD]
-    float* part_ml;                  // [slot][row][head][2]
+    float* part_o;                   // [row][head][slot][HD]
+    float* part_ml;                  // [row][head][slot][2]
     float* raw;                      // WEIGHTS: scores [B][H][raw_ld], raw_ld = Nk rounded up to whole tiles
     int B, H, Nq, P, Nk, R;          // R = B * Nq
     int64_t ldq, bsq, ldkp, ldvp, ldk, bsk, ldv, bsv, ldo, bso, bias_bs, bias_hs, raw_ld;
     int pc, npc, nprg;               // prefix: keys per chunk, chunks, row groups
     int oc, noc, norg;               // own keys: the same, per sequence
+    int ns;                          // slots of a row: npc + noc
     int64_t pjobs;                   // workgroups of the prefix: H * npc * nprg (below 2^31 once checked)
 };
 
@@ -299,7 +304,7 @@ __global__ __launch_bounds__(NWV * 64, 2) void hk_prefix_part_kernel(const Prefi
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[i] += a * x[i];
         }
-        const int64_t at = ((int64_t)slot * p.R + row0 + r) * p.H + head;
+        const int64_t at = ((int64_t)(row0 + r) * p.H + head) * p.ns + slot;
         *reinterpret_cast<f32x4*>(p.part_o + at * HD + 4 * c) = o;
         if (c == 0) {
             p.part_ml[at * 2] = M;
@@ -308,30 +313,392 @@ __global__ __launch_bounds__(NWV * 64, 2) void hk_prefix_part_kernel(const Prefi
     }
 }
 
-// Joins the chunks of a row: o = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), slots in index order; no key at all: zeros.
-template <int HD>
-__global__ __launch_bounds__(256) void hk_prefix_join_kernel(const PrefixParams p) {
-    constexpr int TPR = HD / 4;
-    const int64_t rh = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
-    if (rh >= (int64_t)p.R * p.H) return;
-    const int c = threadIdx.x % TPR;
-    const int row = (int)(rh / p.H), head = (int)(rh - (int64_t)row * p.H);
-    const int ns = p.npc + p.noc;
-    const int64_t step = (int64_t)p.R * p.H;
-    const float* mlp = p.part_ml + rh * 2;
-    const float* op = p.part_o + rh * HD + 4 * c;
-    float M = M_NONE;
-    for (int s = 0; s < ns; ++s) M = fmaxf(M, mlp[s * step * 2]);
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    float l = 0.f;
-    for (int s = 0; s < ns; ++s) {
-        const float a = __builtin_amdgcn_exp2f(mlp[s * step * 2] - M);
-        const f32x4 x = *reinterpret_cast<const f32x4*>(op + s * step * HD);
-        l += a * mlp[s * step * 2 + 1];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] += a * x[i];
+// ---------------------------------------------------------------- many rows
+// hk_prefix_rows_kernel: a workgroup = 128 query rows of one head (four waves of 32) that share 64-key tiles in LDS (two stages,
+// LDS-DMA one tile ahead, two workgroups per CU).  With 32 rows per wave the matrix instructions, not memory, are the bound:
+// v_mfma_f32_32x32x16_bf16, transposed as above (lane -> row lane & 31; the S^T accumulator is the B operand of O^T += V^T . P^T).
+// The running maximum enters as the first instruction's accumulator and is taken again only when a tile's partial row sum leaves
+// [0, 2^20] (that tile is redone): the common path is exp2 and an addition per score.  A row that has met no key yet takes the
+// maximum of every tile until it does.
+// Rows are a sequence's (its keys: the prefix, then its own up to the diagonal; or its own alone) or, for the prefix alone, rows of
+// all sequences packed: whichever leaves fewer 128-row blocks part empty (make_plan).
+struct RowsParams {
+    int packed;                      // prefix by packed row blocks and key chunks, own keys apart; else both in one workgroup
+    int npb, nob;                    // row blocks: of all rows (packed prefix), of a sequence
+    int64_t pjobs;                   // packed: workgroups of the prefix = npb * npc * H
+};
+
+constexpr int RB = 128;
+constexpr int KT = 64;
+constexpr float OVERFLOW_SUM = 1048576.0f;
+
+__device__ __forceinline__ float half_max(float x) {    // the larger of the two lane halves' values (rows live on lane & 31)
+    float a = x, b = x;
+    asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+    return fmaxf(a, b);
+}
+
+template <int HD, bool BIAS>
+__global__ __launch_bounds__(256, 2) void hk_prefix_rows_kernel(const PrefixParams p, const RowsParams q) {
+    constexpr int ROWB = HD * 2, CH = HD / 8, NKS = HD / 16, NDT = HD / 32;
+    constexpr int STAGE = 2 * KT * ROWB;
+    constexpr int RPP = 256 / CH;                          // key rows one workgroup-wide LDS-DMA covers
+    constexpr int NP = KT / RPP;                           // of them per operand and tile
+    extern __shared__ __attribute__((aligned(16))) char smem[];      // [2][K | V][64 keys][ROWB], then [2][64] biases
+    float* blds = reinterpret_cast<float*>(smem + 2 * STAGE);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 31, h = lane >> 5;
+
+    // ---- which rows, which keys (blockIdx = ... * H + head: the row blocks of a head share an XCD's L2 where H is a multiple of 8) ----
+    const int head = blockIdx.x % p.H;
+    int rest = blockIdx.x / p.H;
+    int row0, nrows, a0 = 0, a1 = 0, k1 = 0, slot = -1, brow = 0, b0 = 0;
+    int off = 0x3fffffff;                                  // row i of the block sees own keys <= i + off
+    if (q.packed && blockIdx.x < q.pjobs) {
+        const int rb = rest % q.npb;
+        slot = rest / q.npb;
+        row0 = rb * RB;
+        nrows = min(RB, p.R - row0);
+        a0 = slot * p.pc;
+        a1 = min(a0 + p.pc, p.P);
+    } else {
+        if (q.packed) {
+            rest -= (int)(q.pjobs / p.H);
+            slot = p.npc;
+        } else {
+            a1 = p.P;
+        }
+        brow = rest % p.B;
+        rest /= p.B;
+        const int rb = q.nob - 1 - rest % q.nob;           // longest first
+        const int c = rest / q.nob;                        // packed: the own keys' chunk
+        if (q.packed) {
+            slot += c;
+            b0 = c * p.oc;
+        }
+        const int i0 = rb * RB;
+        row0 = brow * p.Nq + i0;
+        nrows = min(RB, p.Nq - i0);
+        off = i0 + p.Nk - p.Nq - b0;                       // own keys are counted from the chunk's first
+        k1 = max(0, min(q.packed ? min(p.oc, p.Nk - b0) : p.Nk, off + nrows));
     }
-    const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);      // l NaN stays NaN
+    const int nA = (a1 - a0 + KT - 1) / KT, NT = nA + (k1 + KT - 1) / KT;
+    const int q0 = wave * 32;                              // the wave's first row within the block
+    const bool active = q0 < nrows;
+
+    bf16x8 qf[NKS];
+    {
+        const int row = row0 + min(q0 + r, nrows - 1);
+        const int b = row / p.Nq, i = row - b * p.Nq;
+        const __bf16* qp = p.Q + (int64_t)b * p.bsq + (int64_t)i * p.ldq + head * HD + 8 * h;
+#pragma unroll
+        for (int s = 0; s < NKS; ++s) qf[s] = *reinterpret_cast<const bf16x8*>(qp + 16 * s);
+    }
+    const __bf16* kA = p.KP + (int64_t)a0 * p.ldkp + head * HD;
+    const __bf16* vA = p.VP + (int64_t)a0 * p.ldvp + head * HD;
+    const __bf16* kB = p.K + (int64_t)brow * p.bsk + (int64_t)b0 * p.ldk + head * HD;
+    const __bf16* vB = p.V + (int64_t)brow * p.bsv + (int64_t)b0 * p.ldv + head * HD;
+    const float* bias = BIAS ? p.bias + (int64_t)brow * p.bias_bs + (int64_t)head * p.bias_hs + b0 : nullptr;
+
+    // K: 16-byte chunk c of key row x at c ^ swk(x): 16 rows x one chunk touch every bank once; V: at c ^ swv(x): so do the 8 key rows of a
+    // transposing read
+    auto swk = [](int x) { return HD == 128 ? x & 15 : (x >> 1) & 7; };
+    auto swv = [](int x) { return HD == 128 ? (x & 7) << 1 : ((x >> 1) & 1) << 2; };
+    const int lrow = tid / CH, lch = tid % CH;
+    float br = 0.f;
+    auto issue = [&](int t, int stage) __attribute__((always_inline)) {
+        const bool own = t >= nA;
+        const int kt = (own ? t - nA : t) * KT;
+        const int n = own ? k1 : a1 - a0;
+        const int64_t ldk = own ? p.ldk : p.ldkp, ldv = own ? p.ldv : p.ldvp;
+        const __bf16* kb = own ? kB : kA;
+        const __bf16* vb = own ? vB : vA;
+        char* ks = smem + stage * STAGE + wave * (64 / CH) * ROWB;
+        char* vs = ks + KT * ROWB;
+        // the swizzle goes on the source chunk (the LDS image is lane-linear); RPP is a multiple of every swizzle's period
+        const uint32_t kl = (uint32_t)((lrow * ldk + (lch ^ swk(lrow)) * 8) * 2);
+        const uint32_t vl = (uint32_t)((lrow * ldv + (lch ^ swv(lrow)) * 8) * 2);
+        if (kt + KT <= n) {
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                glds16_s(kb + (int64_t)(kt + i * RPP) * ldk, kl, ks + i * RPP * ROWB);
+                glds16_s(vb + (int64_t)(kt + i * RPP) * ldv, vl, vs + i * RPP * ROWB);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const int64_t key = min(kt + i * RPP + lrow, n - 1);
+                glds16_v(kb + key * ldk + (lch ^ swk(lrow)) * 8, ks + i * RPP * ROWB);
+                glds16_v(vb + key * ldv + (lch ^ swv(lrow)) * 8, vs + i * RPP * ROWB);
+            }
+        }
+        if (BIAS && own && tid < KT) br = bias[min(kt + tid, k1 - 1)];
+    };
+    // K fragment (g, s): row 32 g + r, chunk 2 s + h; V fragment (s, d): rows 16 s + vrow (and + 8), dims 32 d + 16 ((lane >> 4) & 1) + ...:
+    // chunk numbers are joined to the swizzle by exclusive or, so one register per operand holds every offset
+    const int vrow = 4 * h + ((lane & 15) >> 2);
+    const int koff0 = r * ROWB + ((h ^ swk(r)) << 4);
+    const int voff0 = vrow * ROWB + (((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ swv(vrow)) << 4) + 8 * (lane & 1);
+
+    f32x16 ot[NDT];
+#pragma unroll
+    for (int d = 0; d < NDT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) ot[d][i] = 0.f;
+    float m = 0.f, l = 0.f;                                // everything stored is relative to m
+    bool unset = true, pending = true;                     // this row / some row of the wave has met no key yet
+
+    auto tile = [&](const int t, auto cur_c) __attribute__((always_inline)) {
+        constexpr int cur = decltype(cur_c)::value;
+        if (t + 1 < NT) issue(t + 1, cur ^ 1);
+        const bool own = t >= nA;
+        const int kt = (own ? t - nA : t) * KT, n = own ? k1 : a1 - a0;
+        if (active && (!own || kt <= q0 + 31 + off)) {
+            int ko = koff0, vo = voff0;
+            asm volatile("" : "+v"(ko), "+v"(vo));          // the offsets are made from these here, not kept across tiles in registers
+            const char* ks = smem + cur * STAGE;
+            const char* vs = ks + KT * ROWB;
+            uint64_t gone = 0;                             // keys of this tile that no row has
+            if (BIAS && own) gone = __builtin_amdgcn_ballot_w64(kt + lane >= n || blds[cur * KT + lane] <= REMOVED);
+            const bool edge = kt + KT > n || (own && kt + KT - 1 > q0 + off);
+            f32x16 st[2];
+            auto scores = [&]() __attribute__((always_inline)) {
+                __builtin_amdgcn_s_setprio(1);
+                f32x16 c0;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) c0[i] = -m;
+#pragma unroll
+                for (int g = 0; g < 2; ++g)
+#pragma unroll
+                    for (int s = 0; s < NKS; ++s) {
+                        const bf16x8 kf = *reinterpret_cast<const bf16x8*>(ks + g * 32 * ROWB + (ko ^ (32 * s)));
+                        st[g] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[s], s == 0 ? c0 : st[g], 0, 0, 0);
+                    }
+                __builtin_amdgcn_s_setprio(0);
+                if (BIAS && own) {                         // register 4 x + j of st[g] <-> key 32 g + 8 x + 4 h + j
+#pragma unroll
+                    for (int g = 0; g < 2; ++g)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const f32x4 bv = *reinterpret_cast<const f32x4*>(blds + cur * KT + 32 * g + 8 * x + 4 * h);
+                            const uint32_t gb = (uint32_t)(gone >> (32 * g + 8 * x)) >> (4 * h);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) st[g][4 * x + j] = (gb >> j) & 1 ? -INFINITY : st[g][4 * x + j] + bv[j] * HK_LOG2E;
+                        }
+                }
+                if (edge) {
+                    const int lim = min(n - 1, own ? q0 + r + off : n - 1) - kt - 4 * h;
+#pragma unroll
+                    for (int g = 0; g < 2; ++g)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (32 * g + (i & 3) + 8 * (i >> 2) > lim) st[g][i] = -INFINITY;
+                }
+            };
+            float rs;
+            auto exp_sum = [&]() __attribute__((always_inline)) {
+                rs = 0.f;
+#pragma unroll
+                for (int g = 0; g < 2; ++g)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float e = __builtin_amdgcn_exp2f(st[g][i]);
+                        st[g][i] = e;
+                        rs += e;
+                    }
+            };
+            auto move_max = [&]() __attribute__((always_inline)) {
+                float mx = fmaxf(st[0][0], st[1][0]);
+#pragma unroll
+                for (int i = 1; i < 16; ++i) mx = fmaxf(mx, fmaxf(st[0][i], st[1][i]));
+                mx = half_max(mx);
+                const float delta = unset ? (mx == -INFINITY ? 0.f : mx) : fmaxf(mx, 0.f);
+                const float a = unset ? 0.f : __builtin_amdgcn_exp2f(-delta);
+                unset = unset && mx == -INFINITY;
+                pending = __builtin_amdgcn_ballot_w64(unset) != 0;
+                m += delta;
+                l *= a;
+#pragma unroll
+                for (int d = 0; d < NDT; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) ot[d][i] *= a;
+#pragma unroll
+                for (int g = 0; g < 2; ++g)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) st[g][i] -= delta;
+            };
+            for (bool take = pending;; take = true) {      // at most twice
+                scores();
+                if (take) move_max();
+                exp_sum();
+                if (take || __builtin_amdgcn_ballot_w64(!(rs <= OVERFLOW_SUM)) == 0) break;
+            }
+            l += rs;
+            __builtin_amdgcn_s_setprio(2);
+            bf16x8 pf[4];                                  // P in bf16, the matrix instruction's operand; l sums the unrounded values
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                u32x4 w;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(st[s >> 1][8 * (s & 1) + 2 * j], st[s >> 1][8 * (s & 1) + 2 * j + 1]);
+                pf[s] = __builtin_bit_cast(bf16x8, w);
+            }
+            auto pv = [&](auto masked_c) __attribute__((always_inline)) {
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    u32x4 keep = {~0u, ~0u, ~0u, ~0u};
+                    if (decltype(masked_c)::value) {       // elements 0-3: keys 16 s + 4 h + j, elements 4-7: 8 further
+                        const uint32_t g = (uint32_t)(gone >> (16 * s)) >> (4 * h);
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            keep[j] = ((g >> (2 * j)) & 1 ? 0u : 0xffffu) | ((g >> (2 * j + 1)) & 1 ? 0u : 0xffff0000u);
+                            keep[j + 2] = ((g >> (8 + 2 * j)) & 1 ? 0u : 0xffffu) | ((g >> (8 + 2 * j + 1)) & 1 ? 0u : 0xffff0000u);
+                        }
+                    }
+#pragma unroll
+                    for (int d = 0; d < NDT; ++d) {
+                        const char* vp = vs + s * 16 * ROWB + (vo ^ (64 * d));
+                        const bf16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(vp));
+                        const bf16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(vp + 8 * ROWB));
+                        bf16x8 vf;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            vf[j] = v0[j];
+                            vf[j + 4] = v1[j];
+                        }
+                        if (decltype(masked_c)::value) vf = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, vf) & keep);
+                        ot[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[s], ot[d], 0, 0, 0);
+                    }
+                }
+            };
+            if (BIAS && gone) pv(std::true_type{});
+            else pv(std::false_type{});
+            __builtin_amdgcn_s_setprio(0);
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the next tile's LDS-DMA, unknown to the compiler
+        if (BIAS && t + 1 >= nA && t + 1 < NT && tid < KT) blds[(cur ^ 1) * KT + tid] = br;
+        __syncthreads();
+    };
+
+    if (NT > 0) {
+        issue(0, 0);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (BIAS && nA == 0 && tid < KT) blds[tid] = br;
+        __syncthreads();
+    }
+    int t = 0;
+    for (; t + 1 < NT; t += 2) {
+        tile(t, std::integral_constant<int, 0>{});
+        tile(t + 1, std::integral_constant<int, 1>{});
+    }
+    if (t < NT) tile(t, std::integral_constant<int, 0>{});
+
+    l += __shfl_xor(l, 32, 64);
+    if (q0 + r >= nrows) return;
+    const int row = row0 + q0 + r;
+    if (slot >= 0) {                                       // register 4 x + j of ot[d] <-> dim 32 d + 8 x + 4 h + j
+        const int64_t at = ((int64_t)row * p.H + head) * p.ns + slot;
+#pragma unroll
+        for (int d = 0; d < NDT; ++d)
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+                *reinterpret_cast<f32x4*>(p.part_o + at * HD + 32 * d + 8 * x + 4 * h) =
+                    f32x4{ot[d][4 * x], ot[d][4 * x + 1], ot[d][4 * x + 2], ot[d][4 * x + 3]};
+        if (h == 0) {
+            p.part_ml[at * 2] = unset ? M_NONE : m;
+            p.part_ml[at * 2 + 1] = l;
+        }
+    } else {
+        const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
+        const int b = row / p.Nq, i = row - b * p.Nq;
+        __bf16* op = p.O + (int64_t)b * p.bso + (int64_t)i * p.ldo + head * HD + 4 * h;
+#pragma unroll
+        for (int d = 0; d < NDT; ++d)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                u32x2 w;
+                w[0] = pack_bf16x2(ot[d][4 * x] * inv, ot[d][4 * x + 1] * inv);
+                w[1] = pack_bf16x2(ot[d][4 * x + 2] * inv, ot[d][4 * x + 3] * inv);
+                *reinterpret_cast<u32x2*>(op + 32 * d + 8 * x) = w;
+            }
+    }
+}
+
+// ---------------------------------------------------------------- joining the chunks
+// One thread group's share of a row's slots (s0, s0 + SG, ...): running (M, l, o) in one pass over (m, l, o) of the slots.
+template <int HD, int SG>
+__device__ __forceinline__ void join_share(const float* mlp, const float* op, int s0, int ns, float& M, float& l, f32x4& o) {
+    M = M_NONE;
+    l = 0.f;
+    o = f32x4{0.f, 0.f, 0.f, 0.f};
+    constexpr int U = 4;                                   // slots in flight
+    for (int s = s0; s < ns; s += U * SG) {
+        float ms[U], ls[U];
+        f32x4 x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int at = min(s + u * SG, ns - 1);
+            ms[u] = s + u * SG < ns ? mlp[2 * at] : M_NONE;
+            ls[u] = s + u * SG < ns ? mlp[2 * at + 1] : 0.f;
+            x[u] = *reinterpret_cast<const f32x4*>(op + (int64_t)at * HD);
+        }
+        float mn = M;
+#pragma unroll
+        for (int u = 0; u < U; ++u) mn = fmaxf(mn, ms[u]);
+        float a = __builtin_amdgcn_exp2f(M - mn);
+        M = mn;
+        l *= a;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] *= a;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            a = s + u * SG < ns ? __builtin_amdgcn_exp2f(ms[u] - M) : 0.f;
+            l += a * ls[u];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] += s + u * SG < ns ? a * x[u][i] : 0.f;
+        }
+    }
+}
+__device__ __forceinline__ float inverse_sum(float l) { return l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l); }     // no key: 0; NaN stays
+
+// o = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), no key at all: zeros.  HD / 4 threads per row and slot group (four dims each),
+// SG groups per row, joined in group order.
+template <int HD, int SG>
+__global__ __launch_bounds__(256) void hk_prefix_join_kernel(const PrefixParams p) {
+    constexpr int TPR = HD / 4, RPB = 256 / (TPR * SG);
+    __shared__ float ml[RPB * SG][2];
+    __shared__ __attribute__((aligned(16))) float os[RPB * SG][HD];
+    const int c = threadIdx.x % TPR, g = threadIdx.x / TPR, rl = g / SG;
+    const int64_t rh = (int64_t)blockIdx.x * RPB + rl;
+    const bool in = rh < (int64_t)p.R * p.H;
+    const int64_t at = (in ? rh : 0) * p.ns;
+    float M, l;
+    f32x4 o;
+    join_share<HD, SG>(p.part_ml + at * 2, p.part_o + at * HD + 4 * c, g % SG, p.ns, M, l, o);
+    if (SG > 1) {
+        if (c == 0) {
+            ml[g][0] = M;
+            ml[g][1] = l;
+        }
+        *reinterpret_cast<f32x4*>(&os[g][4 * c]) = o;
+        __syncthreads();
+        if (g % SG) return;
+        M = M_NONE;
+#pragma unroll
+        for (int x = 0; x < SG; ++x) M = fmaxf(M, ml[g + x][0]);
+        l = 0.f;
+        o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < SG; ++x) {
+            const float a = __builtin_amdgcn_exp2f(ml[g + x][0] - M);
+            l += a * ml[g + x][1];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] += a * os[g + x][4 * c + i];
+        }
+    }
+    if (!in) return;
+    const float inv = inverse_sum(l);
+    const int row = (int)(rh / p.H), head = (int)(rh - (int64_t)row * p.H);
     const int b = row / p.Nq, i = row - b * p.Nq;
     u32x2 w;
     w[0] = pack_bf16x2(o[0] * inv, o[1] * inv);
@@ -339,7 +706,8 @@ __global__ __launch_bounds__(256) void hk_prefix_join_kernel(const PrefixParams 
     *reinterpret_cast<u32x2*>(p.O + (int64_t)b * p.bso + (int64_t)i * p.ldo + head * HD + 4 * c) = w;
 }
 
-// The same for one decode step, and its weights: w_out[j] = w_in[j] + 2^(s_j - M) / l from the scores the first launch left.
+// The same for one decode step, and its weights: w_out[j] = w_in[j] + 2^(s_j - M) / l from the scores the first launch left.  One workgroup
+// per (sequence, head) and 2048 keys; all its groups share the slots.
 struct StepWeights {
     const float* w_in;               // may be w_out; NULL = zeros
     float* w_out;
@@ -347,26 +715,39 @@ struct StepWeights {
 };
 template <int HD>
 __global__ __launch_bounds__(256) void hk_step_join_kernel(const PrefixParams p, const StepWeights sw) {
-    constexpr int TPR = HD / 4;
-    const int head = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
-    const int64_t rh = (int64_t)b * p.H + head, step = (int64_t)p.R * p.H;
-    const float* mlp = p.part_ml + rh * 2;
-    float M = M_NONE, l = 0.f;
-    for (int s = 0; s < p.noc; ++s) M = fmaxf(M, mlp[s * step * 2]);
-    for (int s = 0; s < p.noc; ++s) l += mlp[s * step * 2 + 1] * __builtin_amdgcn_exp2f(mlp[s * step * 2] - M);
-    const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
-    if (blockIdx.z == 0 && tid < TPR) {
-        f32x4 o = {0.f, 0.f, 0.f, 0.f};
-        for (int s = 0; s < p.noc; ++s) {
-            const float a = __builtin_amdgcn_exp2f(mlp[s * step * 2] - M);
-            const f32x4 x = *reinterpret_cast<const f32x4*>(p.part_o + (rh + s * step) * HD + 4 * tid);
+    constexpr int TPR = HD / 4, SG = 256 / TPR;
+    __shared__ float ml[SG][2];
+    __shared__ __attribute__((aligned(16))) float os[SG][HD];
+    const int head = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, c = tid % TPR, g = tid / TPR;
+    const int64_t rh = (int64_t)b * p.H + head, at = rh * p.ns;
+    float M, l;
+    f32x4 o;
+    join_share<HD, SG>(p.part_ml + at * 2, p.part_o + at * HD + 4 * c, g, p.ns, M, l, o);
+    if (c == 0) {
+        ml[g][0] = M;
+        ml[g][1] = l;
+    }
+    *reinterpret_cast<f32x4*>(&os[g][4 * c]) = o;
+    __syncthreads();
+    M = M_NONE;
+    l = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] += a * x[i];
+    for (int x = 0; x < SG; ++x) M = fmaxf(M, ml[x][0]);
+#pragma unroll
+    for (int x = 0; x < SG; ++x) l += __builtin_amdgcn_exp2f(ml[x][0] - M) * ml[x][1];
+    const float inv = inverse_sum(l);
+    if (blockIdx.z == 0 && g == 0) {
+        o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < SG; ++x) {
+            const float a = __builtin_amdgcn_exp2f(ml[x][0] - M);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] += a * os[x][4 * c + i];
         }
         u32x2 w;
         w[0] = pack_bf16x2(o[0] * inv, o[1] * inv);
         w[1] = pack_bf16x2(o[2] * inv, o[3] * inv);
-        *reinterpret_cast<u32x2*>(p.O + (int64_t)b * p.bso + head * HD + 4 * tid) = w;
+        *reinterpret_cast<u32x2*>(p.O + (int64_t)b * p.bso + head * HD + 4 * c) = w;
     }
     const float* rp = p.raw + rh * p.raw_ld;
     const float* wi = sw.w_in ? sw.w_in + (int64_t)b * sw.wi_bs + (int64_t)head * sw.wi_hs : nullptr;
@@ -375,59 +756,118 @@ __global__ __launch_bounds__(256) void hk_step_join_kernel(const PrefixParams p,
         wo[j] = (wi ? wi[j] : 0.f) + __builtin_amdgcn_exp2f(rp[j] - M) * inv;
 }
 
-// How the keys are cut: the whole chip wants about `want` workgroups, a chunk is whole 128-key rounds of the four waves.
-int cut(int keys, long rows_x_heads, long want, int* chunk) {
-    if (keys <= 0) {
-        *chunk = NWV * TK;
-        return 0;
-    }
-    long n = want / (rows_x_heads < 1 ? 1 : rows_x_heads);
+// ---------------------------------------------------------------- host side
+enum { SMALL, MIXED, PACKED, FUSED };
+struct Plan {
+    int mode, rt;
+    RowsParams rows;
+};
+
+// n chunks of `keys` such that `per` workgroups each come to about `want`; a chunk is whole multiples of `unit`, at most `most` keys.
+int cut(int keys, int64_t per, int64_t want, int unit, int most, int* chunk) {
+    *chunk = unit;
+    if (keys <= 0) return 0;
+    int64_t n = want / (per < 1 ? 1 : per);
     if (n < 1) n = 1;
-    long c = (keys + n - 1) / n;
-    c = (c + NWV * TK - 1) / (NWV * TK) * (NWV * TK);
-    if (c > MAX_CHUNK) c = MAX_CHUNK;
+    int64_t c = (keys + n - 1) / n;
+    c = (c + unit - 1) / unit * unit;
+    if (c > most) c = most;
     *chunk = (int)c;
     return (int)((keys + c - 1) / c);
 }
 
-int plan(PrefixParams& p, int rt) {
-    const long want = 1024;
+// Which kernel takes what.  Up to 32 queries per sequence, own keys are bound by reading them: hk_prefix_part_kernel.  So is the prefix up to 64
+// rows in all; beyond, its rows fill 128-row blocks (MIXED).  More queries: hk_prefix_rows_kernel for both, in one workgroup (FUSED) or apart
+// (PACKED), whichever the estimate below finds shorter.
+Plan make_plan(PrefixParams& p, int hd, bool raw) {
+    Plan m = {};
     p.R = p.B * p.Nq;
-    p.nprg = (p.R + rt * 16 - 1) / (rt * 16);
-    p.norg = (p.Nq + rt * 16 - 1) / (rt * 16);
-    p.npc = cut(p.P, (long)p.H * p.nprg, want, &p.pc);
-    p.noc = cut(p.Nk, (long)p.B * p.H * p.norg, want, &p.oc);
-    p.pjobs = (int64_t)p.H * p.npc * p.nprg;
-    return p.npc + p.noc;
+    m.rt = !raw && (p.Nq > 16 || (p.P > 0 && p.R > 16)) ? 2 : 1;
+    m.rows.npb = (p.R + RB - 1) / RB;
+    m.rows.nob = (p.Nq + RB - 1) / RB;
+    p.nprg = (p.R + m.rt * 16 - 1) / (m.rt * 16);
+    p.norg = (p.Nq + m.rt * 16 - 1) / (m.rt * 16);
+    const int64_t H = p.H, B = p.B;
+    const int all = 1 << 28;
+    if (p.Nq <= 32) {
+        m.mode = p.R > 64 && p.P > 0 ? MIXED : SMALL;
+        if (m.mode == SMALL) p.npc = cut(p.P, H * p.nprg, HK_PREFIX_WANT, NWV * TK, MAX_CHUNK, &p.pc);
+        else p.npc = cut(p.P, H * m.rows.npb, 512, KT, all, &p.pc);
+        p.noc = cut(p.Nk, B * H * p.norg, HK_PREFIX_WANT, NWV * TK, MAX_CHUNK, &p.oc);
+    } else {
+        // time of a 128-row x 64-key tile when 512 workgroups (two per CU) run: about 1 us; a lone workgroup's is not much shorter
+        p.npc = cut(p.P, H * m.rows.npb, 512, KT, all, &p.pc);
+        p.noc = cut(p.Nk, H * B * m.rows.nob, 512, KT, all, &p.oc);
+        const double own = (double)H * B * m.rows.nob * ((p.Nk + KT - 1) / KT), pre = (double)((p.P + KT - 1) / KT);
+        const double fused_n = (double)H * B * m.rows.nob;
+        double fused = (own + fused_n * pre) / (fused_n < 512 ? fused_n : 512);
+        const double packed_n = (double)H * m.rows.npb * p.npc + (double)H * B * m.rows.nob * p.noc;
+        double packed = (own + (double)H * m.rows.npb * pre) / (packed_n < 512 ? packed_n : 512);
+        packed += 4.0 + (double)p.R * H * (p.npc + p.noc) * hd * 8 / 4.5e6;      // the join: a launch, partial sums written and read at 4.5 TB/s
+        m.mode = p.P > 0 && packed < fused ? PACKED : FUSED;
+        if (p.P == 0 && packed < fused && p.noc > 1) m.mode = PACKED;
+    }
+    m.rows.packed = m.mode != FUSED;
+    m.rows.pjobs = m.mode == MIXED || m.mode == PACKED ? H * m.rows.npb * p.npc : 0;
+    p.pjobs = m.mode == SMALL ? H * p.npc * p.nprg : 0;
+    p.ns = m.mode == FUSED ? 0 : p.npc + p.noc;
+    return m;
 }
-
-int rows_tiles(int B, int Nq) { return B * Nq > 16 && Nq > 1 ? 2 : (B > 16 ? 2 : 1); }
 
 size_t up16(size_t x) { return (x + 15) / 16 * 16; }
-size_t part_bytes(const PrefixParams& p, int hd, int slots) {
-    return up16((size_t)slots * p.R * p.H * hd * 4) + up16((size_t)slots * p.R * p.H * 8);
+size_t part_bytes(const PrefixParams& p, int hd) {
+    return p.ns == 0 ? 16 : up16((size_t)p.ns * p.R * p.H * hd * 4) + up16((size_t)p.ns * p.R * p.H * 8);
 }
-void set_parts(PrefixParams& p, void* ws, int hd, int slots) {
+void set_parts(PrefixParams& p, void* ws, int hd) {
     p.part_o = reinterpret_cast<float*>(ws);
-    p.part_ml = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + up16((size_t)slots * p.R * p.H * hd * 4));
+    p.part_ml = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + up16((size_t)p.ns * p.R * p.H * hd * 4));
+}
+int64_t part_grid(const PrefixParams& p) { return p.pjobs + (int64_t)p.B * p.noc * p.H * p.norg; }
+int64_t rows_grid(const PrefixParams& p, const Plan& m) {
+    const int64_t own = (int64_t)p.B * m.rows.nob * p.H;
+    return m.mode == MIXED ? m.rows.pjobs : m.mode == PACKED ? m.rows.pjobs + own * p.noc : own;
 }
 
 template <int HD, int RT, bool BIAS, bool RAW>
 void launch_part(const PrefixParams& p, hipStream_t s) {
-    const int64_t grid = p.pjobs + (int64_t)p.B * p.noc * p.H * p.norg;
-    hipLaunchKernelGGL((hk_prefix_part_kernel<HD, RT, BIAS, RAW>), dim3((unsigned)grid), dim3(NWV * 64), 0, s, p);
+    hipLaunchKernelGGL((hk_prefix_part_kernel<HD, RT, BIAS, RAW>), dim3((unsigned)part_grid(p)), dim3(NWV * 64), 0, s, p);
+}
+template <int HD, bool BIAS>
+int launch_rows(const PrefixParams& p, const Plan& m, hipStream_t s) {
+    constexpr int LDS = 2 * 2 * KT * HD * 2 + (BIAS ? 2 * KT * 4 : 0);
+    static std::atomic<unsigned long long> attr_done{0};   // per device
+    const hipError_t e = hk_lds_attr_once(attr_done, reinterpret_cast<const void*>(&hk_prefix_rows_kernel<HD, BIAS>), LDS);
+    if (e != hipSuccess) {
+        hk_set_error("hk_prefix_attn_bf16: hipFuncSetAttribute(%d B LDS): %s", LDS, hipGetErrorString(e));
+        return HK_ELAUNCH;
+    }
+    hipLaunchKernelGGL((hk_prefix_rows_kernel<HD, BIAS>), dim3((unsigned)rows_grid(p, m)), dim3(256), LDS, s, p, m.rows);
+    return HK_OK;
+}
+template <int HD, int SG>
+void launch_join(const PrefixParams& p, hipStream_t s) {
+    const int64_t rh = (int64_t)p.R * p.H, per = 256 / (HD / 4 * SG);
+    hipLaunchKernelGGL((hk_prefix_join_kernel<HD, SG>), dim3((unsigned)((rh + per - 1) / per)), dim3(256), 0, s, p);
 }
 template <int HD>
-void launch_prefix(const PrefixParams& p, int rt, hipStream_t s) {
-    if (rt == 2) {
-        if (p.bias) launch_part<HD, 2, true, false>(p, s);
-        else launch_part<HD, 2, false, false>(p, s);
-    } else {
-        if (p.bias) launch_part<HD, 1, true, false>(p, s);
-        else launch_part<HD, 1, false, false>(p, s);
+int launch_prefix(const PrefixParams& p, const Plan& m, hipStream_t s) {
+    if (m.mode != SMALL) {
+        // MIXED: the rows kernel reads the prefix only, which has no bias
+        const int rc = p.bias && m.mode != MIXED ? launch_rows<HD, true>(p, m, s) : launch_rows<HD, false>(p, m, s);
+        if (rc != HK_OK || m.mode == FUSED) return rc;
     }
-    const int64_t rh = (int64_t)p.R * p.H, per = 256 / (HD / 4);
-    hipLaunchKernelGGL((hk_prefix_join_kernel<HD>), dim3((unsigned)((rh + per - 1) / per)), dim3(256), 0, s, p);
+    if (m.mode != PACKED) {
+        if (m.rt == 2) {
+            if (p.bias) launch_part<HD, 2, true, false>(p, s);
+            else launch_part<HD, 2, false, false>(p, s);
+        } else {
+            if (p.bias) launch_part<HD, 1, true, false>(p, s);
+            else launch_part<HD, 1, false, false>(p, s);
+        }
+    }
+    if (p.ns <= 4) launch_join<HD, 1>(p, s);
+    else launch_join<HD, 4>(p, s);
+    return HK_OK;
 }
 template <int HD>
 void launch_step(const PrefixParams& p, const StepWeights& sw, hipStream_t s) {
@@ -452,8 +892,8 @@ extern "C" size_t hk_prefix_attn_ws(int32_t B, int32_t H, int32_t Nq, int32_t P,
     p.Nq = Nq;
     p.P = P;
     p.Nk = Nk;
-    const int slots = plan(p, rows_tiles(B, Nq));
-    return part_bytes(p, head_dim, slots);
+    make_plan(p, head_dim, false);
+    return part_bytes(p, head_dim);
 }
 
 extern "C" int hk_prefix_attn_bf16(const hk_prefix_attn_desc* d, void* stream) {
@@ -465,6 +905,8 @@ extern "C" int hk_prefix_attn_bf16(const hk_prefix_attn_desc* d, void* stream) {
     const int64_t row = (int64_t)d->H * d->head_dim;
     HK_REQUIRE(((d->ldq | d->bsq | d->ldkp | d->ldvp | d->ldk | d->bsk | d->ldv | d->bsv) & 7) == 0 && ((d->ldo | d->bso) & 3) == 0,
                "hk_prefix_attn_bf16: strides must keep 16-byte rows (8 elements; 4 for the output)");
+    HK_REQUIRE(d->ldkp < (1 << 25) && d->ldvp < (1 << 25) && d->ldk < (1 << 25) && d->ldv < (1 << 25),
+               "hk_prefix_attn_bf16: token strides of 2^25 elements and more are not supported");
     HK_REQUIRE(d->ldq >= 0 && d->ldkp >= 0 && d->ldvp >= 0 && d->ldk >= 0 && d->ldv >= 0 && d->bsq >= 0 && d->bsk >= 0 && d->bsv >= 0 &&
                    (d->Nq == 1 || d->ldo >= row) && (d->B == 1 || d->bso >= row) && d->bias_bs >= 0,
                "hk_prefix_attn_bf16: strides must not be negative, output rows must not overlap");
@@ -495,16 +937,15 @@ extern "C" int hk_prefix_attn_bf16(const hk_prefix_attn_desc* d, void* stream) {
     p.ldo = d->ldo;
     p.bso = d->bso;
     p.bias_bs = d->bias_bs;
-    const int rt = rows_tiles(p.B, p.Nq);
-    const int slots = plan(p, rt);
-    HK_REQUIRE(d->ws && d->ws_bytes >= part_bytes(p, d->head_dim, slots),
+    const Plan m = make_plan(p, d->head_dim, false);
+    HK_REQUIRE(d->ws && d->ws_bytes >= part_bytes(p, d->head_dim),
                "hk_prefix_attn_bf16: workspace of %zu bytes, %zu needed (hk_prefix_attn_ws)", d->ws ? d->ws_bytes : (size_t)0,
-               part_bytes(p, d->head_dim, slots));
-    HK_REQUIRE(p.pjobs + (int64_t)p.B * p.noc * p.H * p.norg < (1LL << 31), "hk_prefix_attn_bf16: grid too large");
-    set_parts(p, d->ws, d->head_dim, slots);
+               part_bytes(p, d->head_dim));
+    HK_REQUIRE(part_grid(p) < (1LL << 31) && rows_grid(p, m) < (1LL << 31), "hk_prefix_attn_bf16: grid too large");
+    set_parts(p, d->ws, d->head_dim);
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    if (d->head_dim == 128) launch_prefix<128>(p, rt, s);
-    else launch_prefix<64>(p, rt, s);
+    const int rc = d->head_dim == 128 ? launch_prefix<128>(p, m, s) : launch_prefix<64>(p, m, s);
+    if (rc != HK_OK) return rc;
     HK_CHECK_LAUNCH("hk_prefix_attn_bf16");
     return HK_OK;
 }
@@ -516,8 +957,8 @@ extern "C" size_t hk_decode_attn_weights_ws(int32_t B, int32_t H, int32_t head_d
     p.H = H;
     p.Nq = 1;
     p.Nk = n_keys;
-    const int slots = plan(p, 1);
-    return part_bytes(p, head_dim, slots) + (size_t)B * H * ((n_keys + TK - 1) / TK * TK) * 4;
+    make_plan(p, head_dim, true);
+    return part_bytes(p, head_dim) + (size_t)B * H * ((n_keys + TK - 1) / TK * TK) * 4;
 }
 
 extern "C" int hk_decode_attn_weights_bf16(const hk_step_weights_desc* d, void* stream) {
@@ -549,12 +990,12 @@ extern "C" int hk_decode_attn_weights_bf16(const hk_step_weights_desc* d, void* 
     p.bias_bs = d->bias_bs;
     p.bias_hs = d->bias_hs;
     p.raw_ld = (d->n_keys + TK - 1) / TK * TK;
-    const int slots = plan(p, 1);
-    const size_t parts = part_bytes(p, d->head_dim, slots), need = parts + (size_t)p.B * p.H * p.raw_ld * 4;
+    make_plan(p, d->head_dim, true);
+    const size_t parts = part_bytes(p, d->head_dim), need = parts + (size_t)p.B * p.H * p.raw_ld * 4;
     HK_REQUIRE(d->ws && d->ws_bytes >= need, "hk_decode_attn_weights_bf16: workspace of %zu bytes, %zu needed (hk_decode_attn_weights_ws)",
                d->ws ? d->ws_bytes : (size_t)0, need);
-    HK_REQUIRE((int64_t)p.B * p.noc * p.H < (1LL << 31), "hk_decode_attn_weights_bf16: grid too large");
-    set_parts(p, d->ws, d->head_dim, slots);
+    HK_REQUIRE(part_grid(p) < (1LL << 31), "hk_decode_attn_weights_bf16: grid too large");
+    set_parts(p, d->ws, d->head_dim);
     p.raw = reinterpret_cast<float*>(reinterpret_cast<char*>(d->ws) + parts);
     StepWeights sw = {d->w_in, d->w_out, d->wi_bs, d->wi_hs, d->wo_bs, d->wo_hs};
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);

@@ -102,6 +102,8 @@ PREFIX = [  # B, Nq, P, Nk, H, hd, bias
     (2, 5, 0, 9, 2, 128, "all"), (5, 3, 777, 130, 12, 64, "add"), (1, 16, 100, 16, 2, 128, None), (3, 17, 64, 64, 2, 64, "holes"),
     (7, 37, 201, 37, 4, 128, "left"), (2, 130, 100, 200, 2, 128, "holes"), (1, 64, 1, 64, 1, 64, None), (2, 257, 300, 257, 3, 128, "left"),
     (1, 129, 0, 129, 2, 64, "all"), (3, 200, 1030, 700, 2, 64, "add"), (2, 512, 1400, 512, 2, 128, None), (9, 100, 65, 100, 2, 128, "left"),
+    (16, 5, 700, 60, 3, 128, "left"), (33, 3, 129, 40, 2, 64, "holes"), (4, 32, 2000, 32, 8, 128, None), (1, 64, 0, 5000, 1, 64, "add"),
+    (1, 100, 0, 3000, 2, 128, "left"), (40, 64, 64, 64, 32, 64, "all"), (1, 33, 4097, 1100, 1, 128, "holes"),
 ]
 
 
