@@ -942,6 +942,15 @@ extern "C" int hk_prefix_attn_bf16(const hk_prefix_attn_desc* d, void* stream) {
                "hk_prefix_attn_bf16: workspace of %zu bytes, %zu needed (hk_prefix_attn_ws)", d->ws ? d->ws_bytes : (size_t)0,
                part_bytes(p, d->head_dim));
     HK_REQUIRE(part_grid(p) < (1LL << 31) && rows_grid(p, m) < (1LL << 31), "hk_prefix_attn_bf16: grid too large");
+    {
+        const HkSpan o = hk_span(p.O, p.B, p.bso, p.Nq, p.ldo, row, 2), w = hk_span(d->ws, 1, 0, 1, 0, (int64_t)part_bytes(p, d->head_dim), 1);
+        const HkSpan in[] = {hk_span(p.KP, 1, 0, p.P, p.ldkp, row, 2), hk_span(p.VP, 1, 0, p.P, p.ldvp, row, 2),
+                             hk_span(p.K, p.B, p.bsk, p.Nk, p.ldk, row, 2), hk_span(p.V, p.B, p.bsv, p.Nk, p.ldv, row, 2),
+                             hk_span(p.bias, p.B, p.bias_bs, 1, 0, p.Nk, 4), hk_span(p.Q, p.B, p.bsq, p.Nq, p.ldq, row, 2)};
+        for (int i = 0; i < 6; ++i)
+            HK_REQUIRE(!hk_overlap(w, in[i]) && !hk_overlap(o, in[i]), "hk_prefix_attn_bf16: the output or the workspace overlaps an input");
+        HK_REQUIRE(!hk_overlap(o, w), "hk_prefix_attn_bf16: the output overlaps the workspace");
+    }
     set_parts(p, d->ws, d->head_dim);
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     const int rc = d->head_dim == 128 ? launch_prefix<128>(p, m, s) : launch_prefix<64>(p, m, s);
@@ -995,6 +1004,17 @@ extern "C" int hk_decode_attn_weights_bf16(const hk_step_weights_desc* d, void* 
     HK_REQUIRE(d->ws && d->ws_bytes >= need, "hk_decode_attn_weights_bf16: workspace of %zu bytes, %zu needed (hk_decode_attn_weights_ws)",
                d->ws ? d->ws_bytes : (size_t)0, need);
     HK_REQUIRE(part_grid(p) < (1LL << 31), "hk_decode_attn_weights_bf16: grid too large");
+    {
+        const HkSpan wo = hk_span(d->w_out, p.B, d->wo_bs, p.H, d->wo_hs, p.Nk, 4), o = hk_span(p.O, p.B, D, 1, 0, D, 2),
+                     w = hk_span(d->ws, 1, 0, 1, 0, (int64_t)need, 1);
+        const HkSpan in[] = {hk_span(p.Q, p.B, D, 1, 0, D, 2), hk_span(p.K, p.B, p.bsk, p.Nk, D, D, 2), hk_span(p.V, p.B, p.bsv, p.Nk, D, D, 2),
+                             hk_span(p.bias, p.B, p.bias_bs, p.H, p.bias_hs, p.Nk, 4),
+                             d->w_in == d->w_out ? HkSpan{0, 0} : hk_span(d->w_in, p.B, d->wi_bs, p.H, d->wi_hs, p.Nk, 4)};
+        for (int i = 0; i < 5; ++i)
+            HK_REQUIRE(!hk_overlap(wo, in[i]) && !hk_overlap(o, in[i]) && !hk_overlap(w, in[i]),
+                       "hk_decode_attn_weights_bf16: an output or the workspace overlaps an input");
+        HK_REQUIRE(!hk_overlap(o, wo) && !hk_overlap(o, w) && !hk_overlap(wo, w), "hk_decode_attn_weights_bf16: outputs and workspace overlap");
+    }
     set_parts(p, d->ws, d->head_dim);
     p.raw = reinterpret_cast<float*>(reinterpret_cast<char*>(d->ws) + parts);
     StepWeights sw = {d->w_in, d->w_out, d->wi_bs, d->wi_hs, d->wo_bs, d->wo_hs};

@@ -389,6 +389,16 @@ extern "C" int hk_attn_key_weights_bf16(const hk_key_weights_desc* d, void* stre
     const size_t need = (size_t)d->B * d->H * d->Nq * 4;
     HK_REQUIRE(d->ws && d->ws_bytes >= need, "hk_attn_key_weights_bf16: workspace of %zu bytes, B * H * Nq floats = %zu needed",
                d->ws ? d->ws_bytes : (size_t)0, need);
+    {
+        const int64_t row = (int64_t)d->H * d->head_dim;
+        const HkSpan wo = hk_span(d->w_out, d->B, d->wo_bs, d->H, d->wo_hs, d->Nk, 4), w = hk_span(d->ws, 1, 0, 1, 0, (int64_t)need, 1);
+        const HkSpan in[] = {hk_span(d->Q, d->B, d->bsq, d->Nq, d->ldq, row, 2), hk_span(d->K, d->B, d->bsk, d->Nk, d->ldk, row, 2),
+                             hk_span(d->key_bias, d->B, d->bias_bs, 1, 0, d->Nk, 4),
+                             d->w_in == d->w_out ? HkSpan{0, 0} : hk_span(d->w_in, d->B, d->wi_bs, d->H, d->wi_hs, d->Nk, 4)};
+        for (int i = 0; i < 4; ++i)
+            HK_REQUIRE(!hk_overlap(wo, in[i]) && !hk_overlap(w, in[i]), "hk_attn_key_weights_bf16: the output or the workspace overlaps an input");
+        HK_REQUIRE(!hk_overlap(wo, w), "hk_attn_key_weights_bf16: the output overlaps the workspace");
+    }
     const int64_t most = ((d->Nq > d->Nk ? d->Nq : d->Nk) + BLK - 1) / BLK;
     HK_REQUIRE(most * d->B * d->H < (1LL << 31), "hk_attn_key_weights_bf16: grid too large");
     KeyWeightParams p = {};
@@ -447,6 +457,20 @@ extern "C" int hk_cache_evict_bf16(const hk_cache_evict_desc* d, void* stream) {
     HK_REQUIRE((d->H == 1 || d->wo_hs >= wlen) && (d->B == 1 || d->wo_bs >= (d->H - 1) * d->wo_hs + wlen) &&
                    (d->key_bias == nullptr || ((d->H == 1 || d->bo_hs >= wlen) && (d->B == 1 || d->bo_bs >= (d->H - 1) * d->bo_hs + wlen))),
                "hk_cache_evict_bf16: rows of the weights and biases written must not overlap");
+    {
+        const HkSpan out[] = {hk_span(d->k_out, d->B, d->bsko, d->budget, d->ldko, row, 2), hk_span(d->v_out, d->B, d->bsvo, d->budget, d->ldvo, row, 2),
+                              hk_span(d->weight_out, d->B, d->wo_bs, d->H, d->wo_hs, wlen, 4),
+                              hk_span(d->key_bias_out, d->B, d->bo_bs, d->H, d->bo_hs, wlen, 4),
+                              hk_span(d->kept, 1, 0, 1, 0, (int64_t)d->B * d->H * d->budget, 4)};
+        const HkSpan in[] = {hk_span(d->K, d->B, d->bsk, d->n_keys, d->ldk, row, 2), hk_span(d->V, d->B, d->bsv, d->n_keys, d->ldv, row, 2),
+                             hk_span(d->weight, d->B, d->w_bs, d->H, d->w_hs, d->n_keys, 4),
+                             hk_span(d->key_bias, d->B, d->b_bs, d->H, d->b_hs, d->n_keys, 4)};
+        for (int i = 0; i < 5; ++i) {
+            for (int j = 0; j < 4; ++j)      // in place, an output is its own input
+                HK_REQUIRE((in_place && i == j) || !hk_overlap(out[i], in[j]), "hk_cache_evict_bf16: an output overlaps an input");
+            for (int j = 0; j < i; ++j) HK_REQUIRE(!hk_overlap(out[i], out[j]), "hk_cache_evict_bf16: two outputs overlap");
+        }
+    }
     EvictParams p = {};
     p.K = reinterpret_cast<const __bf16*>(d->K);
     p.V = reinterpret_cast<const __bf16*>(d->V);

@@ -77,6 +77,18 @@ __device__ __forceinline__ void glds4_s(const void* sbase, uint32_t voff, const 
 
 void hk_set_error(const char* fmt, ...);
 
+// Host-side check that what a call writes overlaps nothing it reads: the bytes [first, behind last) an operand of n1 x n2 rows of `row`
+// elements spans (strides in elements, not negative).  A null operand spans nothing.
+struct HkSpan {
+    uintptr_t a, b;
+};
+static inline HkSpan hk_span(const void* ptr, int64_t n1, int64_t s1, int64_t n2, int64_t s2, int64_t row, int64_t elem) {
+    if (!ptr || n1 < 1 || n2 < 1 || row < 1) return {0, 0};
+    const uintptr_t a = reinterpret_cast<uintptr_t>(ptr);
+    return {a, a + (uintptr_t)(((n1 - 1) * s1 + (n2 - 1) * s2 + row) * elem)};
+}
+static inline bool hk_overlap(HkSpan x, HkSpan y) { return x.a < y.b && y.a < x.b; }
+
 #define HK_REQUIRE(cond, ...)            \
     do {                                 \
         if (!(cond)) {                   \

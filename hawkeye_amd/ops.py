@@ -5,6 +5,7 @@ every function passes raw pointers to libhawkeye_hip.so and raises
 RuntimeError on a non-zero return code.  Nothing in this file computes.
 """
 import ctypes as C
+from operator import index
 from typing import Optional, Tuple
 
 import torch
@@ -489,12 +490,48 @@ def decode_attn_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, po
 
 
 # ---------------------------------------------------------------- a shared prefix; caches cut by attention weight
+# A call's layout (shapes, strides, types, device) is checked once and kept under that layout, with the numbers its descriptor takes from
+# it: a decode loop repeats layouts, and the checks cost the host more than these launches cost the device.  Nothing is kept by a
+# tensor's address; addresses, alignment and overlaps are checked by the library, every time.
+_layouts = {}
+
+
+def _layout(check, *args):
+    """check(*args), remembered by the layout of the tensors among args."""
+    key = (check, *[(a.shape, a.stride(), a.dtype, a.device) if isinstance(a, torch.Tensor) else a for a in args])
+    got = _layouts.get(key)
+    if got is None:
+        got = check(*args)
+        if len(_layouts) >= 4096:
+            _layouts.clear()
+        _layouts[key] = got
+    return got
+
+
+class _On:
+    """with _On(dev) as stream: the current device is dev and stream its current stream's handle (a device switch only if there is one)."""
+    __slots__ = ("dev", "back")
+
+    def __init__(self, dev: torch.device):
+        self.dev = dev
+
+    def __enter__(self) -> int:
+        self.back = torch.cuda.current_device()
+        if self.back != self.dev.index:
+            torch.cuda.set_device(self.dev.index)
+        return torch._C._cuda_getCurrentRawStream(self.dev.index)    # current_stream() builds a Stream object: 2.7 us a call against 0.1
+
+    def __exit__(self, *exc):
+        if self.back != self.dev.index:
+            torch.cuda.set_device(self.back)
+
+
 def _strides(t: torch.Tensor, name: str, H: int, hd: int):
     """(token stride, batch stride) of a bf16 [B, N, H, hd] view whose last two dims are dense; of a dim of size 1 the stride is free."""
     _need(t, torch.bfloat16, name)
     if t.dim() != 4 or t.shape[2] != H or t.shape[3] != hd or t.stride(3) != 1 or (H > 1 and t.stride(2) != hd):
         raise RuntimeError(f"{name} must be [B,N,{H},{hd}] with dense (H,{hd}) dims, got {tuple(t.shape)} strides {t.stride()}")
-    return (t.stride(1) if t.shape[1] > 1 else H * hd), (t.stride(0) if t.shape[0] > 1 else H * hd * t.shape[1])
+    return (t.stride(1) if t.shape[1] > 1 else H * hd), (t.stride(0) if t.shape[0] > 1 else H * hd * max(t.shape[1], 1))
 
 
 def _one_device(what: str, *ts):
@@ -502,7 +539,6 @@ def _one_device(what: str, *ts):
     for t in ts:
         if t is not None and t.device != dev:
             raise RuntimeError(f"{what}: tensors on {dev} and {t.device}")
-    return dev
 
 
 def _per_key(t: Optional[torch.Tensor], name: str, B: int, H: int, n: int, per_head: bool):
@@ -511,23 +547,37 @@ def _per_key(t: Optional[torch.Tensor], name: str, B: int, H: int, n: int, per_h
         return 0, 0
     _need(t, torch.float32, name)
     shared = t.dim() == 2 and not per_head
-    if not shared and t.dim() != 3 or t.shape[0] != B or (not shared and t.shape[1] != H) or t.shape[-1] < n or (n > 1 and t.stride(-1) != 1):
+    if (not shared and t.dim() != 3) or t.shape[0] != B or (not shared and t.shape[1] != H) or t.shape[-1] < n or (n > 1 and t.stride(-1) != 1):
         raise RuntimeError(f"{name} must be fp32 [{B}, {H}, >= {n}]{'' if per_head else f' or [{B}, >= {n}]'} with unit key stride, got {tuple(t.shape)}")
     return (t.stride(0) if B > 1 else H * t.shape[-1]), 0 if shared else (t.stride(1) if H > 1 else t.shape[-1])
 
 
-def _span(t: torch.Tensor):
-    a = t.data_ptr()
-    return a, a + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() if t.numel() else a
-
-
-def _no_overlap(what: str, out: torch.Tensor, *ins):
-    a0, a1 = _span(out)
-    for t in ins:
-        if t is not None:
-            b0, b1 = _span(t)
-            if a0 < b1 and b0 < a1:
-                raise RuntimeError(f"{what}: the output overlaps an input")
+def _prefix_layout(q, k_prefix, v_prefix, k, v, key_bias, out):
+    if q.dim() != 4 or q.shape[3] not in (64, 128):
+        raise RuntimeError("prefix_attention: q must be [B,Nq,H,hd], head size 64 or 128")
+    B, Nq, H, hd = q.shape
+    if k_prefix.dim() != 3 or v_prefix.dim() != 3 or k_prefix.shape != v_prefix.shape:
+        raise RuntimeError("prefix_attention: k_prefix and v_prefix must be [P,H,hd]")
+    if k.dim() != 4 or k.shape != v.shape or k.shape[0] != B:
+        raise RuntimeError("prefix_attention: k and v must be [B,Nk,H,hd]")
+    P, Nk = k_prefix.shape[0], k.shape[1]
+    if B < 1 or Nq < 1 or Nk < Nq:
+        raise RuntimeError(f"prefix_attention: {Nq} queries of {B} sequences need at least as many own keys, got {Nk}")
+    _one_device("prefix_attention", q, k_prefix, v_prefix, k, v, key_bias, out)
+    ldq, bsq = _strides(q, "q", H, hd)
+    ldkp, _ = _strides(k_prefix[None], "k_prefix", H, hd)
+    ldvp, _ = _strides(v_prefix[None], "v_prefix", H, hd)
+    ldk, bsk = _strides(k, "k", H, hd)
+    ldv, bsv = _strides(v, "v", H, hd)
+    if key_bias is not None and key_bias.dim() != 2:
+        raise RuntimeError("prefix_attention: key_bias must be fp32 [B, >= Nk]")
+    bias_bs, _ = _per_key(key_bias, "key_bias", B, 1, Nk, False)
+    ldo, bso = H * hd, Nq * H * hd
+    if out is not None:
+        if out.shape != q.shape:
+            raise RuntimeError(f"prefix_attention: out must be {tuple(q.shape)}")
+        ldo, bso = _strides(out, "out", H, hd)
+    return prefix_attention_ws(B, H, Nq, P, Nk, hd), (B, H, Nq, P, Nk, hd, ldq, bsq, ldkp, ldvp, ldk, bsk, ldv, bsv, ldo, bso, bias_bs)
 
 
 def prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -537,43 +587,19 @@ def prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Te
     k_prefix / v_prefix [P,H,hd] (P >= 0, one copy for all sequences, all visible) and the sequences' own k / v [B,Nk,H,hd]
     (Nk >= Nq >= 1, causal: query i sees own keys <= i + Nk - Nq).  bf16 views, hd 64 or 128, last two dims dense; returns
     [B,Nq,H,hd] bf16.  key_bias: optional fp32 [B, >= Nk] of the own keys (natural-log units); -1e4 or less removes the key.  A row that sees
-    no key gives zeros.  ws: uint8 of at least prefix_attention_ws(...) bytes (default: allocated), for this call alone."""
-    if q.dim() != 4 or q.shape[3] not in (64, 128):
-        raise RuntimeError("prefix_attention: q must be [B,Nq,H,hd], head size 64 or 128")
-    B, Nq, H, hd = q.shape
-    if k_prefix.dim() != 3 or v_prefix.dim() != 3 or k_prefix.shape != v_prefix.shape:
-        raise RuntimeError("prefix_attention: k_prefix and v_prefix must be [P,H,hd]")
-    if k.dim() != 4 or k.shape != v.shape or k.shape[0] != B:
-        raise RuntimeError("prefix_attention: k and v must be [B,Nk,H,hd]")
-    P, Nk = k_prefix.shape[0], k.shape[1]
-    if Nq < 1 or Nk < Nq:
-        raise RuntimeError(f"prefix_attention: {Nq} queries need at least as many own keys, got {Nk}")
-    dev = _one_device("prefix_attention", q, k_prefix, v_prefix, k, v, key_bias, out, ws)
-    ldq, bsq = _strides(q, "q", H, hd)
-    ldkp, _ = _strides(k_prefix[None], "k_prefix", H, hd)
-    ldvp, _ = _strides(v_prefix[None], "v_prefix", H, hd)
-    ldk, bsk = _strides(k, "k", H, hd)
-    ldv, bsv = _strides(v, "v", H, hd)
-    bias_bs = 0
-    if key_bias is not None:
-        if key_bias.dim() != 2:
-            raise RuntimeError("prefix_attention: key_bias must be fp32 [B, >= Nk]")
-        bias_bs, _ = _per_key(key_bias, "key_bias", B, 1, Nk, False)
-    if out is None:
-        out = torch.empty((B, Nq, H, hd), dtype=torch.bfloat16, device=dev)
-    if out.shape != q.shape:
-        raise RuntimeError(f"prefix_attention: out must be {tuple(q.shape)}")
-    ldo, bso = _strides(out, "out", H, hd)
-    _no_overlap("prefix_attention", out, k_prefix, v_prefix, k, v, key_bias, ws)
-    lib = L.load()
-    need = prefix_attention_ws(B, H, Nq, P, Nk, hd)
-    with torch.cuda.device(dev):
+    no key gives zeros.  out may not overlap an input.  ws: uint8 of at least prefix_attention_ws(...) bytes (default: allocated),
+    for this call alone."""
+    need, nums = _layout(_prefix_layout, q, k_prefix, v_prefix, k, v, key_bias, out)
+    with _On(q.device) as stream:
+        if out is None:
+            out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
         if ws is None:
-            ws = torch.empty((need,), dtype=torch.uint8, device=dev)
-        _need(ws, torch.uint8, "ws")
+            ws = torch.empty((need,), dtype=torch.uint8, device=q.device)
+        elif ws.dtype != torch.uint8 or ws.device != q.device or not ws.is_contiguous():
+            raise RuntimeError("prefix_attention: ws must be a contiguous uint8 tensor on q's device")
         d = L.HkPrefixAttnDesc(q.data_ptr(), k_prefix.data_ptr(), v_prefix.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(key_bias),
-                               ws.data_ptr(), ws.numel(), B, H, Nq, P, Nk, hd, ldq, bsq, ldkp, ldvp, ldk, bsk, ldv, bsv, ldo, bso, bias_bs)
-        L.check(lib.hk_prefix_attn_bf16(C.byref(d), _stream()), "hk_prefix_attn_bf16")
+                               ws.data_ptr(), ws.numel(), *nums)
+        L.check(L.load().hk_prefix_attn_bf16(C.byref(d), stream), "hk_prefix_attn_bf16")
     return out
 
 
@@ -585,18 +611,10 @@ def prefix_attention_ws(B: int, H: int, Nq: int, P: int, Nk: int, head_dim: int)
     return need
 
 
-def decode_attn_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, n_keys: int, H: int, head_dim: int,
-                        weight: Optional[torch.Tensor], key_bias: Optional[torch.Tensor] = None,
-                        weight_out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """decode_attn (one query row per (sequence, head) over cache rows [0, n_keys): bf16 [B, H*hd]) that also adds the row's softmax weights
-    to what the keys have collected: weight_out[..., :n_keys] = weight[..., :n_keys] + p, fp32 [B, H, >= n_keys] (weight_out None: in
-    place; weight None: zeros).  key_bias: optional fp32 [B, >= n_keys] or, once heads keep different rows, [B, H, >= n_keys]; -1e4 or
-    less removes the key.  A sequence without a key gives zeros and adds nothing."""
+def _step_layout(q, k_cache, v_cache, n_keys, H, head_dim, weight, key_bias, weight_out):
     _need(q, torch.bfloat16, "q")
     _need(k_cache, torch.bfloat16, "k_cache")
     _need(v_cache, torch.bfloat16, "v_cache")
-    if weight_out is None:
-        weight_out = weight
     if weight_out is None:
         raise RuntimeError("decode_attn_weights: weight and weight_out are both None")
     B, D = q.shape[0], H * head_dim
@@ -605,22 +623,52 @@ def decode_attn_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         raise RuntimeError("decode_attn_weights: q contiguous [B, H*hd], caches contiguous [B, rows, H*hd]")
     if not 1 <= n_keys <= k_cache.shape[1]:
         raise RuntimeError(f"decode_attn_weights: n_keys={n_keys} must be 1..{k_cache.shape[1]}")
-    dev = _one_device("decode_attn_weights", q, k_cache, v_cache, weight, weight_out, key_bias)
-    wi_bs, wi_hs = _per_key(weight, "weight", B, H, n_keys, True)
-    wo_bs, wo_hs = _per_key(weight_out, "weight_out", B, H, n_keys, True)
-    bias_bs, bias_hs = _per_key(key_bias, "key_bias", B, H, n_keys, False)
-    same = weight is not None and weight.data_ptr() == weight_out.data_ptr()
-    _no_overlap("decode_attn_weights", weight_out, q, k_cache, v_cache, key_bias, None if same else weight)
-    lib = L.load()
-    with torch.cuda.device(dev):
+    _one_device("decode_attn_weights", q, k_cache, v_cache, weight, weight_out, key_bias)
+    wi = _per_key(weight, "weight", B, H, n_keys, True)
+    wo = _per_key(weight_out, "weight_out", B, H, n_keys, True)
+    bias = _per_key(key_bias, "key_bias", B, H, n_keys, False)
+    need = L.load().hk_decode_attn_weights_ws(B, H, head_dim, n_keys)
+    if need == 0:
+        raise RuntimeError(f"decode_attn_weights: shape B={B} H={H} n_keys={n_keys} head size {head_dim} is not supported")
+    return need, (B, H, head_dim, n_keys, k_cache.shape[1], *bias, *wi, *wo)
+
+
+def decode_attn_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, n_keys: int, H: int, head_dim: int,
+                        weight: Optional[torch.Tensor], key_bias: Optional[torch.Tensor] = None,
+                        weight_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """decode_attn (one query row per (sequence, head) over cache rows [0, n_keys): bf16 [B, H*hd]) that also adds the row's softmax weights
+    to what the keys have collected: weight_out[..., :n_keys] = weight[..., :n_keys] + p, fp32 [B, H, >= n_keys] (weight_out None: in
+    place; weight None: zeros).  key_bias: optional fp32 [B, >= n_keys] or, once heads keep different rows, [B, H, >= n_keys]; -1e4 or
+    less removes the key.  A sequence without a key gives zeros and adds nothing."""
+    if weight_out is None:
+        weight_out = weight
+    n_keys, H, head_dim = index(n_keys), index(H), index(head_dim)
+    need, nums = _layout(_step_layout, q, k_cache, v_cache, n_keys, H, head_dim, weight, key_bias, weight_out)
+    with _On(q.device) as stream:
         out = torch.empty_like(q)
-        need = lib.hk_decode_attn_weights_ws(B, H, head_dim, n_keys)
-        ws = torch.empty((max(need, 16),), dtype=torch.uint8, device=dev)
+        ws = torch.empty((need,), dtype=torch.uint8, device=q.device)
         d = L.HkStepWeightsDesc(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _ptr(key_bias), _ptr(weight), weight_out.data_ptr(),
-                                out.data_ptr(), ws.data_ptr(), ws.numel(), B, H, head_dim, n_keys, k_cache.shape[1], bias_bs, bias_hs,
-                                wi_bs, wi_hs, wo_bs, wo_hs)
-        L.check(lib.hk_decode_attn_weights_bf16(C.byref(d), _stream()), "hk_decode_attn_weights_bf16")
+                                out.data_ptr(), ws.data_ptr(), need, *nums)
+        L.check(L.load().hk_decode_attn_weights_bf16(C.byref(d), stream), "hk_decode_attn_weights_bf16")
     return out
+
+
+def _key_weights_layout(q, k, key_bias, causal, weight, weight_out):
+    if q.dim() != 4 or k.dim() != 4 or q.shape[3] not in (64, 128) or k.shape[0] != q.shape[0]:
+        raise RuntimeError("attn_key_weights: q [B,Nq,H,hd] and k [B,Nk,H,hd], head size 64 or 128")
+    B, Nq, H, hd = q.shape
+    Nk = k.shape[1]
+    if B < 1 or Nq < 1 or Nk < 1 or (causal and Nk < Nq):
+        raise RuntimeError(f"attn_key_weights: Nq={Nq}, Nk={Nk} (at least one each; causal needs Nk >= Nq)")
+    _one_device("attn_key_weights", q, k, key_bias, weight, weight_out)
+    ldq, bsq = _strides(q, "q", H, hd)
+    ldk, bsk = _strides(k, "k", H, hd)
+    if key_bias is not None and key_bias.dim() != 2:
+        raise RuntimeError("attn_key_weights: key_bias must be fp32 [B, >= Nk]")
+    bias_bs, _ = _per_key(key_bias, "key_bias", B, 1, Nk, False)
+    wi = _per_key(weight, "weight", B, H, Nk, True)
+    wo = (H * Nk, Nk) if weight_out is None else _per_key(weight_out, "weight_out", B, H, Nk, True)
+    return B * H * Nq * 4, (B, H, Nq, Nk, hd, 1 if causal else 0, ldq, bsq, ldk, bsk, bias_bs, *wi, *wo)
 
 
 def attn_key_weights(q: torch.Tensor, k: torch.Tensor, key_bias: Optional[torch.Tensor] = None, causal: bool = True,
@@ -629,32 +677,33 @@ def attn_key_weights(q: torch.Tensor, k: torch.Tensor, key_bias: Optional[torch.
     [B,Nq,H,hd] (pre-scaled) of their softmax weights over k [B,Nk,H,hd] -> fp32 [B,H,Nk]; causal: query i sees keys <= i + Nk - Nq.
     weight fp32 [B,H,>=Nk]: added to it, in place unless weight_out (of the same kind) is given; both None: a new tensor.
     key_bias fp32 [B, >= Nk] (-1e4 or less removes the key).  A query that sees no key adds nothing."""
-    if q.dim() != 4 or k.dim() != 4 or q.shape[3] not in (64, 128) or k.shape[0] != q.shape[0]:
-        raise RuntimeError("attn_key_weights: q [B,Nq,H,hd] and k [B,Nk,H,hd], head size 64 or 128")
-    B, Nq, H, hd = q.shape
-    Nk = k.shape[1]
-    if Nq < 1 or Nk < 1 or (causal and Nk < Nq):
-        raise RuntimeError(f"attn_key_weights: Nq={Nq}, Nk={Nk} (at least one each; causal needs Nk >= Nq)")
-    dev = _one_device("attn_key_weights", q, k, key_bias, weight, weight_out)
-    ldq, bsq = _strides(q, "q", H, hd)
-    ldk, bsk = _strides(k, "k", H, hd)
-    bias_bs = 0
-    if key_bias is not None:
-        if key_bias.dim() != 2:
-            raise RuntimeError("attn_key_weights: key_bias must be fp32 [B, >= Nk]")
-        bias_bs, _ = _per_key(key_bias, "key_bias", B, 1, Nk, False)
-    with torch.cuda.device(dev):
+    if weight_out is None:
+        weight_out = weight
+    need, nums = _layout(_key_weights_layout, q, k, key_bias, bool(causal), weight, weight_out)
+    with _On(q.device) as stream:
         if weight_out is None:
-            weight_out = weight if weight is not None else torch.empty((B, H, Nk), dtype=torch.float32, device=dev)
-        wi_bs, wi_hs = _per_key(weight, "weight", B, H, Nk, True)
-        wo_bs, wo_hs = _per_key(weight_out, "weight_out", B, H, Nk, True)
-        same = weight is not None and weight.data_ptr() == weight_out.data_ptr()
-        _no_overlap("attn_key_weights", weight_out, q, k, key_bias, None if same else weight)
-        ws = torch.empty((B * H * Nq,), dtype=torch.float32, device=dev)
-        d = L.HkKeyWeightsDesc(q.data_ptr(), k.data_ptr(), _ptr(key_bias), _ptr(weight), weight_out.data_ptr(), ws.data_ptr(), ws.numel() * 4,
-                               B, H, Nq, Nk, hd, 1 if causal else 0, ldq, bsq, ldk, bsk, bias_bs, wi_bs, wi_hs, wo_bs, wo_hs)
-        L.check(L.load().hk_attn_key_weights_bf16(C.byref(d), _stream()), "hk_attn_key_weights_bf16")
+            weight_out = torch.empty((nums[0], nums[1], nums[3]), dtype=torch.float32, device=q.device)
+        ws = torch.empty((need,), dtype=torch.uint8, device=q.device)
+        d = L.HkKeyWeightsDesc(q.data_ptr(), k.data_ptr(), _ptr(key_bias), _ptr(weight), weight_out.data_ptr(), ws.data_ptr(), need, *nums)
+        L.check(L.load().hk_attn_key_weights_bf16(C.byref(d), stream), "hk_attn_key_weights_bf16")
     return weight_out
+
+
+def _evict_layout(k, v, weight, n_keys, budget, recent, key_bias, ko, vo, wo, bo):
+    if k.dim() != 4 or k.shape != v.shape:
+        raise RuntimeError("cache_evict: k and v must be [B,rows,H,hd]")
+    B, rows, H, hd = k.shape
+    if not (1 <= budget <= n_keys <= rows and 0 <= recent <= budget):
+        raise RuntimeError(f"cache_evict: n_keys={n_keys} of {rows} rows, budget={budget}, recent={recent} "
+                           "(1 <= budget <= n_keys <= rows, 0 <= recent <= budget)")
+    if (bo is None) != (key_bias is None):
+        raise RuntimeError("cache_evict: key_bias and its output come together")
+    _one_device("cache_evict", k, v, weight, key_bias, ko, vo, wo, bo)
+    if ko.dim() != 4 or vo.dim() != 4 or ko.shape[0] != B or vo.shape[0] != B or ko.shape[1] < budget or vo.shape[1] < budget:
+        raise RuntimeError(f"cache_evict: k_out and v_out must be [{B},>= {budget},{H},{hd}]")
+    return (B, H, hd, n_keys, budget, recent, *_strides(k, "k", H, hd), *_strides(v, "v", H, hd), *_strides(ko, "k_out", H, hd),
+            *_strides(vo, "v_out", H, hd), *_per_key(weight, "weight", B, H, n_keys, True), *_per_key(wo, "weight_out", B, H, budget, True),
+            *_per_key(key_bias, "key_bias", B, H, n_keys, True), *_per_key(bo, "key_bias_out", B, H, budget, True))
 
 
 def cache_evict(k: torch.Tensor, v: torch.Tensor, weight: torch.Tensor, n_keys: int, budget: int, recent: int = 0,
@@ -665,42 +714,14 @@ def cache_evict(k: torch.Tensor, v: torch.Tensor, weight: torch.Tensor, n_keys: 
     Returns kept int32 [B,H,budget], the rows they came from.  1 <= budget <= n_keys, 0 <= recent <= budget.
     out None: in place (weights and biases of rows [budget, n_keys) become 0); out = (k_out, v_out, weight_out, key_bias_out or None):
     other tensors that overlap no input, rows behind budget left alone.  key_bias fp32 [B,H,>=n_keys]: per head, as heads keep different rows."""
-    if k.dim() != 4 or k.shape != v.shape:
-        raise RuntimeError("cache_evict: k and v must be [B,rows,H,hd]")
-    B, rows, H, hd = k.shape
-    if not (1 <= budget <= n_keys <= rows and 0 <= recent <= budget):
-        raise RuntimeError(f"cache_evict: n_keys={n_keys} of {rows} rows, budget={budget}, recent={recent} "
-                           "(1 <= budget <= n_keys <= rows, 0 <= recent <= budget)")
-    inplace = out is None
-    ko, vo, wo, bo = (k, v, weight, key_bias) if inplace else out
-    if (bo is None) != (key_bias is None):
-        raise RuntimeError("cache_evict: key_bias and its output come together")
-    dev = _one_device("cache_evict", k, v, weight, key_bias, ko, vo, wo, bo)
-    ldk, bsk = _strides(k, "k", H, hd)
-    ldv, bsv = _strides(v, "v", H, hd)
-    w_bs, w_hs = _per_key(weight, "weight", B, H, n_keys, True)
-    b_bs, b_hs = _per_key(key_bias, "key_bias", B, H, n_keys, True)
-    if inplace:
-        pairs = [(k, v), (k, weight), (v, weight)] + ([(key_bias, t) for t in (k, v, weight)] if key_bias is not None else [])
-        for a, b in pairs:
-            _no_overlap("cache_evict", a, b)
-        ldko, bsko, ldvo, bsvo, wo_bs, wo_hs, bo_bs, bo_hs = ldk, bsk, ldv, bsv, w_bs, w_hs, b_bs, b_hs
-    else:
-        if ko.dim() != 4 or vo.dim() != 4 or ko.shape[0] != B or vo.shape[0] != B or ko.shape[1] < budget or vo.shape[1] < budget:
-            raise RuntimeError(f"cache_evict: k_out and v_out must be [{B},>= {budget},{H},{hd}]")
-        ldko, bsko = _strides(ko, "k_out", H, hd)
-        ldvo, bsvo = _strides(vo, "v_out", H, hd)
-        wo_bs, wo_hs = _per_key(wo, "weight_out", B, H, budget, True)
-        bo_bs, bo_hs = _per_key(bo, "key_bias_out", B, H, budget, True)
-        outs = [t for t in (ko, vo, wo, bo) if t is not None]
-        for i, t in enumerate(outs):
-            _no_overlap("cache_evict", t, k, v, weight, key_bias, *outs[i + 1:])
-    with torch.cuda.device(dev):
-        kept = torch.empty((B, H, budget), dtype=torch.int32, device=dev)
+    ko, vo, wo, bo = (k, v, weight, key_bias) if out is None else out
+    n_keys, budget, recent = index(n_keys), index(budget), index(recent)
+    nums = _layout(_evict_layout, k, v, weight, n_keys, budget, recent, key_bias, ko, vo, wo, bo)
+    with _On(k.device) as stream:
+        kept = torch.empty((nums[0], nums[1], budget), dtype=torch.int32, device=k.device)
         d = L.HkCacheEvictDesc(k.data_ptr(), v.data_ptr(), ko.data_ptr(), vo.data_ptr(), weight.data_ptr(), wo.data_ptr(), _ptr(key_bias), _ptr(bo),
-                               kept.data_ptr(), B, H, hd, n_keys, budget, recent, ldk, bsk, ldv, bsv, ldko, bsko, ldvo, bsvo,
-                               w_bs, w_hs, wo_bs, wo_hs, b_bs, b_hs, bo_bs, bo_hs)
-        L.check(L.load().hk_cache_evict_bf16(C.byref(d), _stream()), "hk_cache_evict_bf16")
+                               kept.data_ptr(), *nums)
+        L.check(L.load().hk_cache_evict_bf16(C.byref(d), stream), "hk_cache_evict_bf16")
     return kept
 
 
