@@ -394,30 +394,29 @@ __global__ __launch_bounds__(256, 2) void hk_prefix_rows_kernel(const PrefixPara
 #pragma unroll
         for (int s = 0; s < NKS; ++s) qf[s] = *reinterpret_cast<const bf16x8*>(qp + 16 * s);
     }
+    // The loads above are waited for here: left pending, the compiler would wait for them inside the loop, with counts that take the
+    // LDS-DMA in flight there (which it does not know) along.
+#pragma unroll
+    for (int s = 0; s < NKS; ++s) asm volatile("" : "+v"(qf[s]));
     const __bf16* kA = p.KP + (int64_t)a0 * p.ldkp + head * HD;
     const __bf16* vA = p.VP + (int64_t)a0 * p.ldvp + head * HD;
     const __bf16* kB = p.K + (int64_t)brow * p.bsk + (int64_t)b0 * p.ldk + head * HD;
     const __bf16* vB = p.V + (int64_t)brow * p.bsv + (int64_t)b0 * p.ldv + head * HD;
     const float* bias = BIAS ? p.bias + (int64_t)brow * p.bias_bs + (int64_t)head * p.bias_hs + b0 : nullptr;
 
-    // K: 16-byte chunk c of key row x at c ^ swk(x): 16 rows x one chunk touch every bank once; V: at c ^ swv(x): so do the 8 key rows of a
-    // transposing read
+    // K: 16-byte chunk c of key row x at c ^ swk(x): 16 rows x one chunk touch every bank once; V: at c ^ swv(x): so do the 4 key rows x
+    // 64 bytes that half a wave's transposing read takes
     auto swk = [](int x) { return HD == 128 ? x & 15 : (x >> 1) & 7; };
-    auto swv = [](int x) { return HD == 128 ? (x & 7) << 1 : ((x >> 1) & 1) << 2; };
+    auto swv = [](int x) { return HD == 128 ? (x & 3) << 2 : ((x >> 1) & 1) << 2; };
     const int lrow = tid / CH, lch = tid % CH;
+    const uint32_t klA = (uint32_t)((lrow * p.ldkp + (lch ^ swk(lrow)) * 8) * 2), klB = (uint32_t)((lrow * p.ldk + (lch ^ swk(lrow)) * 8) * 2);
+    const uint32_t vlA = (uint32_t)((lrow * p.ldvp + (lch ^ swv(lrow)) * 8) * 2), vlB = (uint32_t)((lrow * p.ldv + (lch ^ swv(lrow)) * 8) * 2);
     float br = 0.f;
-    auto issue = [&](int t, int stage) __attribute__((always_inline)) {
-        const bool own = t >= nA;
-        const int kt = (own ? t - nA : t) * KT;
-        const int n = own ? k1 : a1 - a0;
-        const int64_t ldk = own ? p.ldk : p.ldkp, ldv = own ? p.ldv : p.ldvp;
-        const __bf16* kb = own ? kB : kA;
-        const __bf16* vb = own ? vB : vA;
+    auto load_tile = [&](const __bf16* kb, const __bf16* vb, int64_t ldk, int64_t ldv, uint32_t kl, uint32_t vl, int kt, int n, int stage)
+        __attribute__((always_inline)) {
         char* ks = smem + stage * STAGE + wave * (64 / CH) * ROWB;
         char* vs = ks + KT * ROWB;
         // the swizzle goes on the source chunk (the LDS image is lane-linear); RPP is a multiple of every swizzle's period
-        const uint32_t kl = (uint32_t)((lrow * ldk + (lch ^ swk(lrow)) * 8) * 2);
-        const uint32_t vl = (uint32_t)((lrow * ldv + (lch ^ swv(lrow)) * 8) * 2);
         if (kt + KT <= n) {
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
@@ -432,7 +431,14 @@ __global__ __launch_bounds__(256, 2) void hk_prefix_rows_kernel(const PrefixPara
                 glds16_v(vb + key * ldv + (lch ^ swv(lrow)) * 8, vs + i * RPP * ROWB);
             }
         }
-        if (BIAS && own && tid < KT) br = bias[min(kt + tid, k1 - 1)];
+    };
+    auto issue = [&](int t, int stage) __attribute__((always_inline)) {
+        if (t < nA) {
+            load_tile(kA, vA, p.ldkp, p.ldvp, klA, vlA, t * KT, a1 - a0, stage);
+        } else {
+            load_tile(kB, vB, p.ldk, p.ldv, klB, vlB, (t - nA) * KT, k1, stage);
+            if (BIAS && tid < KT) br = bias[min((t - nA) * KT + tid, k1 - 1)];
+        }
     };
     // K fragment (g, s): row 32 g + r, chunk 2 s + h; V fragment (s, d): rows 16 s + vrow (and + 8), dims 32 d + 16 ((lane >> 4) & 1) + ...:
     // chunk numbers are joined to the swizzle by exclusive or, so one register per operand holds every offset
@@ -468,9 +474,9 @@ __global__ __launch_bounds__(256, 2) void hk_prefix_rows_kernel(const PrefixPara
 #pragma unroll
                 for (int i = 0; i < 16; ++i) c0[i] = -m;
 #pragma unroll
-                for (int g = 0; g < 2; ++g)
+                for (int s = 0; s < NKS; ++s)              // two independent chains
 #pragma unroll
-                    for (int s = 0; s < NKS; ++s) {
+                    for (int g = 0; g < 2; ++g) {
                         const bf16x8 kf = *reinterpret_cast<const bf16x8*>(ks + g * 32 * ROWB + (ko ^ (32 * s)));
                         st[g] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[s], s == 0 ? c0 : st[g], 0, 0, 0);
                     }

@@ -1,5 +1,6 @@
 // Cutting a cache to the keys that attention has used: the weight every key collects from the queries of a prompt, and the move
 // of the keys with the most weight to the front of the cache.
+#include <type_traits>
 #include "hk_common.h"
 
 namespace {
@@ -11,7 +12,8 @@ constexpr float REMOVED = -1.0e4f;   // a key whose bias is at or below this doe
 // Two launches of one structure: a wave keeps 32 rows of one operand in registers and walks 64-row tiles of the other, which the
 // four waves of a workgroup share in LDS (two stages, LDS-DMA one tile ahead).  Both compute S^T = K . Q^T with
 // v_mfma_f32_32x32x16_bf16: lane -> query lane & 31, register i -> key (i & 3) + 8 (i >> 2) + 4 (lane >> 5).
-//   STATS: queries stay, keys pass: running maximum and sum of a query's row in the lane -> z.
+//   STATS: queries stay, keys pass: a reference point m and the sum of 2^(s - m) in the lane -> z.  m is the maximum of the row's first keys and
+//     moves only when a tile's partial sum leaves [0, 2^20] (that tile is redone): the common path is exp2 and an addition per score.
 //   SUMS:  keys stay, queries pass: 2^(s - z) added up in 16 registers per lane, over the 32 lanes at the end.
 // No sum crosses workgroups: every order is fixed.
 struct KeyWeightParams {
@@ -24,6 +26,8 @@ struct KeyWeightParams {
     int64_t ldq, bsq, ldk, bsk, bias_bs, wi_bs, wi_hs, wo_bs, wo_hs;
 };
 
+constexpr int NST = 2;               // stages (a power of two): a tile is requested NST - 1 tiles ahead.  4 measured alike (STATS) or 13 % slower (SUMS)
+constexpr float OVERFLOW_SUM = 1048576.0f;
 constexpr int BLK = 128;             // rows of the operand that stays, per workgroup
 constexpr int TILE = 64;             // rows of the operand that passes, per stage
 
@@ -33,8 +37,9 @@ __global__ __launch_bounds__(256, 2) void hk_key_weights_kernel(const KeyWeightP
     constexpr int STAGE = TILE * ROWB;
     constexpr int RPI = 64 / CH;                           // rows one wave-wide LDS-DMA covers
     constexpr int NI = TILE / (4 * RPI);                   // of them per wave and tile
-    extern __shared__ __attribute__((aligned(16))) char smem[];      // 2 stages, then [2][TILE] floats: bias (STATS) or z (SUMS)
-    float* side = reinterpret_cast<float*>(smem + 2 * STAGE);
+    constexpr bool SIDE = SUMS || BIAS;                    // 64 floats come with a tile: its queries' z (SUMS), its keys' biases (STATS)
+    constexpr int PER = NI + (SIDE ? 1 : 0);               // LDS-DMAs per wave and tile
+    extern __shared__ __attribute__((aligned(16))) char smem[];      // NST stages, then [NST][wave][TILE] floats (each wave its own copy)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 31, h = lane >> 5;
     const int nbh = p.B * p.H;
@@ -53,28 +58,39 @@ __global__ __launch_bounds__(256, 2) void hk_key_weights_kernel(const KeyWeightP
 #pragma unroll
         for (int s = 0; s < NKS; ++s) sf[s] = *reinterpret_cast<const bf16x8*>(sp + 16 * s);
     }
+    // The loads above are waited for here: left pending, the compiler would wait for them inside the loop, with counts that take the
+    // LDS-DMA in flight there (which it does not know) along.
+#pragma unroll
+    for (int s = 0; s < NKS; ++s) asm volatile("" : "+v"(sf[s]));
     const __bf16* pbase = (SUMS ? p.Q + (int64_t)b * p.bsq : p.K + (int64_t)b * p.bsk) + head * HD;
     const int64_t ldp = SUMS ? p.ldq : p.ldk;
     const float* bias = BIAS ? p.bias + (int64_t)b * p.bias_bs : nullptr;
     float* z = p.z + (int64_t)bh * p.Nq;
 
-    // 16-byte chunk c of row x lives at chunk c ^ (x & (CH - 1)): 16 rows x one chunk touch every bank once
-    float sr = 0.f;
-    auto issue = [&](int t, int stage) {
+    // 16-byte chunk c of row x lives at chunk c ^ swz(x): 16 rows x one chunk touch every bank once
+    auto swz = [](int x) { return HD == 128 ? x & 15 : (x >> 1) & 7; };
+    float* side = reinterpret_cast<float*>(smem + NST * STAGE) + wave * TILE;
+    const int lx = lane / CH, lc = (lane % CH) ^ swz(lx);  // this lane's row and (source) chunk of a piece of RPI rows from lr:
+    // swz(lr + lx) == swz(lr) ^ swz(lx), as RPI is 4 (HD 128) or 8
+    const uint32_t lane_off = (uint32_t)((lx * ldp) * 2);
+    auto issue = [&](int t) {
+        char* st = smem + (t & (NST - 1)) * STAGE;
+        if ((t + 1) * TILE <= n_pass) {                    // scalar base + 32-bit lane offset
 #pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            const int lr = (wave * NI + i) * RPI;          // first row of this piece
-            const int x = lr + lane / CH, c = (lane % CH) ^ (x & (CH - 1));
-            glds16_v(pbase + (int64_t)min(t * TILE + x, n_pass - 1) * ldp + c * 8, smem + stage * STAGE + lr * ROWB);
+            for (int i = 0; i < NI; ++i) {
+                const int lr = (wave * NI + i) * RPI;      // first row of this piece
+                glds16_s(pbase + (int64_t)(t * TILE + lr) * ldp, lane_off + (uint32_t)((lc ^ swz(lr)) << 4), st + lr * ROWB);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const int lr = (wave * NI + i) * RPI;
+                glds16_v(pbase + (int64_t)min(t * TILE + lr + lx, n_pass - 1) * ldp + (lc ^ swz(lr)) * 8, st + lr * ROWB);
+            }
         }
-        if ((SUMS || BIAS) && tid < TILE) {
-            const int x = min(t * TILE + tid, n_pass - 1);
-            sr = SUMS ? z[x] : bias[x];
-        }
+        if (SIDE) glds4_s(SUMS ? z : bias, (uint32_t)min(t * TILE + lane, n_pass - 1) * 4u, side + (t & (NST - 1)) * 4 * TILE);
     };
-    int roff[NKS];
-#pragma unroll
-    for (int s = 0; s < NKS; ++s) roff[s] = r * ROWB + (((2 * s + h) ^ (r & (CH - 1))) << 4);
+    const int ro = r * ROWB + ((h ^ swz(r)) << 4);         // chunk 2 s + h: the 2 s joins by exclusive or
 
     int t0 = 0, t1 = (n_pass + TILE - 1) / TILE;
     if (p.causal) {
@@ -82,89 +98,147 @@ __global__ __launch_bounds__(256, 2) void hk_key_weights_kernel(const KeyWeightP
         else t1 = min(t1, (min(blk * BLK + BLK, p.Nq) - 1 + off) / TILE + 1);                // last key the block's last query sees
     }
     float kb[16];                                          // SUMS: the bias of this lane's keys, -inf for removed ones
+    bool kplain = true, kall = false;                      // all of the wave's biases are 0, all of its keys are removed
     if (SUMS && BIAS) {
+        const float kv = bias[min(s0 + r, p.Nk - 1)];
+        kplain = __builtin_amdgcn_ballot_w64(kv != 0.f) == 0;
+        kall = __builtin_amdgcn_ballot_w64(kv <= REMOVED || s0 + r >= p.Nk) == ~0ull;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const float v = bias[min(s0 + (i & 3) + 8 * (i >> 2) + 4 * h, p.Nk - 1)];
             kb[i] = v <= REMOVED ? -INFINITY : v * HK_LOG2E;
+            asm volatile("" : "+v"(kb[i]));
         }
     }
     float acc[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-    float m = -1.0e30f, l = 0.f;
+    float m = 0.f, l = 0.f;                                // STATS: everything is relative to m
+    bool unset = true, pending = true;                     // STATS: this half row / some row of the wave has met no key yet
 
-    if (t0 < t1) issue(t0, 0);
+#pragma unroll
+    for (int i = 0; i < NST - 1; ++i)
+        if (t0 + i < t1) issue(t0 + i);
     for (int t = t0; t < t1; ++t) {
-        const int cur = (t - t0) & 1;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the LDS-DMA of this tile, unknown to the compiler
-        if ((SUMS || BIAS) && tid < TILE) side[cur * TILE + tid] = sr;
-        __syncthreads();                                   // tile t stands; everyone has left tile t - 1
-        if (t + 1 < t1) issue(t + 1, cur ^ 1);
+        const int cur = t & (NST - 1);
+        // this tile's LDS-DMA has arrived, those of the NST - 2 tiles behind it may be on their way (the compiler knows of none)
+        if (t + NST - 2 < t1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 2) * PER) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      // tile t stands; everyone has left tile t - 1
+        if (t + NST - 1 < t1) issue(t + NST - 1);
         const char* ts = smem + cur * STAGE;
+        const float* sd = side + cur * 4 * TILE;
+        // edges: rows of the passing operand that do not exist, keys behind the query's last
+        const int p0 = t * TILE;
+        const bool edge = SUMS ? (p0 + TILE > p.Nq || (p.causal && s0 + 31 > p0 + off)) : (p0 + TILE > p.Nk || (p.causal && p0 + TILE - 1 > s0 + off));
+        // What the biases do to this tile, for all its keys at once: nothing (the rule: zeros), everything (all removed: no work), or some.
+        // Likewise a tile of queries that see no key (padding: z = inf).
+        bool plain = !BIAS;
+        if (BIAS && !SUMS) {
+            const float v = sd[lane];
+            if (__builtin_amdgcn_ballot_w64(v <= REMOVED || p0 + lane >= p.Nk) == ~0ull) continue;
+            plain = __builtin_amdgcn_ballot_w64(v != 0.f) == 0;
+        }
+        if (BIAS && SUMS) {
+            if (kall || __builtin_amdgcn_ballot_w64(sd[lane] == INFINITY) == ~0ull) continue;
+            plain = kplain;
+        }
+        for (bool take = !SUMS && pending;; take = true) { // STATS: a second time if a partial sum left the range; SUMS: once
+            f32x16 st[2];                                  // the half tiles' products: two independent chains
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-            f32x16 st;
+            for (int s = 0; s < NKS; ++s)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) st[i] = 0.f;
+                for (int g = 0; g < 2; ++g) {
+                    if (s == 0) {
 #pragma unroll
-            for (int s = 0; s < NKS; ++s) {
-                const bf16x8 pf = *reinterpret_cast<const bf16x8*>(ts + g * 32 * ROWB + roff[s]);
-                st = SUMS ? __builtin_amdgcn_mfma_f32_32x32x16_bf16(sf[s], pf, st, 0, 0, 0)
-                          : __builtin_amdgcn_mfma_f32_32x32x16_bf16(pf, sf[s], st, 0, 0, 0);
-            }
-            const int p0 = t * TILE + g * 32;              // first row of this half tile
-            const int q = SUMS ? p0 + r : s0 + r;          // the lane's query
-            const int key0 = (SUMS ? s0 : p0) + 4 * h;     // register i: key key0 + (i & 3) + 8 (i >> 2)
-            if (BIAS) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    if (SUMS) {
-                        st[i] = kb[i] == -INFINITY ? -INFINITY : st[i] + kb[i];
-                    } else {
-                        const float v = side[cur * TILE + g * 32 + 4 * h + (i & 3) + 8 * (i >> 2)];
-                        st[i] = v <= REMOVED ? -INFINITY : st[i] + v * HK_LOG2E;
+                        for (int i = 0; i < 16; ++i) st[g][i] = SUMS ? 0.f : -m;
                     }
+                    const bf16x8 pf = *reinterpret_cast<const bf16x8*>(ts + g * 32 * ROWB + (ro ^ (32 * s)));
+                    st[g] = SUMS ? __builtin_amdgcn_mfma_f32_32x32x16_bf16(sf[s], pf, st[g], 0, 0, 0)
+                                 : __builtin_amdgcn_mfma_f32_32x32x16_bf16(pf, sf[s], st[g], 0, 0, 0);
                 }
+            if (!plain) {
+#pragma unroll
+                for (int g = 0; g < 2; ++g)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        if (SUMS) {
+                            st[g][i] = kb[i] == -INFINITY ? -INFINITY : st[g][i] + kb[i];
+                        } else {
+                            const float v = sd[g * 32 + 4 * h + (i & 3) + 8 * (i >> 2)];
+                            st[g][i] = v <= REMOVED ? -INFINITY : st[g][i] + v * HK_LOG2E;
+                        }
+                    }
             }
-            const int lim = p.causal ? min(p.Nk - 1, q + off) : p.Nk - 1;    // last key the query sees
-            const bool edge = SUMS ? (p0 + 32 > p.Nq || (p.causal && s0 + 31 > p0 + off)) : (p0 + 32 > p.Nk || (p.causal && p0 + 31 > s0 + off));
             if (edge) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (key0 + (i & 3) + 8 * (i >> 2) > lim || (SUMS && q >= p.Nq)) st[i] = -INFINITY;
+                for (int g = 0; g < 2; ++g) {
+                    const int q = SUMS ? p0 + g * 32 + r : s0 + r;                           // the lane's query
+                    int lim = p.causal ? min(p.Nk - 1, q + off) : p.Nk - 1;                  // last key it sees
+                    if (SUMS && q >= p.Nq) lim = -1;
+                    lim -= (SUMS ? s0 : p0 + g * 32) + 4 * h;                                // register i: key (i & 3) + 8 (i >> 2) from here
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if ((i & 3) + 8 * (i >> 2) > lim) st[g][i] = -INFINITY;
+                }
             }
             if (SUMS) {
-                const float zq = side[cur * TILE + g * 32 + r];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) acc[i] += __builtin_amdgcn_exp2f(st[i] - zq);
-            } else {
-                float mx = fmaxf(st[0], st[1]);
+                for (int g = 0; g < 2; ++g) {
+                    const float zq = sd[g * 32 + r];
 #pragma unroll
-                for (int i = 2; i < 16; i += 2) mx = fmaxf(mx, fmaxf(st[i], st[i + 1]));
-                if (__builtin_amdgcn_ballot_w64(mx > m + 8.f)) {
-                    const float mn = fmaxf(m, mx);
-                    l *= __builtin_amdgcn_exp2f(m - mn);
-                    m = mn;
+                    for (int i = 0; i < 16; ++i) acc[i] += __builtin_amdgcn_exp2f(st[g][i] - zq);
                 }
+                break;
+            }
+            if (take) {
+                float mx = fmaxf(st[0][0], st[1][0]);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) l += __builtin_amdgcn_exp2f(st[i] - m);
+                for (int i = 1; i < 16; ++i) mx = fmaxf(mx, fmaxf(st[0][i], st[1][i]));
+                const float delta = unset ? (mx == -INFINITY ? 0.f : mx) : fmaxf(mx, 0.f);
+                l *= unset ? 0.f : __builtin_amdgcn_exp2f(-delta);
+                unset = unset && mx == -INFINITY;
+                pending = __builtin_amdgcn_ballot_w64(unset) != 0;
+                m += delta;
+#pragma unroll
+                for (int g = 0; g < 2; ++g)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) st[g][i] -= delta;
+            }
+            float rs = 0.f;
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) rs += __builtin_amdgcn_exp2f(st[g][i]);
+            if (take || __builtin_amdgcn_ballot_w64(!(rs <= OVERFLOW_SUM)) == 0) {
+                l += rs;
+                break;
             }
         }
     }
     if (SUMS) {
+        // over the 32 lanes of a half: each step sends the half of the values that the partner lane keeps; value r & 15 ends in lane r
+        auto halve = [&](auto o_c) {
+            constexpr int o = decltype(o_c)::value;
+            const bool up = (r & o) != 0;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[i] += __shfl_xor(acc[i], o, 64);
-        const float* wi = p.w_in ? p.w_in + (int64_t)b * p.wi_bs + (int64_t)head * p.wi_hs : nullptr;
-        float* wo = p.w_out + (int64_t)b * p.wo_bs + (int64_t)head * p.wo_hs;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int key = s0 + (i & 3) + 8 * (i >> 2) + 4 * h;
-            if (r == i && key < p.Nk) wo[key] = (wi ? wi[key] : 0.f) + acc[i];
+            for (int i = 0; i < o; ++i) {
+                const float keep = up ? acc[i + o] : acc[i], send = up ? acc[i] : acc[i + o];
+                acc[i] = keep + __shfl_xor(send, o, 64);
+            }
+        };
+        halve(std::integral_constant<int, 8>{});
+        halve(std::integral_constant<int, 4>{});
+        halve(std::integral_constant<int, 2>{});
+        halve(std::integral_constant<int, 1>{});
+        acc[0] += __shfl_xor(acc[0], 16, 64);
+        const int key = s0 + (r & 3) + 8 * ((r & 15) >> 2) + 4 * h;
+        if (r < 16 && key < p.Nk) {
+            const int64_t at = (int64_t)b * p.wi_bs + (int64_t)head * p.wi_hs + key;
+            p.w_out[(int64_t)b * p.wo_bs + (int64_t)head * p.wo_hs + key] = (p.w_in ? p.w_in[at] : 0.f) + acc[0];
         }
     } else {
+        if (unset) m = -1.0e30f;                           // this lane half met no key
         const float mo = __shfl_xor(m, 32, 64), lo = __shfl_xor(l, 32, 64);
         const float M = fmaxf(m, mo);
         const float sum = l * __builtin_amdgcn_exp2f(m - M) + lo * __builtin_amdgcn_exp2f(mo - M);
@@ -174,20 +248,22 @@ __global__ __launch_bounds__(256, 2) void hk_key_weights_kernel(const KeyWeightP
 
 template <int HD, bool SUMS, bool BIAS>
 int launch_key_weights(KeyWeightParams p, hipStream_t s) {
-    constexpr int LDS = 2 * TILE * HD * 2 + 2 * TILE * 4;
+    constexpr int LDS = NST * (TILE * HD * 2 + 4 * TILE * 4);
+    static std::atomic<unsigned long long> attr_done{0};   // per device
+    const hipError_t e = hk_lds_attr_once(attr_done, reinterpret_cast<const void*>(&hk_key_weights_kernel<HD, SUMS, BIAS>), LDS);
+    if (e != hipSuccess) {
+        hk_set_error("hk_attn_key_weights_bf16: hipFuncSetAttribute(%d B LDS): %s", LDS, hipGetErrorString(e));
+        return HK_ELAUNCH;
+    }
     p.nblk = ((SUMS ? p.Nk : p.Nq) + BLK - 1) / BLK;
     hipLaunchKernelGGL((hk_key_weights_kernel<HD, SUMS, BIAS>), dim3((unsigned)((int64_t)p.nblk * p.B * p.H)), dim3(256), LDS, s, p);
     return HK_OK;
 }
 template <int HD>
-void launch_both(const KeyWeightParams& p, hipStream_t s) {
-    if (p.bias) {
-        launch_key_weights<HD, false, true>(p, s);
-        launch_key_weights<HD, true, true>(p, s);
-    } else {
-        launch_key_weights<HD, false, false>(p, s);
-        launch_key_weights<HD, true, false>(p, s);
-    }
+int launch_both(const KeyWeightParams& p, hipStream_t s) {
+    const int rc = p.bias ? launch_key_weights<HD, false, true>(p, s) : launch_key_weights<HD, false, false>(p, s);
+    if (rc != HK_OK) return rc;
+    return p.bias ? launch_key_weights<HD, true, true>(p, s) : launch_key_weights<HD, true, false>(p, s);
 }
 
 // ---------------------------------------------------------------- eviction
@@ -202,7 +278,7 @@ struct EvictParams {
 };
 
 constexpr int SEL_T = 1024;
-constexpr int SEL_LDS = 12288;       // keys whose ranks fit the workgroup's LDS
+constexpr int REG_KEYS = 16 * 1024;  // keys per (sequence, head) up to which a workgroup keeps all ranks in registers
 
 // fp32 -> a whole number that orders like it: removed < NaN < -inf < ... < -0 = 0 < ... < inf < recent
 __device__ __forceinline__ uint32_t rank_of(float w, bool removed, bool recent) {
@@ -213,12 +289,149 @@ __device__ __forceinline__ uint32_t rank_of(float w, bool removed, bool recent) 
     return recent ? 0xffffffffu : k;
 }
 
-// One workgroup per (sequence, head): the budget-th largest rank by four rounds of an 8-bit histogram, then one ordered pass that
-// keeps the ranks above it and, of those equal, the first ones; indices, weights and biases move with it (a round's values are in
-// registers before any of its stores, and go to places at or below the ones they came from: in place is safe).
-template <bool IN_LDS>
+// Kept rows within one (sequence, head), walked upwards by a workgroup of T threads.  Row `at` comes from src(at) >= at, so a step's stores
+// can only hit sources of the same or an earlier step: all of a step's loads have arrived before its first store.  Not in place: copied.
+template <int HD, int T, typename Src>
+__device__ __forceinline__ void move_rows(const EvictParams& p, int b, int head, bool is_v, Src src) {
+    constexpr int CH = HD / 8, RPS = T / CH, U = 8;
+    const int col = head * HD + ((int)threadIdx.x % CH) * 8, g = threadIdx.x / CH;
+    const __bf16* from = is_v ? p.V + (int64_t)b * p.bsv + col : p.K + (int64_t)b * p.bsk + col;
+    __bf16* to = is_v ? p.VO + (int64_t)b * p.bsvo + col : p.KO + (int64_t)b * p.bsko + col;
+    const int64_t ldf = is_v ? p.ldv : p.ldk, ldt = is_v ? p.ldvo : p.ldko;
+    for (int r0 = 0; r0 < p.budget; r0 += RPS * U) {
+        u32x4 x[U];
+        int s[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            s[u] = src(min(r0 + u * RPS + g, p.budget - 1));
+            x[u] = *reinterpret_cast<const u32x4*>(from + (int64_t)s[u] * ldf);
+        }
+        if (p.in_place) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int at = r0 + u * RPS + g;
+            if (at < p.budget && !(p.in_place && s[u] == at)) *reinterpret_cast<u32x4*>(to + (int64_t)at * ldt) = x[u];
+        }
+    }
+}
+
+// One workgroup per (sequence, head), every rank in a register (key u * T + thread in slot u).  The budget-th largest rank is found bit by
+// bit: count the ranks at or above the candidate (a comparison, a ballot and a bit count per slot; the waves add up through LDS), keep the
+// bit if there are enough; done as soon as there are exactly enough.  An ordered pass then keeps the ranks above the threshold and, of those
+// equal to it, the first ones: positions from a scan over the (slot, wave) counts.  Weights and biases move through registers (in place is
+// safe), and MOVE != 0 moves K and V in the same launch.
+template <int T, int KPT, int HD, bool MOVE>
+__global__ __launch_bounds__(T) void hk_evict_kernel(const EvictParams p) {
+    constexpr int NW = T / 64, NC = KPT * NW;              // (slot, wave) pairs
+    static_assert(NC <= 256, "one wave scans four counts per lane");
+    __shared__ uint32_t part[2][NW];
+    __shared__ uint32_t cnt[NC];
+    extern __shared__ uint16_t rows[];                     // MOVE: [budget] the kept rows
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int b = blockIdx.x / p.H, head = blockIdx.x - b * p.H;
+    const float* w = p.w + (int64_t)b * p.w_bs + (int64_t)head * p.w_hs;
+    const float* bias = p.bias ? p.bias + (int64_t)b * p.b_bs + (int64_t)head * p.b_hs : nullptr;
+    float* wo = p.w_out + (int64_t)b * p.wo_bs + (int64_t)head * p.wo_hs;
+    float* bo = p.bias ? p.bias_out + (int64_t)b * p.bo_bs + (int64_t)head * p.bo_hs : nullptr;
+    int32_t* kept = p.kept + (int64_t)blockIdx.x * p.budget;
+    float wv[KPT], bv[KPT];
+    uint32_t k[KPT];
+#pragma unroll
+    for (int u = 0; u < KPT; ++u) {
+        const int j = min(u * T + tid, p.n - 1);
+        wv[u] = w[j];
+        bv[u] = bias ? bias[j] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < KPT; ++u) {
+        const int j = u * T + tid;
+        k[u] = rank_of(wv[u], bv[u] <= REMOVED, j >= p.n - p.recent);
+        if (j >= p.n) k[u] = 0u;                           // behind the last key: never counted (candidates are above 0), never kept
+    }
+    const uint32_t want = (uint32_t)p.budget;
+    uint32_t thr = 0;                                      // the largest value that at least `want` ranks reach, so far
+    bool exact = false;
+    for (int bit = 31; bit >= 0 && !exact; --bit) {
+        const uint32_t cand = thr | (1u << bit);
+        uint32_t c = 0;
+#pragma unroll
+        for (int u = 0; u < KPT; ++u) c += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(k[u] >= cand));
+        if (lane == 0) part[bit & 1][wave] = c;            // two turns: the next round's counts do not meet this round's readers
+        __syncthreads();
+        c = 0;
+#pragma unroll
+        for (int x = 0; x < NW; ++x) c += part[bit & 1][x];
+        if (c >= want) thr = cand;
+        exact = c == want;
+    }
+    // ranks above thr - all of them are kept - and those equal to it, of which the first `want - above` are
+    uint64_t ga[KPT], ge[KPT];
+#pragma unroll
+    for (int u = 0; u < KPT; ++u) {
+        const bool in = u * T + tid < p.n;
+        ga[u] = __builtin_amdgcn_ballot_w64(in && k[u] > thr);
+        ge[u] = __builtin_amdgcn_ballot_w64(in && k[u] == thr);
+        if (lane == 0) cnt[u * NW + wave] = (uint32_t)__popcll(ga[u]) | (uint32_t)__popcll(ge[u]) << 16;   // at most 2^14 of each in all
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // every weight and bias is in a register before any is stored
+    __syncthreads();
+    if (wave == 0) {
+        constexpr int CPL = (NC + 63) / 64;
+        uint32_t c[CPL], s = 0;
+#pragma unroll
+        for (int i = 0; i < CPL; ++i) {
+            c[i] = lane * CPL + i < NC ? cnt[lane * CPL + i] : 0u;
+            s += c[i];
+        }
+        uint32_t before = s;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t x = __shfl_up(before, o, 64);
+            if (lane >= o) before += x;
+        }
+        if (lane == 63) part[0][0] = before & 0xffffu;     // ranks above thr in all
+        before -= s;
+#pragma unroll
+        for (int i = 0; i < CPL; ++i) {
+            if (lane * CPL + i < NC) cnt[lane * CPL + i] = before;
+            before += c[i];
+        }
+    }
+    __syncthreads();
+    const uint32_t ties = want - part[0][0];
+    const uint64_t lower = (1ull << lane) - 1;
+#pragma unroll
+    for (int u = 0; u < KPT; ++u) {
+        const int j = u * T + tid;
+        const uint32_t base = cnt[u * NW + wave];
+        const uint32_t ba = (base & 0xffffu) + (uint32_t)__popcll(ga[u] & lower), be = (base >> 16) + (uint32_t)__popcll(ge[u] & lower);
+        if (j < p.n && (k[u] > thr || (k[u] == thr && be < ties))) {
+            const uint32_t at = ba + min(be, ties);
+            kept[at] = j;
+            wo[at] = wv[u];
+            if (bo) bo[at] = bv[u];
+            if (MOVE) rows[at] = (uint16_t)j;
+        }
+    }
+    if (p.in_place)                                        // the places that became free: nothing collected, nothing removed
+        for (int j = p.budget + tid; j < p.n; j += T) {
+            wo[j] = 0.f;
+            if (bo) bo[j] = 0.f;
+        }
+    if (MOVE) {
+        __syncthreads();
+        auto src = [&](int at) { return (int)rows[at]; };
+        move_rows<HD, T>(p, b, head, false, src);
+        move_rows<HD, T>(p, b, head, true, src);
+    }
+}
+
+// More keys than registers hold: the budget-th largest rank by four rounds of an 8-bit histogram over the weights in memory, then the ordered
+// pass chunk by chunk (a chunk's values are in registers before any of its stores, and go to places at or below the ones they came from).
 __global__ __launch_bounds__(SEL_T) void hk_evict_select_kernel(const EvictParams p) {
-    extern __shared__ uint32_t ranks[];
     __shared__ uint32_t hist[256];
     __shared__ uint32_t pick[2];
     __shared__ uint32_t wsum[SEL_T / 64];
@@ -230,15 +443,12 @@ __global__ __launch_bounds__(SEL_T) void hk_evict_select_kernel(const EvictParam
     float* bo = p.bias ? p.bias_out + (int64_t)b * p.bo_bs + (int64_t)head * p.bo_hs : nullptr;
     int32_t* kept = p.kept + (int64_t)blockIdx.x * p.budget;
     auto rank_at = [&](int j) { return rank_of(w[j], bias && bias[j] <= REMOVED, j >= p.n - p.recent); };
-    if (IN_LDS) {
-        for (int j = tid; j < p.n; j += SEL_T) ranks[j] = rank_at(j);
-    }
     uint32_t prefix = 0, want = (uint32_t)p.budget;        // the want-th largest of the ranks that begin with prefix
     for (int shift = 24; shift >= 0; shift -= 8) {
         if (tid < 256) hist[tid] = 0;
         __syncthreads();
         for (int j = tid; j < p.n; j += SEL_T) {
-            const uint32_t k = IN_LDS ? ranks[j] : rank_at(j);
+            const uint32_t k = rank_at(j);
             if (shift == 24 || (k >> (shift + 8)) == prefix) atomicAdd(&hist[(k >> shift) & 255u], 1u);
         }
         __syncthreads();
@@ -274,7 +484,7 @@ __global__ __launch_bounds__(SEL_T) void hk_evict_select_kernel(const EvictParam
     for (int j0 = 0; j0 < p.n; j0 += SEL_T) {
         const int j = j0 + tid;
         const bool in = j < p.n;
-        const uint32_t k = !in ? 0u : IN_LDS ? ranks[j] : rank_at(j);
+        const uint32_t k = in ? rank_at(j) : 0u;
         const float wv = in ? w[j] : 0.f, bv = in && bias ? bias[j] : 0.f;
         const uint64_t ga = __builtin_amdgcn_ballot_w64(in && k > prefix), ge = __builtin_amdgcn_ballot_w64(in && k == prefix);
         const uint64_t lower = (1ull << lane) - 1;
@@ -301,7 +511,7 @@ __global__ __launch_bounds__(SEL_T) void hk_evict_select_kernel(const EvictParam
         }
         __syncthreads();
     }
-    if (p.in_place)                                        // the places that became free: nothing collected, nothing removed
+    if (p.in_place)
         for (int j = p.budget + tid; j < p.n; j += SEL_T) {
             wo[j] = 0.f;
             if (bo) bo[j] = 0.f;
@@ -338,34 +548,43 @@ __global__ __launch_bounds__(256) void hk_evict_copy_kernel(const EvictParams p)
         }
 }
 
-// Rows within the cache: one workgroup per (sequence, head, K or V) walks the kept rows upwards.  Row `at` comes from kept[at] >= at, so
-// a step's stores can only hit sources of the same or an earlier step: all of a step's loads have arrived before its first store.
+// Rows within the cache, the kept list in memory: one workgroup per (sequence, head, K or V).
 template <int HD>
 __global__ __launch_bounds__(512) void hk_evict_move_kernel(const EvictParams p) {
-    constexpr int CH = HD / 8, RPS = 512 / CH, U = 8;
     const int bh = blockIdx.x >> 1, b = bh / p.H, head = bh - b * p.H;
-    const bool is_v = blockIdx.x & 1;
-    const int64_t ld = is_v ? p.ldvo : p.ldko;
-    __bf16* base = (is_v ? p.VO + (int64_t)b * p.bsvo : p.KO + (int64_t)b * p.bsko) + head * HD + (threadIdx.x % CH) * 8;
     const int32_t* kept = p.kept + (int64_t)bh * p.budget;
-    const int g = threadIdx.x / CH;
-    for (int r0 = 0; r0 < p.budget; r0 += RPS * U) {
-        u32x4 x[U];
-        int src[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int at = r0 + u * RPS + g;
-            src[u] = kept[min(at, p.budget - 1)];
-            x[u] = *reinterpret_cast<const u32x4*>(base + (int64_t)src[u] * ld);
-        }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int at = r0 + u * RPS + g;
-            if (at < p.budget && src[u] != at) *reinterpret_cast<u32x4*>(base + (int64_t)at * ld) = x[u];
-        }
+    move_rows<HD, 512>(p, b, head, blockIdx.x & 1, [&](int at) { return kept[at]; });
+}
+
+template <int T, int KPT, int HD, bool MOVE>
+int launch_evict(const EvictParams& p, hipStream_t s) {
+    hipLaunchKernelGGL((hk_evict_kernel<T, KPT, HD, MOVE>), dim3((unsigned)(p.B * p.H)), dim3(T), MOVE ? (size_t)p.budget * 2 : 0, s, p);
+    return HK_OK;
+}
+template <int HD, bool MOVE>
+int launch_evict_any(const EvictParams& p, hipStream_t s) {
+    if (p.n <= 512) return launch_evict<256, 2, HD, MOVE>(p, s);
+    if (p.n <= 2048) return launch_evict<256, 8, HD, MOVE>(p, s);
+    if (p.n <= 4096) return launch_evict<512, 8, HD, MOVE>(p, s);
+    return launch_evict<1024, 16, HD, MOVE>(p, s);
+}
+template <int HD>
+int launch_evict_all(const EvictParams& p, hipStream_t s) {
+    const unsigned pairs = (unsigned)(p.B * p.H);
+    // One launch or two?  A workgroup per pair moves its rows in pieces of one head; the copy kernel writes whole rows with the whole chip
+    // (5.5 TB/s against 4.6) and costs a launch.  128 pairs (353 keys to 256): 12 us against 13.7 and the gap; 512 pairs (2047 to 1024): 119
+    // against 114.5.  In place only the pair's own workgroup knows when a row may be overwritten.
+    if (p.n <= REG_KEYS && (p.in_place || pairs <= 256)) return launch_evict_any<HD, true>(p, s);
+    if (p.n <= REG_KEYS) launch_evict_any<HD, false>(p, s);
+    else hipLaunchKernelGGL(hk_evict_select_kernel, dim3(pairs), dim3(SEL_T), 0, s, p);
+    if (p.in_place) {
+        hipLaunchKernelGGL((hk_evict_move_kernel<HD>), dim3(pairs * 2), dim3(512), 0, s, p);
+    } else {
+        const int64_t pieces = (int64_t)p.B * p.H * p.budget, per = 256 / (HD / 8) * 2;
+        HK_REQUIRE((pieces + per - 1) / per < (1LL << 31), "hk_cache_evict_bf16: grid too large");
+        hipLaunchKernelGGL((hk_evict_copy_kernel<HD>), dim3((unsigned)((pieces + per - 1) / per)), dim3(256), 0, s, p);
     }
+    return HK_OK;
 }
 
 }  // namespace
@@ -378,6 +597,7 @@ extern "C" int hk_attn_key_weights_bf16(const hk_key_weights_desc* d, void* stre
                d->Nq, d->Nk, d->head_dim);
     HK_REQUIRE(((d->ldq | d->bsq | d->ldk | d->bsk) & 7) == 0 && d->ldq >= 0 && d->bsq >= 0 && d->ldk >= 0 && d->bsk >= 0,
                "hk_attn_key_weights_bf16: strides must be multiples of 8 elements, not negative");
+    HK_REQUIRE(d->ldq < (1 << 25) && d->ldk < (1 << 25), "hk_attn_key_weights_bf16: token strides of 2^25 elements and more are not supported");
     HK_REQUIRE(((uintptr_t)d->Q | (uintptr_t)d->K) % 16 == 0 &&
                    ((uintptr_t)d->key_bias | (uintptr_t)d->w_in | (uintptr_t)d->w_out | (uintptr_t)d->ws) % 4 == 0,
                "hk_attn_key_weights_bf16: operands must be 16-byte aligned");
@@ -423,8 +643,8 @@ extern "C" int hk_attn_key_weights_bf16(const hk_key_weights_desc* d, void* stre
     p.wo_bs = d->wo_bs;
     p.wo_hs = d->wo_hs;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    if (d->head_dim == 128) launch_both<128>(p, s);
-    else launch_both<64>(p, s);
+    const int rc = d->head_dim == 128 ? launch_both<128>(p, s) : launch_both<64>(p, s);
+    if (rc != HK_OK) return rc;
     HK_CHECK_LAUNCH("hk_attn_key_weights_bf16");
     return HK_OK;
 }
@@ -504,19 +724,8 @@ extern "C" int hk_cache_evict_bf16(const hk_cache_evict_desc* d, void* stream) {
     p.bo_bs = d->bo_bs;
     p.bo_hs = d->bo_hs;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    const unsigned pairs = (unsigned)(p.B * p.H);
-    if (p.n <= SEL_LDS) hipLaunchKernelGGL((hk_evict_select_kernel<true>), dim3(pairs), dim3(SEL_T), (size_t)p.n * 4, s, p);
-    else hipLaunchKernelGGL((hk_evict_select_kernel<false>), dim3(pairs), dim3(SEL_T), 0, s, p);
-    if (in_place) {
-        if (d->head_dim == 128) hipLaunchKernelGGL((hk_evict_move_kernel<128>), dim3(pairs * 2), dim3(512), 0, s, p);
-        else hipLaunchKernelGGL((hk_evict_move_kernel<64>), dim3(pairs * 2), dim3(512), 0, s, p);
-    } else {
-        const int64_t pieces = (int64_t)p.B * p.H * p.budget, per = 256 / (d->head_dim / 8) * 2;
-        HK_REQUIRE((pieces + per - 1) / per < (1LL << 31), "hk_cache_evict_bf16: grid too large");
-        const unsigned grid = (unsigned)((pieces + per - 1) / per);
-        if (d->head_dim == 128) hipLaunchKernelGGL((hk_evict_copy_kernel<128>), dim3(grid), dim3(256), 0, s, p);
-        else hipLaunchKernelGGL((hk_evict_copy_kernel<64>), dim3(grid), dim3(256), 0, s, p);
-    }
+    const int rc = d->head_dim == 128 ? launch_evict_all<128>(p, s) : launch_evict_all<64>(p, s);
+    if (rc != HK_OK) return rc;
     HK_CHECK_LAUNCH("hk_cache_evict_bf16");
     return HK_OK;
 }

@@ -230,7 +230,8 @@ def _ref_evict(w, bias, n, budget, recent):
 @pytest.mark.parametrize("B,n,budget,recent,H,hd,masked", [
     (1, 1, 1, 0, 1, 64, False), (1, 2, 1, 0, 2, 128, False), (1, 2, 1, 1, 1, 64, True), (2, 353, 256, 64, 4, 128, False), (3, 100, 100, 0, 2, 64, True),
     (2, 1025, 512, 512, 3, 128, True), (1, 2049, 1, 0, 2, 64, False), (2, 2500, 1111, 7, 2, 128, True), (1, 13000, 900, 100, 1, 64, True),
-    (4, 64, 63, 0, 5, 64, False)])
+    (4, 64, 63, 0, 5, 64, False), (1, 512, 300, 9, 2, 128, True), (2, 2048, 2000, 0, 1, 64, True), (1, 4096, 17, 3, 2, 64, True),
+    (1, 16384, 16000, 1, 1, 64, False), (2, 17000, 5000, 33, 1, 128, True)])
 @pytest.mark.parametrize("inplace", [False, True])
 def test_cache_evict_keeps_the_heaviest_rows(B, n, budget, recent, H, hd, masked, inplace):
     rows = n + 6
