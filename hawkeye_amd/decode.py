@@ -21,7 +21,7 @@ import torch
 from . import lib as L
 from . import ops
 from .engine import _Pool
-from .llm import LOG2E, LlamaPrefill
+from .llm import LOG2E, LlamaPrefill, PromptPrefix
 
 MAX_ROWS = 16          # sequences per step hk_gemv_bf16 takes
 ROW_GRANULE = 64       # cache rows are allocated in multiples of this, so nearby prompt lengths share one plan
@@ -35,6 +35,8 @@ class _DecodePlan:
         self.ws: Dict[str, torch.Tensor] = {}
         self.steps: List[Tuple] = []       # (fn, args list, kind, name)
         self.keep: List = []
+        self.prefix_descs: List = []       # hk_prefix_attn_desc per layer: Nk is set per step, KP / VP per call
+        self.weight_descs: List = []       # hk_step_weights_desc per layer: n_keys is set per step
         self.pool_epoch = 0
 
 
@@ -68,7 +70,7 @@ class LlamaGenerator:
                 for k, v in prefill.w.items():
                     if k == "lm_head" or k.endswith((".qkv", ".o", ".gu", ".down")):
                         self.wt[k] = ops.tile_gemv_weight(v)
-        self.plans: Dict[Tuple[int, int, bool], _DecodePlan] = {}
+        self.plans: Dict[Tuple[int, int, bool, int, bool], _DecodePlan] = {}    # (B, rows, masked, prefix rows, with key weights)
         self.k_cache: Optional[torch.Tensor] = None     # [layers, B, rows, D] views of the last call (inspection / tests)
         self.v_cache: Optional[torch.Tensor] = None
 
@@ -76,20 +78,20 @@ class LlamaGenerator:
         return self.pool.nbytes()
 
     # ------------------------------------------------------------------ plan
-    def _plan_for(self, B: int, rows: int, masked: bool) -> _DecodePlan:
-        key = (B, rows, masked)
+    def _plan_for(self, B: int, rows: int, masked: bool, P: int = 0, weights: bool = False) -> _DecodePlan:
+        key = (B, rows, masked, P, weights)
         plan = self.plans.get(key)
         if plan is not None and plan.pool_epoch == self.pool.epoch:
             return plan
         epoch = self.pool.epoch
-        plan = self._build_plan(B, rows, masked)
+        plan = self._build_plan(B, rows, masked, P, weights)
         if self.pool.epoch != epoch:
             self.plans.clear()
         plan.pool_epoch = self.pool.epoch
         self.plans[key] = plan
         return plan
 
-    def _build_plan(self, B: int, rows: int, masked: bool) -> _DecodePlan:
+    def _build_plan(self, B: int, rows: int, masked: bool, P_rows: int = 0, weights: bool = False) -> _DecodePlan:
         cfg, w = self.cfg, self.pre.w
         D, I, H, hd, Lyr, V = (cfg.hidden_size, cfg.intermediate_size, cfg.num_attention_heads, cfg.head_dim,
                                cfg.num_hidden_layers, cfg.vocab_size)
@@ -109,6 +111,13 @@ class LlamaGenerator:
             ws["att"] = buf("att", (B, D), bf16)
             ws["act"] = buf("act", (B, I), bf16)
             ws["logits"] = buf("logits", (B, (V + 3) // 4 * 4), f32)[:, :V]      # rows 16-byte aligned whatever V is
+            if weights:
+                ws["kw"] = buf("kw", (Lyr, B, H, rows), f32)                     # what the keys have collected
+                ws["kbias_h"] = buf("kbias_h", (Lyr, B, H, rows), f32) if masked else None    # per head: heads keep different rows
+            if P_rows or weights:      # one workspace for all layers (they run one after another), enough for every length of the own keys
+                need = max(ops.prefix_attention_ws(B, H, 1, P_rows, n, hd) if P_rows else self.lib.hk_decode_attn_weights_ws(B, H, hd, n)
+                           for n in range(1, rows + 1))
+                aws = buf("attn_ws", (need,), torch.uint8)
         P = lambda t: t.data_ptr()  # noqa: E731
         x, xn, qkv, q, att, act = (P(ws[k]) for k in ("x", "xn", "qkv", "q", "att", "act"))
         qscale = (hd ** -0.5) * LOG2E
@@ -141,7 +150,22 @@ class LlamaGenerator:
             o = f"l{i}."
             kc, vc = P(ws["kc"][i]), P(ws["vc"][i])
             normed_gemv(w[o + "n1"], o + "qkv", qkv, 3 * D)
-            if self.fused_attn:
+            if P_rows or weights:
+                # args 4 (pos_add) and 11 (slot) are set per step
+                steps.append((lib.hk_decode_rope_append, [qkv, P(w["cos"]), P(w["sin"]), P(ws["pos0"]), 0, q, kc, vc, B, H, hd, 0, rows,
+                                                          cfg.max_position_embeddings, qscale], _ROPE, "hk_decode_rope_append"))
+                if P_rows:
+                    d = L.HkPrefixAttnDesc(q, None, None, kc, vc, att, P(ws["kbias"]) if masked else None, P(aws), aws.numel(), B, H, 1, P_rows, 1,
+                                           hd, D, D, D, D, D, rows * D, D, rows * D, D, D, rows if masked else 0)
+                    plan.prefix_descs.append(d)
+                    steps.append((lib.hk_prefix_attn_bf16, [C.byref(d)], _STATIC, "hk_prefix_attn_bf16"))
+                else:
+                    kw = P(ws["kw"][i])
+                    d = L.HkStepWeightsDesc(q, kc, vc, P(ws["kbias_h"][i]) if masked else None, kw, kw, att, P(aws), aws.numel(), B, H, hd, 1, rows,
+                                            H * rows if masked else 0, rows if masked else 0, H * rows, rows, H * rows, rows)
+                    plan.weight_descs.append(d)
+                    steps.append((lib.hk_decode_attn_weights_bf16, [C.byref(d)], _STATIC, "hk_decode_attn_weights_bf16"))
+            elif self.fused_attn:
                 # rotary + cache append + attention in one launch; args 4 (pos_add) and 12 (slot) are set per step
                 steps.append((lib.hk_decode_attn_rope_bf16, [qkv, P(w["cos"]), P(w["sin"]), P(ws["pos0"]), 0, kc, vc,
                                                              P(ws["kbias"]) if masked else None, att, B, H, hd, 0, rows, rows,
@@ -161,15 +185,19 @@ class LlamaGenerator:
         steps.append((lib.hk_argmax_f32, [P(ws["logits"]), P(ws["tok"]), B, V, ws["logits"].stride(0)], _STATIC, "hk_argmax_f32"))
         return plan
 
-    def _step(self, plan: _DecodePlan, t: int, S: int, stream: int):
-        """Decode step t: consumes token t (ws['tok']) at cache row S + t, leaves logits and token t + 1."""
+    def _step(self, plan: _DecodePlan, t: int, slot: int, stream: int):
+        """Decode step t: consumes token t (ws['tok']) at cache row `slot`, leaves logits and token t + 1."""
+        for d in plan.prefix_descs:
+            d.Nk = slot + 1
+        for d in plan.weight_descs:
+            d.n_keys = slot + 1
         for fn, args, kind, name in plan.steps:
             if kind == _ROPE:
-                args[4], args[11] = t, S + t
+                args[4], args[11] = t, slot
             elif kind == _ATTN:
-                args[8] = S + t + 1
+                args[8] = slot + 1
             elif kind == _FUSED:
-                args[4], args[12] = t, S + t
+                args[4], args[12] = t, slot
             rc = fn(*args, stream)
             if rc != 0:
                 L.check(rc, name)
@@ -181,7 +209,8 @@ class LlamaGenerator:
                  max_new_tokens: int = 20, stop_sequences: Optional[Sequence[Sequence[int]]] = None,
                  eos_token_id: Optional[int] = None, pad_token_id: int = 0, forced_tokens: Optional[torch.Tensor] = None,
                  next_token_fn=None,
-                 return_logits: bool = False, sync_every: int = 1):
+                 return_logits: bool = False, sync_every: int = 1, prefix: Optional[PromptPrefix] = None,
+                 cache_budget: Optional[int] = None, cache_recent: Optional[int] = None):
         """Prompt arguments as LlamaPrefill.prefill (a mask, if given, must be all ones or LEFT-padded).  Greedy decoding:
         token 0 is the arg-max of the prefill's last-position logits, token t + 1 of decode step t's.
         stop_sequences: generation ends once the generated tokens of ROW 0 end with one of them (StoppingCriteriaSub,
@@ -196,6 +225,11 @@ class LlamaGenerator:
         forward of every step is still the HIP path.
         sync_every: the host looks at the new tokens every this many steps (1 = the reference's per-token check; larger
         values decode up to sync_every - 1 tokens past a stop and cut them off -- same output, fewer host round trips).
+        prefix: what all prompts of the batch continue (LlamaPrefill.make_prefix: several questions about one clip).  Its keys exist and are
+        read once for the batch, in the prefill and in every step; src then holds what follows it.
+        cache_budget: the sequences' caches are cut to this many rows per layer and head whenever they have outgrown it by ROW_GRANULE (the
+        prompt's at once): the last cache_recent rows (default: half of the budget) and those that have collected the most attention
+        weight stay.  Not together with prefix (cut the prefix itself: make_prefix(budget=)).
         Returns {"tokens": int64 [B, T] (T <= max_new_tokens), "logits": fp32 [T, B, V] if return_logits}."""
         cfg = self.cfg
         if max_new_tokens < 1:
@@ -206,8 +240,21 @@ class LlamaGenerator:
         B, S = int(ref.shape[0]), int(ref.shape[1])
         if B > MAX_ROWS:
             raise RuntimeError(f"generate: {B} sequences; the decode step takes at most {MAX_ROWS}")
-        if S + max_new_tokens > cfg.max_position_embeddings:
-            raise RuntimeError(f"generate: prompt {S} + {max_new_tokens} new tokens exceeds max_position_embeddings "
+        p0 = 0
+        if prefix is not None:
+            if cache_budget is not None:
+                raise RuntimeError("generate: prefix and cache_budget together; cut the prefix itself (make_prefix(budget=))")
+            self.pre._check_prefix(prefix)
+            p0 = prefix.n_positions
+        if cache_budget is not None:
+            if cache_recent is None:
+                cache_recent = cache_budget // 2
+            if not (1 <= cache_budget and 0 <= cache_recent <= cache_budget):
+                raise RuntimeError(f"generate: cache_budget={cache_budget}, cache_recent={cache_recent} (1 <= budget, 0 <= recent <= budget)")
+        elif cache_recent is not None:
+            raise RuntimeError("generate: cache_recent needs cache_budget")
+        if p0 + S + max_new_tokens > cfg.max_position_embeddings:
+            raise RuntimeError(f"generate: prompt {p0 + S} + {max_new_tokens} new tokens exceeds max_position_embeddings "
                                f"{cfg.max_position_embeddings}")
         masked = attention_mask is not None
         if masked:
@@ -218,25 +265,33 @@ class LlamaGenerator:
                                           or forced_tokens.shape[1] < max_new_tokens or not forced_tokens.is_cuda):
             raise RuntimeError(f"generate: forced_tokens must be int64 [{B}, >= {max_new_tokens}] on {self.device}")
         out = self.pre.prefill(src=src, video=video, inputs_embeds=inputs_embeds, attention_mask=attention_mask,
-                               position_ids="generate" if masked else None)
-        rows = -(-(S + max_new_tokens) // ROW_GRANULE) * ROW_GRANULE
-        plan = self._plan_for(B, rows, masked)
+                               position_ids="generate" if masked else None, prefix=prefix)
+        live = S if cache_budget is None else min(S, cache_budget)          # cache rows in use
+        most = S + max_new_tokens if cache_budget is None else min(live + max_new_tokens, cache_budget + ROW_GRANULE)
+        rows = -(-most // ROW_GRANULE) * ROW_GRANULE
+        plan = self._plan_for(B, rows, masked, 0 if prefix is None else prefix.rows, cache_budget is not None)
+        for i, d in enumerate(plan.prefix_descs):
+            d.KP, d.VP = prefix.k[i].data_ptr(), prefix.v[i].data_ptr()
         ws = plan.ws
         D, Lyr, V = cfg.hidden_size, cfg.num_hidden_layers, cfg.vocab_size
         stops = [list(map(int, s)) for s in (stop_sequences or []) if len(s)]
         with torch.cuda.device(self.device):
             stream = torch.cuda.current_stream().cuda_stream
-            # the prefill's K (post-rotary) / V of every layer -> cache rows [0, S): one strided copy each
             pws = self.pre.last_ws
-            qkv_all = pws["qkv"].view(Lyr, B, S, 3, D)
-            ws["kc"][:, :, :S].copy_(qkv_all[:, :, :, 1])
-            ws["vc"][:, :, :S].copy_(qkv_all[:, :, :, 2])
-            if masked:
-                ws["kbias"].zero_()
-                ws["kbias"][:, :S].copy_(pws["kbias"])
-                ws["pos0"].copy_(attention_mask.sum(1).to(torch.int32))     # position of new token t = n_valid + t
+            if cache_budget is None:
+                # the prefill's K (post-rotary) / V of every layer -> cache rows [0, S): one strided copy each
+                qkv_all = pws["qkv"].view(Lyr, B, S, 3, D)
+                ws["kc"][:, :, :S].copy_(qkv_all[:, :, :, 1])
+                ws["vc"][:, :, :S].copy_(qkv_all[:, :, :, 2])
             else:
-                ws["pos0"].fill_(S)
+                self._fill_weighted(plan, pws, B, S, rows, masked, live, cache_recent)
+            if masked:
+                if cache_budget is None:
+                    ws["kbias"].zero_()
+                    ws["kbias"][:, :S].copy_(pws["kbias"])
+                ws["pos0"].copy_(p0 + attention_mask.sum(1).to(torch.int32))     # position of new token t = n_valid + t
+            else:
+                ws["pos0"].fill_(p0 + S)
             logits_all = torch.empty((max_new_tokens, B, V), dtype=torch.float32, device=self.device) if return_logits else None
             toks = torch.empty((B, max_new_tokens), dtype=torch.int64, device=self.device)
             L.check(self.lib.hk_argmax_f32(out["logits"].data_ptr(), ws["tok"].data_ptr(), B, V, V, stream), "hk_argmax_f32")
@@ -263,7 +318,13 @@ class LlamaGenerator:
                         break
                 if t + 1 == max_new_tokens:
                     break
-                self._step(plan, t, S, stream)
+                if cache_budget is not None and live == cache_budget + ROW_GRANULE:
+                    H, hd = cfg.num_attention_heads, cfg.head_dim
+                    ops.cache_evict(ws["kc"].view(Lyr * B, rows, H, hd), ws["vc"].view(Lyr * B, rows, H, hd), ws["kw"].view(Lyr * B, H, rows), live,
+                                    cache_budget, cache_recent, key_bias=ws["kbias_h"].view(Lyr * B, H, rows) if masked else None)
+                    live = cache_budget
+                self._step(plan, t, live, stream)
+                live += 1
                 if return_logits:
                     logits_all[t + 1].copy_(ws["logits"])
             tokens = toks[:, :n_out].clone()
@@ -280,6 +341,30 @@ class LlamaGenerator:
         if return_logits:
             res["logits"] = logits_all[:n_out]
         return res
+
+    def _fill_weighted(self, plan: _DecodePlan, pws, B: int, S: int, rows: int, masked: bool, live: int, recent: int):
+        """The prefill's K / V, and the weight its queries gave every key, into cache rows [0, live): all rows, or the budget's."""
+        cfg, ws = self.cfg, plan.ws
+        Lyr, H, hd = cfg.num_hidden_layers, cfg.num_attention_heads, cfg.head_dim
+        n = Lyr * B
+        qkv = pws["qkv"].view(n, S, 3, H, hd)
+        kc, vc, kw = ws["kc"].view(n, rows, H, hd), ws["vc"].view(n, rows, H, hd), ws["kw"].view(n, H, rows)
+        kw.zero_()
+        bias = kb = None
+        if masked:
+            bias = pws["kbias"].repeat(Lyr, 1)                               # [layers * B, S]
+            kb = ws["kbias_h"].view(n, H, rows)
+            kb.zero_()
+        if live == S:
+            ops.attn_key_weights(qkv[:, :, 0], qkv[:, :, 1], key_bias=bias, weight_out=kw)
+            kc[:, :S].copy_(qkv[:, :, 1])
+            vc[:, :S].copy_(qkv[:, :, 2])
+            if masked:
+                kb[:, :, :S].copy_(bias[:, None])
+            return
+        w = ops.attn_key_weights(qkv[:, :, 0], qkv[:, :, 1], key_bias=bias)
+        ops.cache_evict(qkv[:, :, 1], qkv[:, :, 2], w, S, live, recent, key_bias=None if bias is None else bias[:, None].expand(n, H, S),
+                        out=(kc, vc, kw, kb))
 
     @staticmethod
     def _first_stop(host: torch.Tensor, checked: int, stops: List[List[int]], eos: Optional[int], finished: List[bool]):

@@ -61,7 +61,21 @@ class _Plan:
         self.ws: Dict[str, torch.Tensor] = {}
         self.steps: List[Tuple] = []
         self.keep: List = []
+        self.prefix_descs: List = []       # one hk_prefix_attn_desc per layer where the prompt continues a prefix
         self.pool_epoch = 0
+
+
+class PromptPrefix:
+    """K (post-rotary) and V of the tokens that several prompts begin with, made by LlamaPrefill.make_prefix: bf16 [layers, rows, D] in
+    memory of their own.  n_positions: how many tokens stood there (the position of what follows; rows is smaller once the prefix has been
+    cut to a budget, and kept int32 [layers, heads, rows] then says which rows every head has kept)."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, n_positions: int, kept: Optional[torch.Tensor] = None):
+        self.k, self.v, self.n_positions, self.kept = k, v, n_positions, kept
+
+    @property
+    def rows(self) -> int:
+        return self.k.shape[1]
 
 
 class LlamaPrefill:
@@ -89,7 +103,7 @@ class LlamaPrefill:
         # buffer was ever asked for (qkv alone is 2.2 GB at B = 8, S = 352), not the sum over shapes; plans are host-side
         # descriptor sets, kept LRU and rebuilt when a buffer had to grow.
         self.pool = _Pool(self.device)
-        self.plans: "OrderedDict[Tuple[int, int, bool, bool], _Plan]" = OrderedDict()   # (B, S, masked, explicit position ids)
+        self.plans: "OrderedDict[Tuple[int, int, bool, bool, int], _Plan]" = OrderedDict()   # (B, S, masked, explicit position ids, prefix rows)
         self.last_ws: Dict[str, torch.Tensor] = {}
         # projection weights streamed from a 64 x 64-block copy (hk_gemm_desc.w_tiled): HK_LLM_TILED=0 = row-major (A/B aid)
         self.tiled = os.environ.get("HK_LLM_TILED", "1") != "0"
@@ -98,8 +112,8 @@ class LlamaPrefill:
     def pooled_bytes(self) -> int:
         return self.pool.nbytes()
 
-    def plan_for(self, B: int, S: int, masked: bool, with_pos: bool) -> "_Plan":
-        key = (B, S, masked, with_pos)
+    def plan_for(self, B: int, S: int, masked: bool, with_pos: bool, P: int = 0) -> "_Plan":
+        key = (B, S, masked, with_pos, P)
         plan = self.plans.get(key)
         if plan is not None and plan.pool_epoch == self.pool.epoch:
             self.plans.move_to_end(key)
@@ -107,7 +121,7 @@ class LlamaPrefill:
         if plan is not None:
             del self.plans[key]
         epoch = self.pool.epoch
-        plan = self._build_plan(B, S, masked, with_pos)
+        plan = self._build_plan(B, S, masked, with_pos, P)
         if self.pool.epoch != epoch:
             self.plans.clear()              # a buffer grew: every older plan points into the released allocation
         plan.pool_epoch = self.pool.epoch
@@ -213,7 +227,7 @@ class LlamaPrefill:
         plan.keep.append(d)
         plan.steps.append((self.lib.hk_gemm_bf16, (C.byref(d),), "hk_gemm_bf16"))
 
-    def _build_plan(self, B: int, S: int, masked: bool, with_pos: bool = False) -> _Plan:
+    def _build_plan(self, B: int, S: int, masked: bool, with_pos: bool = False, P_rows: int = 0) -> _Plan:
         cfg, dev, w = self.cfg, self.device, self.w
         D, I, H, hd, Lyr, V = (cfg.hidden_size, cfg.intermediate_size, cfg.num_attention_heads, cfg.head_dim,
                                cfg.num_hidden_layers, cfg.vocab_size)
@@ -241,6 +255,7 @@ class LlamaPrefill:
             # fp32 slices summed by the norm that follows (hk_rmsnorm_add_parts)
             sk_o, sk_d = self.split_k_for(M, D, D), self.split_k_for(M, D, I)
             ws["parts"] = buf("parts", (max(sk_o, sk_d), M, D), f32) if max(sk_o, sk_d) > 1 else None
+            pws = buf("prefix_ws", (ops.prefix_attention_ws(B, H, S, P_rows, S, hd),), torch.uint8) if P_rows else None
         P = lambda t: t.data_ptr()  # noqa: E731
         x, xn, att, gu, act = ws["x"], ws["xn"], ws["att"], ws["gu"], ws["act"]
         qscale = (hd ** -0.5) * LOG2E
@@ -267,11 +282,19 @@ class LlamaPrefill:
             self._gemm(plan, P(xn), w[o + "qkv"], P(qkv), M, 3 * D, D)
             plan.steps.append((self.lib.hk_rope_bf16, (P(qkv), P(w["cos"]), P(w["sin"]), P(ws["pos"]) if with_pos else None, M, H, hd, S,
                                                        cfg.max_position_embeddings, qscale), "hk_rope_bf16"))
-            ad = ops.attn_desc(P(qkv), P(qkv) + D * eb, P(qkv) + 2 * D * eb, P(att), B, H, S, S,
-                               3 * D, 3 * D, 3 * D, D, S * 3 * D, S * 3 * D, S * 3 * D, S * D,
-                               key_bias=P(ws["kbias"]) if masked else None, head_dim=hd, causal=True)
-            plan.keep.append(ad)
-            plan.steps.append((self.lib.hk_flash_attn_bf16, (C.byref(ad),), "hk_flash_attn_bf16"))
+            if P_rows:
+                # the prompt continues a shared prefix: its rows once for all sequences, then the own keys; KP / VP are set per call
+                pd = L.HkPrefixAttnDesc(P(qkv), None, None, P(qkv) + D * eb, P(qkv) + 2 * D * eb, P(att), P(ws["kbias"]) if masked else None,
+                                        P(pws), pws.numel(), B, H, S, P_rows, S, hd, 3 * D, S * 3 * D, D, D, 3 * D, S * 3 * D, 3 * D, S * 3 * D,
+                                        D, S * D, S if masked else 0)
+                plan.prefix_descs.append(pd)
+                plan.steps.append((self.lib.hk_prefix_attn_bf16, (C.byref(pd),), "hk_prefix_attn_bf16"))
+            else:
+                ad = ops.attn_desc(P(qkv), P(qkv) + D * eb, P(qkv) + 2 * D * eb, P(att), B, H, S, S,
+                                   3 * D, 3 * D, 3 * D, D, S * 3 * D, S * 3 * D, S * 3 * D, S * D,
+                                   key_bias=P(ws["kbias"]) if masked else None, head_dim=hd, causal=True)
+                plan.keep.append(ad)
+                plan.steps.append((self.lib.hk_flash_attn_bf16, (C.byref(ad),), "hk_flash_attn_bf16"))
             residual_gemm(P(att), w[o + "o"], D, sk_o)
             norm(w[o + "n2"], sk_o)
             if self.fused_swiglu:
@@ -297,7 +320,7 @@ class LlamaPrefill:
     @torch.no_grad()
     def prefill(self, src: Optional[torch.Tensor] = None, video: Optional[torch.Tensor] = None,
                 inputs_embeds: Optional[torch.Tensor] = None, attention_mask: Optional[torch.Tensor] = None,
-                position_ids=None):
+                position_ids=None, prefix: Optional[PromptPrefix] = None):
         """Either `src` int64 [B,S] (token id >= 0, or -(video row)-1 for a spliced video token) with `video`
         [B*n, D] bf16/fp32 (encode_img's output), or ready `inputs_embeds` [B,S,D].  attention_mask [B,S] (1 =
         token, 0 = padding on either side) or None; logits are read at the LAST 1 of every row.
@@ -306,6 +329,8 @@ class LlamaPrefill:
         `generate` builds for a (left-)padded batch, cumsum(mask) - 1 with padded positions at 1
         (prepare_inputs_for_generation :751-754); or an explicit integer tensor [B,S].  A left-padded mask with the
         default ids is refused: the reference never runs that combination and its positions would be shifted.
+        prefix: what every sequence of the batch continues (make_prefix): the tokens attend to its rows, all visible, and among themselves,
+        at positions that follow it (default ids: prefix.n_positions + 0..S-1; "generate": the same offset).
         Returns {"hidden": bf16 [B,S,D] after the final RMSNorm,
         "logits": fp32 [B,V] at each row's last valid position, "kv": [(k, v)] per layer as [B,S,H,hd] bf16 views
         (k post-rotary)}.  Every returned tensor is a view of the pooled workspace, valid until the NEXT prefill call of this
@@ -317,8 +342,12 @@ class LlamaPrefill:
             raise RuntimeError("prefill: pass exactly one of src / inputs_embeds")
         ref = src if src is not None else inputs_embeds
         B, S = int(ref.shape[0]), int(ref.shape[1])
-        if S > cfg.max_position_embeddings:
-            raise RuntimeError(f"sequence length {S} exceeds max_position_embeddings {cfg.max_position_embeddings}")
+        p0 = 0
+        if prefix is not None:
+            self._check_prefix(prefix)
+            p0 = prefix.n_positions
+        if p0 + S > cfg.max_position_embeddings:
+            raise RuntimeError(f"sequence length {p0 + S} exceeds max_position_embeddings {cfg.max_position_embeddings}")
         if ref.device != self.device:
             raise RuntimeError(f"inputs are on {ref.device}, model on {self.device}")
         masked = attention_mask is not None
@@ -328,7 +357,14 @@ class LlamaPrefill:
                 raise RuntimeError('position_ids must be None, "generate" (needs attention_mask) or an int tensor [B,S]')
         elif with_pos and (tuple(position_ids.shape) != (B, S) or position_ids.device != self.device):
             raise RuntimeError(f"position_ids must be an integer tensor [{B},{S}] on {self.device}")
-        plan = self.plan_for(B, S, masked, with_pos)
+        if prefix is not None and not with_pos:
+            if masked and bool((attention_mask[:, 0] == 0).any()):
+                raise RuntimeError('prefill: the mask is left-padded; pass position_ids="generate" or explicit position_ids')
+            position_ids = torch.arange(p0, p0 + S, device=self.device).expand(B, S)
+            with_pos = True
+        plan = self.plan_for(B, S, masked, with_pos, 0 if prefix is None else prefix.rows)
+        for i, d in enumerate(plan.prefix_descs):
+            d.KP, d.VP = prefix.k[i].data_ptr(), prefix.v[i].data_ptr()
         ws = plan.ws
         D, H, hd = cfg.hidden_size, cfg.num_attention_heads, cfg.head_dim
         with torch.cuda.device(self.device):
@@ -349,7 +385,7 @@ class LlamaPrefill:
                 ws["last"].copy_(last)
                 if with_pos:
                     if isinstance(position_ids, str):
-                        pos = (m.cumsum(1) - 1).masked_fill_(m == 0, 1)
+                        pos = (p0 + m.cumsum(1) - 1).masked_fill_(m == 0, 1)
                     else:
                         pos = position_ids
                     if int(pos.min()) < 0 or int(pos.max()) >= cfg.max_position_embeddings:
@@ -386,6 +422,45 @@ class LlamaPrefill:
         kv = [(ws["qkv"][i].view(B, S, 3, H, hd)[:, :, 1], ws["qkv"][i].view(B, S, 3, H, hd)[:, :, 2])
               for i in range(cfg.num_hidden_layers)]
         return {"hidden": ws["xn"].view(B, S, D), "logits": ws["logits"], "kv": kv}
+
+    def _check_prefix(self, prefix: PromptPrefix):
+        cfg = self.cfg
+        want = (cfg.num_hidden_layers, prefix.rows, cfg.hidden_size)
+        for t in (prefix.k, prefix.v):
+            if t.dtype != torch.bfloat16 or t.device != self.device or tuple(t.shape) != want or not t.is_contiguous():
+                raise RuntimeError(f"prefix: K and V must be contiguous bf16 {list(want)} on {self.device}")
+        if not 1 <= prefix.rows <= prefix.n_positions:
+            raise RuntimeError(f"prefix: {prefix.rows} rows of {prefix.n_positions} positions")
+
+    @torch.no_grad()
+    def make_prefix(self, src: Optional[torch.Tensor] = None, video: Optional[torch.Tensor] = None,
+                    inputs_embeds: Optional[torch.Tensor] = None, budget: Optional[int] = None, recent: Optional[int] = None,
+                    window: Optional[int] = None) -> PromptPrefix:
+        """Prefill, once, what several prompts begin with (system text, video tokens, instruction: the same for every question about a clip
+        where the instruction is, tasks/test.py:79-97): src [1, S] or inputs_embeds [1, S, D].  Pass the result as prefill(prefix=) /
+        LlamaGenerator.generate(prefix=).
+        budget: keep at most this many rows per layer and head: the last `recent` (default: half of them) and those with the most
+        attention weight from the prompt's own queries (its last `window` ones; default: all).  Positions stay the original ones."""
+        ref = src if src is not None else inputs_embeds
+        if ref is None or ref.shape[0] != 1:
+            raise RuntimeError("make_prefix: pass src [1, S] or inputs_embeds [1, S, D]")
+        cfg = self.cfg
+        Lyr, H, hd, D, S = cfg.num_hidden_layers, cfg.num_attention_heads, cfg.head_dim, cfg.hidden_size, int(ref.shape[1])
+        if budget is not None and not (1 <= budget and 0 <= (budget // 2 if recent is None else recent) <= budget):
+            raise RuntimeError(f"make_prefix: budget={budget}, recent={recent} (1 <= budget, 0 <= recent <= budget)")
+        if window is not None and window < 1:
+            raise RuntimeError(f"make_prefix: window={window} must be at least 1")
+        self.prefill(src=src, video=video, inputs_embeds=inputs_embeds)
+        qkv = self.last_ws["qkv"].view(Lyr, S, 3, H, hd)
+        with torch.cuda.device(self.device):
+            if budget is None or budget >= S:
+                return PromptPrefix(qkv[:, :, 1].reshape(Lyr, S, D).clone(), qkv[:, :, 2].reshape(Lyr, S, D).clone(), S)
+            w = ops.attn_key_weights(qkv[:, S - min(window or S, S):, 0], qkv[:, :, 1])
+            k = torch.empty((Lyr, budget, H, hd), dtype=torch.bfloat16, device=self.device)
+            v = torch.empty_like(k)
+            kept = ops.cache_evict(qkv[:, :, 1], qkv[:, :, 2], w, S, budget, budget // 2 if recent is None else recent,
+                                   out=(k, v, torch.empty((Lyr, H, budget), dtype=torch.float32, device=self.device), None))
+            return PromptPrefix(k.view(Lyr, budget, D), v.view(Lyr, budget, D), S, kept)
 
 
 def prefill_flops(cfg: LlmConfig, B: int, S: int) -> float:

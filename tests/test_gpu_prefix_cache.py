@@ -264,3 +264,238 @@ def test_cache_evict_keeps_the_heaviest_rows(B, n, budget, recent, H, hd, masked
     else:
         assert all(bool((t[:, budget:] == 7.0).all()) for t in out[:2]) and bool((wo[..., budget:] == 7.0).all())
         assert torch.equal(k, k0) and torch.equal(v, v0) and torch.equal(w.view(torch.int32), w0.view(torch.int32))
+
+
+# ---------------------------------------------------------------- the paths that use them: prompts that continue a prefix, bounded caches
+def _llm(seed, **kw):
+    from dataclasses import replace
+    from hawkeye_amd import weights as W
+    from hawkeye_amd.config import SMALL_LLM
+    from hawkeye_amd.decode import LlamaGenerator
+    from hawkeye_amd.llm import LlamaPrefill
+    cfg = replace(SMALL_LLM, **kw)
+    pre = LlamaPrefill(cfg, DEV).load_state_dict(W.make_llm_state_dict(cfg, seed))
+    return cfg, pre, LlamaGenerator(pre)
+
+
+def _prompt(cfg, P, lengths, seed):
+    """One prefix [1, P] with 8 video rows, and questions of the given lengths left-padded to the longest: (prefix, questions, mask, video)"""
+    from hawkeye_amd import weights as W
+    g = torch.Generator(device="cpu").manual_seed(seed)
+    prefix = torch.randint(3, cfg.vocab_size, (1, P), generator=g)
+    prefix[0, 5:13] = -torch.arange(1, 9)
+    S = max(lengths)
+    ask = torch.randint(3, cfg.vocab_size, (len(lengths), S), generator=g)
+    mask = (torch.arange(S)[None] >= S - torch.tensor(lengths)[:, None]).long()
+    ask[mask == 0] = 2
+    return prefix.to(DEV), ask.to(DEV), mask.to(DEV), W._normal("video_tokens", seed, (8, cfg.hidden_size), 0.05).to(DEV)
+
+
+def _rel(a, ref):
+    return ((a.double() - ref.double()).abs().max() / ref.double().abs().max()).item()
+
+
+@pytest.mark.parametrize("P,lengths", [(60, [17, 17, 17]), (100, [40]), (33, [5, 20, 1, 12]), (90, [70] * 3), (64, [3] * 16)])
+def test_prompts_that_continue_a_prefix_equal_whole_prompts(P, lengths):
+    """make_prefix + prefill / generate(prefix=): logits, hidden states and tokens of the same prompts written out in full."""
+    cfg, pre, gen = _llm(21)
+    prefix, ask, mask, video = _prompt(cfg, P, lengths, 21)
+    B, S, T = len(lengths), max(lengths), 6
+    ragged = min(lengths) < S
+    whole = torch.cat([prefix.expand(B, P), ask], 1)
+    wmask = None
+    if ragged:                                                # whole prompts left-pad in front of the prefix
+        for b, n in enumerate(lengths):
+            whole[b] = torch.cat([torch.full((S - n,), 2, device=DEV), prefix[0], ask[b, S - n:]])
+        wmask = torch.cat([torch.ones_like(whole[:, :P]), torch.ones_like(mask)], 1)
+        for b, n in enumerate(lengths):
+            wmask[b, :S - n] = 0
+    ref = gen.generate(src=whole, video=video, attention_mask=wmask, max_new_tokens=T, return_logits=True)
+    full = pre.prefill(src=whole, video=video, attention_mask=wmask, position_ids="generate" if ragged else None)
+    hidden = full["hidden"][:, P:].clone()
+    pf = pre.make_prefix(src=prefix, video=video)
+    assert pf.rows == pf.n_positions == P and pf.kept is None
+    out = pre.prefill(src=ask, attention_mask=mask if ragged else None, position_ids="generate" if ragged else None, prefix=pf)
+    # two kernels for one operator: bf16 products and residual stream differ by their roundings (the tolerance of the cache tests)
+    valid = mask.bool()
+    assert _rel(out["hidden"][valid], hidden[valid]) < 2e-2 and _rel(out["logits"], ref["logits"][0]) < 2e-2
+    got = gen.generate(src=ask, attention_mask=mask if ragged else None, prefix=pf, max_new_tokens=T, forced_tokens=ref["tokens"], return_logits=True)
+    for t in range(T):
+        assert _rel(got["logits"][t], ref["logits"][t]) < 2e-2, t
+    again = gen.generate(src=ask, attention_mask=mask if ragged else None, prefix=pf, max_new_tokens=T, forced_tokens=ref["tokens"], return_logits=True)
+    assert torch.equal(again["logits"], got["logits"])
+    free = gen.generate(src=ask, attention_mask=mask if ragged else None, prefix=pf, max_new_tokens=T)["tokens"]
+    top2 = ref["logits"].topk(2, -1).values
+    sure = ((top2[..., 0] - top2[..., 1]) / ref["logits"].abs().amax(-1) > 5e-2).t()      # [B, T]
+    for b in range(B):
+        for t in range(T):
+            if not bool(sure[b, t]):
+                break                                         # what follows depends on a near-tie
+            assert free[b, t] == ref["tokens"][b, t], (b, t)
+
+
+def test_a_prefix_cut_to_its_own_length_less_nothing_is_the_prefix():
+    cfg, pre, gen = _llm(22)
+    prefix, ask, mask, video = _prompt(cfg, 70, [12, 12], 22)
+    a, b = pre.make_prefix(src=prefix, video=video), pre.make_prefix(src=prefix, video=video, budget=70)
+    assert torch.equal(a.k, b.k) and torch.equal(a.v, b.v)
+    cut = pre.make_prefix(src=prefix, video=video, budget=40, recent=10)
+    assert cut.rows == 40 and cut.n_positions == 70 and tuple(cut.kept.shape) == (cfg.num_hidden_layers, cfg.num_attention_heads, 40)
+    hd = cfg.head_dim
+    for layer in range(cfg.num_hidden_layers):
+        for h in range(cfg.num_attention_heads):
+            rows = cut.kept[layer, h].long()
+            assert torch.equal(cut.k[layer, :, h * hd:(h + 1) * hd], a.k[layer, rows, h * hd:(h + 1) * hd])
+            assert torch.equal(cut.v[layer, :, h * hd:(h + 1) * hd], a.v[layer, rows, h * hd:(h + 1) * hd])
+            assert rows[-10:].tolist() == list(range(60, 70)) and bool((rows[1:] > rows[:-1]).all())
+    # the kept rows are those the prompt's own queries weigh most
+    pre.prefill(src=prefix, video=video)
+    qkv = pre.last_ws["qkv"].view(cfg.num_hidden_layers, 70, 3, cfg.num_attention_heads, hd)
+    p, _ = _ref_weights(qkv[:, :, 0], qkv[:, :, 1], None, True)
+    w = p.sum(2)
+    inside = torch.zeros_like(w, dtype=torch.bool).scatter_(2, cut.kept.long(), True)
+    for layer in range(cfg.num_hidden_layers):
+        for h in range(cfg.num_attention_heads):
+            old = torch.arange(70, device=DEV) < 60
+            assert float(w[layer, h][inside[layer, h] & old].min()) >= float(w[layer, h][~inside[layer, h] & old].max()) * (1 - 1e-4)
+    out = gen.generate(src=ask, prefix=cut, max_new_tokens=3, return_logits=True)
+    assert bool(torch.isfinite(out["logits"]).all()) and out["tokens"].shape == (2, 3)
+    with pytest.raises(RuntimeError, match="budget=0"):
+        pre.make_prefix(src=prefix, video=video, budget=0)
+    with pytest.raises(RuntimeError, match="window=0"):
+        pre.make_prefix(src=prefix, video=video, budget=5, window=0)
+    with pytest.raises(RuntimeError, match="together"):
+        gen.generate(src=ask, prefix=cut, cache_budget=20, max_new_tokens=2)
+    with pytest.raises(RuntimeError, match="exceeds max_position_embeddings"):
+        gen.generate(src=ask, prefix=cut, max_new_tokens=200)
+    with pytest.raises(RuntimeError, match="left-padded"):
+        m = mask.clone()
+        m[0, 0] = 0
+        pre.prefill(src=ask, attention_mask=m, prefix=cut)
+
+
+@pytest.mark.parametrize("masked", [False, True])
+def test_a_budget_that_never_binds_changes_nothing(masked):
+    cfg, pre, gen = _llm(23)
+    prefix, ask, mask, video = _prompt(cfg, 40, [50, 50] if not masked else [50, 31, 8], 23)
+    kw = dict(src=ask, attention_mask=mask if masked else None, max_new_tokens=8, return_logits=True)
+    ref = gen.generate(**kw)
+    got = gen.generate(cache_budget=100, forced_tokens=ref["tokens"], **kw)
+    for t in range(8):
+        assert _rel(got["logits"][t], ref["logits"][t]) < 2e-2, t
+
+
+@pytest.mark.parametrize("lengths", [[90], [60, 60, 60], [70, 22, 41]])
+def test_a_bounded_cache_follows_its_definition_step_by_step(lengths):
+    """generate(cache_budget=): the caches after every cut, against a 64-bit bookkeeping of weights over the same keys."""
+    budget, recent, T = 24, 8, 150
+    cfg, pre, gen = _llm(24)
+    _, ask, mask, video = _prompt(cfg, 20, lengths, 24)
+    masked = min(lengths) < max(lengths)
+    B, S, Lyr, H, hd = len(lengths), max(lengths), cfg.num_hidden_layers, cfg.num_attention_heads, cfg.head_dim
+    kw = dict(src=ask, attention_mask=mask if masked else None, cache_budget=budget, cache_recent=recent)
+    cuts = []
+    whole = ops.cache_evict
+
+    def spy(k, v, w, n, b, r=0, key_bias=None, out=None):
+        before = (k[:, :n].clone(), v[:, :n].clone(), w[..., :n].clone(), None if key_bias is None else key_bias[..., :n].clone())
+        kept = whole(k, v, w, n, b, r, key_bias=key_bias, out=out)
+        ko, vo = (k, v) if out is None else out[:2]
+        cuts.append((before, n, kept.clone(), ko[:, :b].clone(), vo[:, :b].clone()))
+        return kept
+
+    ops.cache_evict = spy
+    try:
+        out = gen.generate(max_new_tokens=T, return_logits=True, **kw)
+    finally:
+        ops.cache_evict = whole
+    assert out["tokens"].shape == (B, T) and bool(torch.isfinite(out["logits"]).all())
+    assert len(cuts) == 1 + (T - 2) // 64                      # the prompt's, then every 64 steps
+    for (k0, v0, w0, b0), n, kept, ko, vo in cuts:
+        want = _ref_evict(w0, b0, n, budget, recent).to(DEV)
+        assert torch.equal(kept, want)
+        src = want.long().transpose(1, 2)[..., None].expand(-1, -1, -1, hd)
+        assert torch.equal(ko, k0.gather(1, src)) and torch.equal(vo, v0.gather(1, src))
+    # the weights themselves: before the first cut in place they are the kept prompt weights plus 64 steps', whose sum over the live
+    # keys is one per step (and the prompt's queries gave one each in all)
+    first, second = cuts[0], cuts[1]
+    kept_w = first[0][2].double().gather(2, first[2].long())
+    grown = second[0][2].double().sum(-1) - kept_w.sum(-1)
+    assert float((grown - 64).abs().max()) < 64 * (budget + 64 + 128) * 2.0 ** -24 + float(kept_w.sum(-1).max()) * 2.0 ** -18
+    valid = torch.tensor(lengths, dtype=torch.float64, device=DEV).repeat(Lyr)[:, None]
+    tot = first[0][2].double()
+    if masked:                                                 # a padded query sees removed keys only and adds nothing
+        assert float((tot.masked_select(first[0][3] <= -1.0e4)).abs().max()) == 0.0
+    assert float((tot.sum(-1) - valid).abs().max()) < S * 2.0 ** -12
+    # what was not cut yet equals the unbounded run: token 0 comes from the same prefill
+    ref = gen.generate(src=ask, attention_mask=mask if masked else None, max_new_tokens=1, return_logits=True)
+    assert torch.equal(ref["logits"][0], out["logits"][0])
+    with pytest.raises(RuntimeError, match="cache_budget=0"):
+        gen.generate(src=ask, cache_budget=0, max_new_tokens=2)
+    with pytest.raises(RuntimeError, match="needs cache_budget"):
+        gen.generate(src=ask, cache_recent=3, max_new_tokens=2)
+
+
+def test_streams_graphs_and_strides():
+    """Another stream, a captured call replayed with eager work between, and caches whose offsets pass 2^31 elements."""
+    B, H, hd, P, n = 3, 2, 128, 300, 90
+    q, kp, vp = _rand((B, 1, H, hd), 1, 0.2), _rand((P, H, hd), 2), _rand((P, H, hd), 3)
+    k, v = _rand((B, n, H, hd), 4), _rand((B, n, H, hd), 5)
+    w = _rand((B, H, n), 6, 1.0, torch.float32).abs()
+
+    def run(wo, kc, vc, ww):
+        a = ops.prefix_attention(q, kp, vp, k, v)
+        wk = ops.attn_key_weights(q, k)
+        o = ops.decode_attn_weights(q.view(B, H * hd), k.view(B, n, H * hd), v.view(B, n, H * hd), n, H, hd, w, weight_out=wo)
+        kept = ops.cache_evict(k, v, wo, n, 40, 9, out=(kc, vc, ww, None))
+        return a, wk, o, kept
+
+    def bufs():
+        return torch.empty_like(w), torch.empty((B, 40, H, hd), dtype=torch.bfloat16, device=DEV), torch.empty((B, 40, H, hd), dtype=torch.bfloat16, device=DEV), \
+            torch.empty((B, H, 40), device=DEV)
+    base_b = bufs()
+    base = [t.clone() for t in run(*base_b)] + [t.clone() for t in base_b]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    other_b = bufs()
+    with torch.cuda.stream(side):
+        other = run(*other_b)
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(base, list(other) + list(other_b)))
+    graph_b = bufs()
+    with torch.cuda.stream(side):
+        run(*graph_b)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        res = run(*graph_b)
+    q0 = q.clone()
+    for rep in range(4):
+        q.copy_(q0 * (1 + rep))
+        want = [t.clone() for t in run(*base_b)] + [t.clone() for t in base_b]
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, list(res) + list(graph_b))), rep
+    # a cache of 2^31 elements and more per tensor: the rows used lie behind the 32-bit offsets
+    H, hd, rows = 32, 128, 300000
+    big = torch.zeros((2, rows, H * hd), dtype=torch.bfloat16, device=DEV)              # 2.46e9 elements, sequence 1 behind 1.2e9
+    bigv = torch.zeros_like(big)
+    n = 70
+    kk, vv = _rand((2, n, H * hd), 7), _rand((2, n, H * hd), 8)
+    big[:, rows - n:], bigv[:, rows - n:] = kk, vv
+    qq = _rand((2, 1, H, hd), 9, 0.2)
+    got = ops.prefix_attention(qq, kp[:0].new_empty((0, H, hd)), vp[:0].new_empty((0, H, hd)), big[:, rows - n:].unflatten(2, (H, hd)), bigv[:, rows - n:].unflatten(2, (H, hd)))
+    assert torch.equal(got, ops.prefix_attention(qq, kp[:0].new_empty((0, H, hd)), vp[:0].new_empty((0, H, hd)), kk.unflatten(2, (H, hd)), vv.unflatten(2, (H, hd))))
+    flat = big.view(-1, H, hd)                                                          # one prefix of 600000 rows, its end used
+    got = ops.prefix_attention(qq, flat[-n:], bigv.view(-1, H, hd)[-n:], kk.unflatten(2, (H, hd)), vv.unflatten(2, (H, hd)))
+    assert torch.equal(got, ops.prefix_attention(qq, kk[1].unflatten(1, (H, hd)), vv[1].unflatten(1, (H, hd)), kk.unflatten(2, (H, hd)), vv.unflatten(2, (H, hd))))
+    wbig = torch.zeros((2, H, rows), device=DEV)
+    o = ops.decode_attn_weights(qq.view(2, -1), big, bigv, rows, H, hd, wbig, key_bias=torch.cat([torch.full((2, rows - n), -1.0e4, device=DEV), torch.zeros((2, n), device=DEV)], 1))
+    ref, tol = _ref_prefix(qq, kp[:0].new_empty((0, H, hd)), vp[:0].new_empty((0, H, hd)), kk.unflatten(2, (H, hd)), vv.unflatten(2, (H, hd)), None)
+    _near(o.view(2, 1, H, hd), ref, tol)
+    assert float((wbig.sum(-1) - 1).abs().max()) < 1e-4 and bool((wbig[..., :rows - n] == 0).all())
+    kept = ops.cache_evict(big.unflatten(2, (H, hd)), bigv.unflatten(2, (H, hd)), wbig, rows, 50, 20)
+    assert bool((kept[..., -20:] == torch.arange(rows - 20, rows, device=DEV)).all()) and bool((kept >= rows - n).all())
+    src = (kept.long() - (rows - n)).transpose(1, 2)[..., None].expand(-1, -1, -1, hd)
+    assert torch.equal(big[:, :50].unflatten(2, (H, hd)), kk.unflatten(2, (H, hd)).gather(1, src))
