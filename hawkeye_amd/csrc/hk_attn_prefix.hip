@@ -26,6 +26,9 @@ constexpr float M_NONE = -1.0e30f;   // running maximum of a row that has met no
 constexpr int TK = 32;               // keys per tile
 constexpr int NWV = 4;               // waves per workgroup
 constexpr int MAX_CHUNK = 1024;      // keys per chunk at most: the chunk's bias lives in LDS
+#ifndef HK_ROWS_WANT
+#define HK_ROWS_WANT 320
+#endif
 #ifndef HK_PREFIX_WANT
 #define HK_PREFIX_WANT 1024          // workgroups per launch the chunks are cut for
 #endif
@@ -51,8 +54,23 @@ __device__ __forceinline__ void wave_lds_sync() {   // LDS written by this wave'
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-template <int HD, int RT, bool BIAS, bool RAW>
-__global__ __launch_bounds__(NWV * 64, 2) void hk_prefix_part_kernel(const PrefixParams p) {
+__device__ __forceinline__ float inverse_sum(float l) { return l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l); }     // no key: 0; NaN stays
+
+// A decode step's weights: w_out[j] = w_in[j] + 2^(s_j - M) / l from its scores.
+struct StepWeights {
+    const float* w_in;               // may be w_out; NULL = zeros
+    float* w_out;
+    int64_t wi_bs, wi_hs, wo_bs, wo_hs;
+};
+__device__ __forceinline__ void add_weights(const PrefixParams& p, const StepWeights& sw, int b, int head, const float* raw, float M, float inv,
+                                            int j0, int step) {
+    const float* wi = sw.w_in ? sw.w_in + (int64_t)b * sw.wi_bs + (int64_t)head * sw.wi_hs : nullptr;
+    float* wo = sw.w_out + (int64_t)b * sw.wo_bs + (int64_t)head * sw.wo_hs;
+    for (int j = j0; j < p.Nk; j += step) wo[j] = (wi ? wi[j] : 0.f) + __builtin_amdgcn_exp2f(raw[j] - M) * inv;
+}
+
+template <int HD, int RT, bool BIAS, bool RAW, int NW, bool ONE>
+__global__ __launch_bounds__(NW * 64, 2) void hk_prefix_part_kernel(const PrefixParams p, const StepWeights sw) {
     constexpr int CH = HD / 8;            // 16-byte chunks per key row
     constexpr int KS = HD / 32;           // contraction steps of S^T
     constexpr int DT = HD / 16;           // 16-dim blocks of O^T
@@ -61,9 +79,10 @@ __global__ __launch_bounds__(NWV * 64, 2) void hk_prefix_part_kernel(const Prefi
     constexpr int VB = TK * HD * 2;       // bytes of a wave's V tile
     constexpr int OB = RT * 16 * HD * 4;  // bytes of a wave's O block at the end
     constexpr int WB = VB > OB ? VB : OB;
-    __shared__ __attribute__((aligned(16))) char vlds[NWV * WB];
-    __shared__ float ml[NWV][RT * 16][2];
+    __shared__ __attribute__((aligned(16))) char vlds[NW * WB];
+    __shared__ float ml[NW][RT * 16][2];
     __shared__ __attribute__((aligned(16))) float blds[BIAS ? MAX_CHUNK : 4];
+    __shared__ __attribute__((aligned(16))) float rawl[ONE && RAW ? MAX_CHUNK : 4];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int l15 = lane & 15, quad = lane >> 4;
@@ -73,7 +92,8 @@ __global__ __launch_bounds__(NWV * 64, 2) void hk_prefix_part_kernel(const Prefi
     const __bf16 *kb, *vb;
     int64_t ldk, ldv;
     bool shared_keys;
-    if (blockIdx.x < p.pjobs) {      // row groups of one (head, chunk) follow each other: the later ones find K and V in L2
+    const int pA = ONE ? p.P : 0, nA = (pA + TK - 1) / TK;      // ONE: tiles [0, nA) are the prefix's, the own keys' follow
+    if (!ONE && blockIdx.x < p.pjobs) {      // row groups of one (head, chunk) follow each other: the later ones find K and V in L2
         const int rg = blockIdx.x % p.nprg, hc = blockIdx.x / p.nprg;
         head = hc % p.H;
         slot = hc / p.H;
@@ -87,16 +107,16 @@ __global__ __launch_bounds__(NWV * 64, 2) void hk_prefix_part_kernel(const Prefi
         ldv = p.ldvp;
         shared_keys = true;
     } else {
-        int j = (int)(blockIdx.x - p.pjobs);
+        int j = (int)(blockIdx.x - (ONE ? 0 : p.pjobs));
         const int rg = j % p.norg;
         j /= p.norg;
         head = j % p.H;
         j /= p.H;
-        brow = j / p.noc;
-        const int c = j - brow * p.noc;
+        brow = ONE ? j : j / p.noc;
+        const int c = ONE ? 0 : j - brow * p.noc;
         slot = p.npc + c;
-        k0 = c * p.oc;
-        k1 = min(k0 + p.oc, p.Nk);
+        k0 = ONE ? 0 : c * p.oc;
+        k1 = ONE ? p.Nk : min(k0 + p.oc, p.Nk);
         const int i0 = rg * RT * 16;
         row0 = brow * p.Nq + i0;
         nrows = min(RT * 16, p.Nq - i0);
@@ -111,7 +131,7 @@ __global__ __launch_bounds__(NWV * 64, 2) void hk_prefix_part_kernel(const Prefi
     const bool has_bias = BIAS && !shared_keys;
     if (has_bias) {
         const float* bp = p.bias + (int64_t)brow * p.bias_bs + (int64_t)head * p.bias_hs;
-        for (int i = tid; i < MAX_CHUNK && k0 + i < k1; i += NWV * 64) blds[i] = bp[k0 + i];
+        for (int i = tid; i < MAX_CHUNK && k0 + i < k1; i += NW * 64) blds[i] = bp[k0 + i];
         __syncthreads();
     }
 
@@ -139,17 +159,25 @@ __global__ __launch_bounds__(NWV * 64, 2) void hk_prefix_part_kernel(const Prefi
     u32x4 vr[NL];
     const int vrow = lane / CH, vch = lane % CH;
     auto load_k = [&](int t) {
+        const bool pre = ONE && t < nA;
+        const __bf16* base = pre ? p.KP + head * HD : kb;
+        const int64_t ld = pre ? p.ldkp : ldk;
+        const int first = pre ? t * TK : k0 + (t - nA) * TK, last = (pre ? pA : k1) - 1;
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-            const __bf16* kp = kb + (int64_t)min(k0 + t * TK + 16 * g + l15, k1 - 1) * ldk + 8 * quad;
+            const __bf16* kp = base + (int64_t)min(first + 16 * g + l15, last) * ld + 8 * quad;
 #pragma unroll
             for (int s = 0; s < KS; ++s) kr[g][s] = *reinterpret_cast<const bf16x8*>(kp + 32 * s);
         }
     };
     auto load_v = [&](int t) {
+        const bool pre = ONE && t < nA;
+        const __bf16* base = pre ? p.VP + head * HD : vb;
+        const int64_t ld = pre ? p.ldvp : ldv;
+        const int first = pre ? t * TK : k0 + (t - nA) * TK, last = (pre ? pA : k1) - 1;
 #pragma unroll
         for (int i = 0; i < NL; ++i)
-            vr[i] = *reinterpret_cast<const u32x4*>(vb + (int64_t)min(k0 + t * TK + i * RPL + vrow, k1 - 1) * ldv + vch * 8);
+            vr[i] = *reinterpret_cast<const u32x4*>(base + (int64_t)min(first + i * RPL + vrow, last) * ld + vch * 8);
     };
     // 16-byte chunk c of key row r lives at chunk c ^ swz(r): the 16 key rows x 32 bytes of one transposing read then touch every
     // bank twice, the least there is (512 bytes at 128 a cycle)
@@ -160,12 +188,12 @@ __global__ __launch_bounds__(NWV * 64, 2) void hk_prefix_part_kernel(const Prefi
 #pragma unroll
     for (int d = 0; d < DT; ++d) toff[d] = trow * HD * 2 + (((2 * d + ((lane & 3) >> 1)) ^ swz(trow)) << 4) + 8 * (lane & 1);
 
-    const int nt = k1 > k0 ? (k1 - k0 + TK - 1) / TK : 0;
+    const int nt = nA + (k1 > k0 ? (k1 - k0 + TK - 1) / TK : 0);
     if (wave < nt) {
         load_k(wave);
         load_v(wave);
     }
-    for (int t = wave; t < nt; t += NWV) {
+    for (int t = wave; t < nt; t += NW) {
         f32x4 st[RT][2];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
@@ -175,30 +203,32 @@ __global__ __launch_bounds__(NWV * 64, 2) void hk_prefix_part_kernel(const Prefi
 #pragma unroll
                 for (int s = 0; s < KS; ++s) st[rt][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kr[g][s], qf[rt][s], st[rt][g], 0, 0, 0);
             }
-        const bool more = t + NWV < nt;
-        if (more) load_k(t + NWV);
+        const bool more = t + NW < nt;
+        if (more) load_k(t + NW);
         // ---- bias, removed and invisible keys ----
-        const int kt = k0 + t * TK;
+        const bool pre = ONE && t < nA;
+        const int kt = pre ? t * TK : k0 + (t - nA) * TK, ke = pre ? pA : k1;
         uint32_t gone = 0;                                // keys of this tile that no row has: their V rows are made zero
-        if (has_bias) {
-            const bool rem = lane < TK && (kt + lane >= k1 || blds[t * TK + lane] <= REMOVED);
+        if (has_bias && !pre) {
+            const float* bl = blds + (t - nA) * TK;
+            const bool rem = lane < TK && (kt + lane >= ke || bl[lane] <= REMOVED);
             gone = (uint32_t)__builtin_amdgcn_ballot_w64(rem);
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
-                const f32x4 bv = *reinterpret_cast<const f32x4*>(blds + t * TK + 16 * g + 4 * quad);
+                const f32x4 bv = *reinterpret_cast<const f32x4*>(bl + 16 * g + 4 * quad);
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         st[rt][g][i] = (gone >> (16 * g + 4 * quad + i)) & 1 ? -INFINITY : st[rt][g][i] + bv[i] * HK_LOG2E;
             }
-        } else if (kt + TK > k1) {
-            gone = 0xffffffffu << (k1 - kt);              // k1 - kt is 1 .. 31 here
+        } else if (kt + TK > ke) {
+            gone = 0xffffffffu << (ke - kt);              // ke - kt is 1 .. 31 here
         }
-        if (kt + TK > k1 || kt + TK - 1 > lim0) {
+        if (kt + TK > ke || (!pre && kt + TK - 1 > lim0)) {
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                const int lim = min(k1 - 1, lim0 + rt * 16 + l15);
+                const int lim = pre ? ke - 1 : min(ke - 1, lim0 + rt * 16 + l15);
 #pragma unroll
                 for (int g = 0; g < 2; ++g)
 #pragma unroll
@@ -207,7 +237,7 @@ __global__ __launch_bounds__(NWV * 64, 2) void hk_prefix_part_kernel(const Prefi
             }
         }
         if (RAW && l15 == 0) {                            // one row: its scores, for the weights
-            float* rp = p.raw + ((int64_t)brow * p.H + head) * p.raw_ld + kt;
+            float* rp = ONE ? rawl + kt : p.raw + ((int64_t)brow * p.H + head) * p.raw_ld + kt;
             *reinterpret_cast<f32x4*>(rp + 4 * quad) = st[0][0];
             *reinterpret_cast<f32x4*>(rp + 16 + 4 * quad) = st[0][1];
         }
@@ -256,7 +286,7 @@ __global__ __launch_bounds__(NWV * 64, 2) void hk_prefix_part_kernel(const Prefi
             *reinterpret_cast<u32x4*>(vw + r * HD * 2 + ((vch ^ swz(r)) << 4)) = vr[i];
         }
         wave_lds_sync();
-        if (more) load_v(t + NWV);
+        if (more) load_v(t + NW);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
             const bf16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(vw + toff[d]));
@@ -289,20 +319,29 @@ __global__ __launch_bounds__(NWV * 64, 2) void hk_prefix_part_kernel(const Prefi
     }
     __syncthreads();
     constexpr int TPR = HD / 4;                            // threads per row, four dims each
-    for (int r = tid / TPR; r < nrows; r += NWV * 64 / TPR) {
+    for (int r = tid / TPR; r < nrows; r += NW * 64 / TPR) {
         const int c = tid % TPR;
         float M = ml[0][r][0];
 #pragma unroll
-        for (int w = 1; w < NWV; ++w) M = fmaxf(M, ml[w][r][0]);
+        for (int w = 1; w < NW; ++w) M = fmaxf(M, ml[w][r][0]);
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
         float ls = 0.f;
 #pragma unroll
-        for (int w = 0; w < NWV; ++w) {
+        for (int w = 0; w < NW; ++w) {
             const float a = __builtin_amdgcn_exp2f(ml[w][r][0] - M);
             const f32x4 x = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(vlds + w * WB) + r * HD + ((c ^ (r & 7)) << 2));
             ls += a * ml[w][r][1];
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[i] += a * x[i];
+        }
+        if (ONE) {
+            const float inv = inverse_sum(ls);
+            const int row = row0 + r, b = row / p.Nq, i = row - b * p.Nq;
+            u32x2 w;
+            w[0] = pack_bf16x2(o[0] * inv, o[1] * inv);
+            w[1] = pack_bf16x2(o[2] * inv, o[3] * inv);
+            *reinterpret_cast<u32x2*>(p.O + (int64_t)b * p.bso + (int64_t)i * p.ldo + head * HD + 4 * c) = w;
+            continue;
         }
         const int64_t at = ((int64_t)(row0 + r) * p.H + head) * p.ns + slot;
         *reinterpret_cast<f32x4*>(p.part_o + at * HD + 4 * c) = o;
@@ -310,6 +349,13 @@ __global__ __launch_bounds__(NWV * 64, 2) void hk_prefix_part_kernel(const Prefi
             p.part_ml[at * 2] = M;
             p.part_ml[at * 2 + 1] = ls;
         }
+    }    if (ONE && RAW) {                                      // the weights of the one row
+        float M = ml[0][0][0], ls = 0.f;
+#pragma unroll
+        for (int w = 1; w < NW; ++w) M = fmaxf(M, ml[w][0][0]);
+#pragma unroll
+        for (int w = 0; w < NW; ++w) ls += __builtin_amdgcn_exp2f(ml[w][0][0] - M) * ml[w][0][1];
+        add_weights(p, sw, brow, head, rawl, M, inverse_sum(ls), tid, NW * 64);
     }
 }
 
@@ -329,7 +375,7 @@ struct RowsParams {
 };
 
 constexpr int RB = 128;
-constexpr int KT = 64;
+constexpr int KT = 64;               // keys per tile
 constexpr float OVERFLOW_SUM = 1048576.0f;
 
 __device__ __forceinline__ float half_max(float x) {    // the larger of the two lane halves' values (rows live on lane & 31)
@@ -344,7 +390,7 @@ __global__ __launch_bounds__(256, 2) void hk_prefix_rows_kernel(const PrefixPara
     constexpr int STAGE = 2 * KT * ROWB;
     constexpr int RPP = 256 / CH;                          // key rows one workgroup-wide LDS-DMA covers
     constexpr int NP = KT / RPP;                           // of them per operand and tile
-    extern __shared__ __attribute__((aligned(16))) char smem[];      // [2][K | V][64 keys][ROWB], then [2][64] biases
+    extern __shared__ __attribute__((aligned(16))) char smem[];      // [2][K | V][KT keys][ROWB], then [2][KT] biases
     float* blds = reinterpret_cast<float*>(smem + 2 * STAGE);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 31, h = lane >> 5;
@@ -454,8 +500,14 @@ __global__ __launch_bounds__(256, 2) void hk_prefix_rows_kernel(const PrefixPara
     float m = 0.f, l = 0.f;                                // everything stored is relative to m
     bool unset = true, pending = true;                     // this row / some row of the wave has met no key yet
 
-    auto tile = [&](const int t, auto cur_c) __attribute__((always_inline)) {
-        constexpr int cur = decltype(cur_c)::value;
+    if (NT > 0) {
+        issue(0, 0);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (BIAS && nA == 0 && tid < KT) blds[tid] = br;
+        __syncthreads();
+    }
+    for (int t = 0; t < NT; ++t) {
+        const int cur = t & 1;
         if (t + 1 < NT) issue(t + 1, cur ^ 1);
         const bool own = t >= nA;
         const int kt = (own ? t - nA : t) * KT, n = own ? k1 : a1 - a0;
@@ -465,139 +517,203 @@ __global__ __launch_bounds__(256, 2) void hk_prefix_rows_kernel(const PrefixPara
             const char* ks = smem + cur * STAGE;
             const char* vs = ks + KT * ROWB;
             uint64_t gone = 0;                             // keys of this tile that no row has
-            if (BIAS && own) gone = __builtin_amdgcn_ballot_w64(kt + lane >= n || blds[cur * KT + lane] <= REMOVED);
+            bool biased = false;
+            if (BIAS && own) {
+                const float v = blds[cur * KT + lane];
+                gone = __builtin_amdgcn_ballot_w64(kt + lane >= n || v <= REMOVED);
+                biased = __builtin_amdgcn_ballot_w64(v != 0.f) != 0;
+            }
             const bool edge = kt + KT > n || (own && kt + KT - 1 > q0 + off);
             f32x16 st[2];
-            auto scores = [&]() __attribute__((always_inline)) {
-                __builtin_amdgcn_s_setprio(1);
+            auto kread = [&](int i) __attribute__((always_inline)) {   // K fragment of step i: half i / NKS, contraction step i % NKS
+                return *reinterpret_cast<const bf16x8*>(ks + (i / NKS) * 32 * ROWB + (ko ^ (32 * (i % NKS))));
+            };
+            auto vread = [&](int j) __attribute__((always_inline)) {   // V fragment of step j: 16 keys j / NDT, 32 dims j % NDT
+                const char* vp = vs + (j / NDT) * 16 * ROWB + (vo ^ (64 * (j % NDT)));
+                const bf16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(vp));
+                const bf16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(vp + 8 * ROWB));
+                bf16x8 vf;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    vf[x] = v0[x];
+                    vf[x + 4] = v1[x];
+                }
+                return vf;
+            };
+            const bool plain = !pending && !edge && !(BIAS && (biased || gone));
+            int from = 0;                                  // the tile's keys from here on are left to the general form below
+            if (plain) {
+                // The ordinary tile, by halves of 32 keys, one matrix instruction after the other with what fits beside it:
+                //   S(0)   |   S(1), exp of half 0   |   P(0) . V, exp of half 1   |   P(1) . V
+                // fragments are read four instructions ahead; sched_barrier keeps the order (left to itself the compiler reads into one
+                // set of registers and waits for every read right before its use).
+                bf16x8 kf[4], vf[4];
+                float e0 = 0.f, e1 = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) kf[i] = kread(i);
                 f32x16 c0;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) c0[i] = -m;
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int s = 0; s < NKS; ++s)              // two independent chains
+                for (int i = 0; i < 2 * NKS; ++i) {
+                    const int g = i / NKS, s = i % NKS;
+                    st[g] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i & 3], qf[s], s == 0 ? c0 : st[g], 0, 0, 0);
+                    if (i + 4 < 2 * NKS) kf[i & 3] = kread(i + 4);
+                    else vf[i + 4 - 2 * NKS] = vread(i + 4 - 2 * NKS);
+                    if (g == 1 && s >= NKS / 4) {          // half 0's scores have left the matrix unit
+                        constexpr int ST = NKS - NKS / 4;
+                        const int x = s - NKS / 4;
 #pragma unroll
-                    for (int g = 0; g < 2; ++g) {
-                        const bf16x8 kf = *reinterpret_cast<const bf16x8*>(ks + g * 32 * ROWB + (ko ^ (32 * s)));
-                        st[g] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[s], s == 0 ? c0 : st[g], 0, 0, 0);
-                    }
-                __builtin_amdgcn_s_setprio(0);
-                if (BIAS && own) {                         // register 4 x + j of st[g] <-> key 32 g + 8 x + 4 h + j
-#pragma unroll
-                    for (int g = 0; g < 2; ++g)
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const f32x4 bv = *reinterpret_cast<const f32x4*>(blds + cur * KT + 32 * g + 8 * x + 4 * h);
-                            const uint32_t gb = (uint32_t)(gone >> (32 * g + 8 * x)) >> (4 * h);
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) st[g][4 * x + j] = (gb >> j) & 1 ? -INFINITY : st[g][4 * x + j] + bv[j] * HK_LOG2E;
+                        for (int y = 16 * x / ST; y < 16 * (x + 1) / ST; ++y) {
+                            st[0][y] = __builtin_amdgcn_exp2f(st[0][y]);
+                            e0 += st[0][y];
                         }
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                if (edge) {
-                    const int lim = min(n - 1, own ? q0 + r + off : n - 1) - kt - 4 * h;
+                auto pack = [&](int s) __attribute__((always_inline)) {
+                    u32x4 w;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(st[s >> 1][8 * (s & 1) + 2 * j], st[s >> 1][8 * (s & 1) + 2 * j + 1]);
+                    return __builtin_bit_cast(bf16x8, w);
+                };
+                if (__builtin_amdgcn_ballot_w64(!(e0 <= OVERFLOW_SUM)) == 0) {
+                    l += e0;
+                    bf16x8 pf[2] = {pack(0), pack(1)};
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int j = 0; j < 2 * NDT; ++j) {
+                        ot[j % NDT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[j & 3], pf[j / NDT], ot[j % NDT], 0, 0, 0);
+                        if (j + 4 < 4 * NDT) vf[j & 3] = vread(j + 4);
+#pragma unroll
+                        for (int y = 16 * j / (2 * NDT); y < 16 * (j + 1) / (2 * NDT); ++y) {
+                            st[1][y] = __builtin_amdgcn_exp2f(st[1][y]);
+                            e1 += st[1][y];
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    from = 32;
+                    if (__builtin_amdgcn_ballot_w64(!(e1 <= OVERFLOW_SUM)) == 0) {
+                        l += e1;
+                        pf[0] = pack(2);
+                        pf[1] = pack(3);
+                        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                        for (int j = 2 * NDT; j < 4 * NDT; ++j) {
+                            ot[j % NDT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[j & 3], pf[j / NDT - 2], ot[j % NDT], 0, 0, 0);
+                            if (j + 4 < 4 * NDT) vf[j & 3] = vread(j + 4);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                        from = 64;
+                    }
+                }
+            }
+            if (from < 64) {
+                // ends, diagonals, biases, rows without a key so far, scores that outgrew m: the tile as a whole, masks and all
+                float rs;
+                auto scores = [&]() __attribute__((always_inline)) {
+                    f32x16 c0;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) c0[i] = -m;
+#pragma unroll
+                    for (int s = 0; s < NKS; ++s)              // two independent chains
+#pragma unroll
+                        for (int g = 0; g < 2; ++g) st[g] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kread(g * NKS + s), qf[s], s == 0 ? c0 : st[g], 0, 0, 0);
+                    if (BIAS && biased) {                      // register 4 x + j of st[g] <-> key 32 g + 8 x + 4 h + j
+#pragma unroll
+                        for (int g = 0; g < 2; ++g)
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) {
+                                const f32x4 bv = *reinterpret_cast<const f32x4*>(blds + cur * KT + 32 * g + 8 * x + 4 * h);
+                                const uint32_t gb = (uint32_t)(gone >> (32 * g + 8 * x)) >> (4 * h);
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) st[g][4 * x + j] = (gb >> j) & 1 ? -INFINITY : st[g][4 * x + j] + bv[j] * HK_LOG2E;
+                            }
+                    }
+                    if (edge || from) {
+                        const int lim = min(n - 1, own ? q0 + r + off : n - 1) - kt - 4 * h;
+#pragma unroll
+                        for (int g = 0; g < 2; ++g)
+#pragma unroll
+                            for (int i = 0; i < 16; ++i)
+                                if (32 * g + (i & 3) + 8 * (i >> 2) > lim || (g == 0 && from)) st[g][i] = -INFINITY;
+                    }
+                };
+                auto exp_sum = [&]() __attribute__((always_inline)) {
+                    rs = 0.f;
 #pragma unroll
                     for (int g = 0; g < 2; ++g)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (32 * g + (i & 3) + 8 * (i >> 2) > lim) st[g][i] = -INFINITY;
-                }
-            };
-            float rs;
-            auto exp_sum = [&]() __attribute__((always_inline)) {
-                rs = 0.f;
+                        for (int i = 0; i < 16; ++i) {
+                            const float e = __builtin_amdgcn_exp2f(st[g][i]);
+                            st[g][i] = e;
+                            rs += e;
+                        }
+                };
+                auto move_max = [&]() __attribute__((always_inline)) {
+                    float mx = fmaxf(st[0][0], st[1][0]);
 #pragma unroll
-                for (int g = 0; g < 2; ++g)
+                    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, fmaxf(st[0][i], st[1][i]));
+                    mx = half_max(mx);
+                    const float delta = unset ? (mx == -INFINITY ? 0.f : mx) : fmaxf(mx, 0.f);
+                    const float a = unset ? 0.f : __builtin_amdgcn_exp2f(-delta);
+                    unset = unset && mx == -INFINITY;
+                    pending = __builtin_amdgcn_ballot_w64(unset) != 0;
+                    m += delta;
+                    l *= a;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float e = __builtin_amdgcn_exp2f(st[g][i]);
-                        st[g][i] = e;
-                        rs += e;
+                    for (int d = 0; d < NDT; ++d)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) ot[d][i] *= a;
+#pragma unroll
+                    for (int g = 0; g < 2; ++g)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) st[g][i] -= delta;
+                };
+                auto pv = [&](const bf16x8* pf, auto masked_c) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int s = 0; s < 4; ++s) {
+                        u32x4 keep = {~0u, ~0u, ~0u, ~0u};
+                        if (decltype(masked_c)::value) {       // elements 0-3: keys 16 s + 4 h + j, elements 4-7: 8 further
+                            const uint32_t g = (uint32_t)(gone >> (16 * s)) >> (4 * h);
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                keep[j] = ((g >> (2 * j)) & 1 ? 0u : 0xffffu) | ((g >> (2 * j + 1)) & 1 ? 0u : 0xffff0000u);
+                                keep[j + 2] = ((g >> (8 + 2 * j)) & 1 ? 0u : 0xffffu) | ((g >> (8 + 2 * j + 1)) & 1 ? 0u : 0xffff0000u);
+                            }
+                        }
+#pragma unroll
+                        for (int d = 0; d < NDT; ++d) {
+                            bf16x8 vf = vread(s * NDT + d);
+                            if (decltype(masked_c)::value) vf = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, vf) & keep);
+                            ot[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[s], ot[d], 0, 0, 0);
+                        }
                     }
-            };
-            auto move_max = [&]() __attribute__((always_inline)) {
-                float mx = fmaxf(st[0][0], st[1][0]);
-#pragma unroll
-                for (int i = 1; i < 16; ++i) mx = fmaxf(mx, fmaxf(st[0][i], st[1][i]));
-                mx = half_max(mx);
-                const float delta = unset ? (mx == -INFINITY ? 0.f : mx) : fmaxf(mx, 0.f);
-                const float a = unset ? 0.f : __builtin_amdgcn_exp2f(-delta);
-                unset = unset && mx == -INFINITY;
-                pending = __builtin_amdgcn_ballot_w64(unset) != 0;
-                m += delta;
-                l *= a;
-#pragma unroll
-                for (int d = 0; d < NDT; ++d)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) ot[d][i] *= a;
-#pragma unroll
-                for (int g = 0; g < 2; ++g)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) st[g][i] -= delta;
-            };
-            for (bool take = pending;; take = true) {      // at most twice
-                scores();
-                if (take) move_max();
-                exp_sum();
-                if (take || __builtin_amdgcn_ballot_w64(!(rs <= OVERFLOW_SUM)) == 0) break;
-            }
-            l += rs;
-            __builtin_amdgcn_s_setprio(2);
-            bf16x8 pf[4];                                  // P in bf16, the matrix instruction's operand; l sums the unrounded values
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                u32x4 w;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(st[s >> 1][8 * (s & 1) + 2 * j], st[s >> 1][8 * (s & 1) + 2 * j + 1]);
-                pf[s] = __builtin_bit_cast(bf16x8, w);
-            }
-            auto pv = [&](auto masked_c) __attribute__((always_inline)) {
+                };
+                for (bool take = pending || plain;; take = true) {      // at most twice
+                    scores();
+                    if (take) move_max();
+                    exp_sum();
+                    if (take || __builtin_amdgcn_ballot_w64(!(rs <= OVERFLOW_SUM)) == 0) break;
+                }
+                l += rs;
+                bf16x8 pf[4];                                  // P in bf16, the matrix instruction's operand; l sums the unrounded values
 #pragma unroll
                 for (int s = 0; s < 4; ++s) {
-                    u32x4 keep = {~0u, ~0u, ~0u, ~0u};
-                    if (decltype(masked_c)::value) {       // elements 0-3: keys 16 s + 4 h + j, elements 4-7: 8 further
-                        const uint32_t g = (uint32_t)(gone >> (16 * s)) >> (4 * h);
+                    u32x4 w;
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            keep[j] = ((g >> (2 * j)) & 1 ? 0u : 0xffffu) | ((g >> (2 * j + 1)) & 1 ? 0u : 0xffff0000u);
-                            keep[j + 2] = ((g >> (8 + 2 * j)) & 1 ? 0u : 0xffffu) | ((g >> (8 + 2 * j + 1)) & 1 ? 0u : 0xffff0000u);
-                        }
-                    }
-#pragma unroll
-                    for (int d = 0; d < NDT; ++d) {
-                        const char* vp = vs + s * 16 * ROWB + (vo ^ (64 * d));
-                        const bf16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(vp));
-                        const bf16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(vp + 8 * ROWB));
-                        bf16x8 vf;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            vf[j] = v0[j];
-                            vf[j + 4] = v1[j];
-                        }
-                        if (decltype(masked_c)::value) vf = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, vf) & keep);
-                        ot[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[s], ot[d], 0, 0, 0);
-                    }
+                    for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(st[s >> 1][8 * (s & 1) + 2 * j], st[s >> 1][8 * (s & 1) + 2 * j + 1]);
+                    pf[s] = __builtin_bit_cast(bf16x8, w);
                 }
-            };
-            if (BIAS && gone) pv(std::true_type{});
-            else pv(std::false_type{});
-            __builtin_amdgcn_s_setprio(0);
+                if (BIAS && gone) pv(pf, std::true_type{});
+                else pv(pf, std::false_type{});
+            }
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the next tile's LDS-DMA, unknown to the compiler
         if (BIAS && t + 1 >= nA && t + 1 < NT && tid < KT) blds[(cur ^ 1) * KT + tid] = br;
         __syncthreads();
-    };
-
-    if (NT > 0) {
-        issue(0, 0);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        if (BIAS && nA == 0 && tid < KT) blds[tid] = br;
-        __syncthreads();
     }
-    int t = 0;
-    for (; t + 1 < NT; t += 2) {
-        tile(t, std::integral_constant<int, 0>{});
-        tile(t + 1, std::integral_constant<int, 1>{});
-    }
-    if (t < NT) tile(t, std::integral_constant<int, 0>{});
 
     l += __shfl_xor(l, 32, 64);
     if (q0 + r >= nrows) return;
@@ -615,7 +731,7 @@ __global__ __launch_bounds__(256, 2) void hk_prefix_rows_kernel(const PrefixPara
             p.part_ml[at * 2 + 1] = l;
         }
     } else {
-        const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
+        const float inv = inverse_sum(l);
         const int b = row / p.Nq, i = row - b * p.Nq;
         __bf16* op = p.O + (int64_t)b * p.bso + (int64_t)i * p.ldo + head * HD + 4 * h;
 #pragma unroll
@@ -665,8 +781,6 @@ __device__ __forceinline__ void join_share(const float* mlp, const float* op, in
         }
     }
 }
-__device__ __forceinline__ float inverse_sum(float l) { return l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l); }     // no key: 0; NaN stays
-
 // o = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), no key at all: zeros.  HD / 4 threads per row and slot group (four dims each),
 // SG groups per row, joined in group order.
 template <int HD, int SG>
@@ -712,13 +826,8 @@ __global__ __launch_bounds__(256) void hk_prefix_join_kernel(const PrefixParams 
     *reinterpret_cast<u32x2*>(p.O + (int64_t)b * p.bso + (int64_t)i * p.ldo + head * HD + 4 * c) = w;
 }
 
-// The same for one decode step, and its weights: w_out[j] = w_in[j] + 2^(s_j - M) / l from the scores the first launch left.  One workgroup
-// per (sequence, head) and 2048 keys; all its groups share the slots.
-struct StepWeights {
-    const float* w_in;               // may be w_out; NULL = zeros
-    float* w_out;
-    int64_t wi_bs, wi_hs, wo_bs, wo_hs;
-};
+// The same for one decode step, and its weights from the scores the first launch left.  One workgroup per (sequence, head) and 2048 keys; all
+// its groups share the slots.
 template <int HD>
 __global__ __launch_bounds__(256) void hk_step_join_kernel(const PrefixParams p, const StepWeights sw) {
     constexpr int TPR = HD / 4, SG = 256 / TPR;
@@ -755,15 +864,11 @@ __global__ __launch_bounds__(256) void hk_step_join_kernel(const PrefixParams p,
         w[1] = pack_bf16x2(o[2] * inv, o[3] * inv);
         *reinterpret_cast<u32x2*>(p.O + (int64_t)b * p.bso + head * HD + 4 * c) = w;
     }
-    const float* rp = p.raw + rh * p.raw_ld;
-    const float* wi = sw.w_in ? sw.w_in + (int64_t)b * sw.wi_bs + (int64_t)head * sw.wi_hs : nullptr;
-    float* wo = sw.w_out + (int64_t)b * sw.wo_bs + (int64_t)head * sw.wo_hs;
-    for (int j = blockIdx.z * 256 + tid; j < p.Nk; j += gridDim.z * 256)
-        wo[j] = (wi ? wi[j] : 0.f) + __builtin_amdgcn_exp2f(rp[j] - M) * inv;
+    add_weights(p, sw, b, head, p.raw + rh * p.raw_ld, M, inv, blockIdx.z * 256 + tid, gridDim.z * 256);
 }
 
 // ---------------------------------------------------------------- host side
-enum { SMALL, MIXED, PACKED, FUSED };
+enum { ONCE, SMALL, MIXED, PACKED, FUSED };
 struct Plan {
     int mode, rt;
     RowsParams rows;
@@ -795,15 +900,28 @@ Plan make_plan(PrefixParams& p, int hd, bool raw) {
     p.norg = (p.Nq + m.rt * 16 - 1) / (m.rt * 16);
     const int64_t H = p.H, B = p.B;
     const int all = 1 << 28;
+    // One launch, a workgroup per (sequence, head) for all its keys, or chunks and a join?  Measured in a graph, 32 heads of 128 (us, one : two
+    // launches).  One sequence, 55 / 372 / 720 keys: 4.6 : 6.3, 7.3 : 6.8, 10.8 : 7.1 - and a launch costs the host 2.6.  The prefix is
+    // read once per sequence here: 16 sequences over 352 + 20 keys 13.0 : 8.8.  Without one nothing is read twice, and 256 pairs fill the
+    // chip: 8 sequences' step over 353 / 1000 keys 11.3 : 15.8, 23.5 : 26.3; 4 sequences' over 1000 15.9 : 18.4, one's 13.7 : 8.0; 32 sequences'
+    // over 100 20.7 : 16.6.
+    const int64_t pairs = H * B, keys = (int64_t)p.P + p.Nk;
+    if (p.Nq <= 16 && (p.P > 0 ? pairs <= 256 && keys <= 384 : pairs <= 512 && (keys <= 384 || (pairs >= 128 && keys <= MAX_CHUNK)))) {
+        m.mode = ONCE;
+        m.rt = 1;
+        p.norg = 1;
+        p.ns = 0;
+        return m;
+    }
     if (p.Nq <= 32) {
         m.mode = p.R > 64 && p.P > 0 ? MIXED : SMALL;
         if (m.mode == SMALL) p.npc = cut(p.P, H * p.nprg, HK_PREFIX_WANT, NWV * TK, MAX_CHUNK, &p.pc);
-        else p.npc = cut(p.P, H * m.rows.npb, 512, KT, all, &p.pc);
+        else p.npc = cut(p.P, H * m.rows.npb, HK_ROWS_WANT, KT, all, &p.pc);
         p.noc = cut(p.Nk, B * H * p.norg, HK_PREFIX_WANT, NWV * TK, MAX_CHUNK, &p.oc);
     } else {
         // time of a 128-row x 64-key tile when 512 workgroups (two per CU) run: about 1 us; a lone workgroup's is not much shorter
-        p.npc = cut(p.P, H * m.rows.npb, 512, KT, all, &p.pc);
-        p.noc = cut(p.Nk, H * B * m.rows.nob, 512, KT, all, &p.oc);
+        p.npc = cut(p.P, H * m.rows.npb, HK_ROWS_WANT, KT, all, &p.pc);
+        p.noc = cut(p.Nk, H * B * m.rows.nob, HK_ROWS_WANT, KT, all, &p.oc);
         const double own = (double)H * B * m.rows.nob * ((p.Nk + KT - 1) / KT), pre = (double)((p.P + KT - 1) / KT);
         const double fused_n = (double)H * B * m.rows.nob;
         double fused = (own + fused_n * pre) / (fused_n < 512 ? fused_n : 512);
@@ -828,7 +946,7 @@ void set_parts(PrefixParams& p, void* ws, int hd) {
     p.part_o = reinterpret_cast<float*>(ws);
     p.part_ml = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + up16((size_t)p.ns * p.R * p.H * hd * 4));
 }
-int64_t part_grid(const PrefixParams& p) { return p.pjobs + (int64_t)p.B * p.noc * p.H * p.norg; }
+int64_t part_grid(const PrefixParams& p) { return p.ns == 0 ? (int64_t)p.B * p.H : p.pjobs + (int64_t)p.B * p.noc * p.H * p.norg; }
 int64_t rows_grid(const PrefixParams& p, const Plan& m) {
     const int64_t own = (int64_t)p.B * m.rows.nob * p.H;
     return m.mode == MIXED ? m.rows.pjobs : m.mode == PACKED ? m.rows.pjobs + own * p.noc : own;
@@ -836,7 +954,13 @@ int64_t rows_grid(const PrefixParams& p, const Plan& m) {
 
 template <int HD, int RT, bool BIAS, bool RAW>
 void launch_part(const PrefixParams& p, hipStream_t s) {
-    hipLaunchKernelGGL((hk_prefix_part_kernel<HD, RT, BIAS, RAW>), dim3((unsigned)part_grid(p)), dim3(NWV * 64), 0, s, p);
+    hipLaunchKernelGGL((hk_prefix_part_kernel<HD, RT, BIAS, RAW, NWV, false>), dim3((unsigned)part_grid(p)), dim3(NWV * 64), 0, s, p, StepWeights{});
+}
+template <int HD, bool RAW>
+void launch_once(const PrefixParams& p, const StepWeights& sw, hipStream_t s) {
+    const dim3 grid((unsigned)(p.B * p.H));
+    if (p.bias) hipLaunchKernelGGL((hk_prefix_part_kernel<HD, 1, true, RAW, 8, true>), grid, dim3(512), 0, s, p, sw);
+    else hipLaunchKernelGGL((hk_prefix_part_kernel<HD, 1, false, RAW, 8, true>), grid, dim3(512), 0, s, p, sw);
 }
 template <int HD, bool BIAS>
 int launch_rows(const PrefixParams& p, const Plan& m, hipStream_t s) {
@@ -857,6 +981,10 @@ void launch_join(const PrefixParams& p, hipStream_t s) {
 }
 template <int HD>
 int launch_prefix(const PrefixParams& p, const Plan& m, hipStream_t s) {
+    if (m.mode == ONCE) {
+        launch_once<HD, false>(p, StepWeights{}, s);
+        return HK_OK;
+    }
     if (m.mode != SMALL) {
         // MIXED: the rows kernel reads the prefix only, which has no bias
         const int rc = p.bias && m.mode != MIXED ? launch_rows<HD, true>(p, m, s) : launch_rows<HD, false>(p, m, s);
@@ -876,7 +1004,11 @@ int launch_prefix(const PrefixParams& p, const Plan& m, hipStream_t s) {
     return HK_OK;
 }
 template <int HD>
-void launch_step(const PrefixParams& p, const StepWeights& sw, hipStream_t s) {
+void launch_step(const PrefixParams& p, const Plan& m, const StepWeights& sw, hipStream_t s) {
+    if (m.mode == ONCE) {
+        launch_once<HD, true>(p, sw, s);
+        return;
+    }
     if (p.bias) launch_part<HD, 1, true, true>(p, s);
     else launch_part<HD, 1, false, true>(p, s);
     const int z = p.Nk < 2048 * 64 ? (p.Nk + 2047) / 2048 : 64;
@@ -1005,7 +1137,7 @@ extern "C" int hk_decode_attn_weights_bf16(const hk_step_weights_desc* d, void* 
     p.bias_bs = d->bias_bs;
     p.bias_hs = d->bias_hs;
     p.raw_ld = (d->n_keys + TK - 1) / TK * TK;
-    make_plan(p, d->head_dim, true);
+    const Plan m = make_plan(p, d->head_dim, true);
     const size_t parts = part_bytes(p, d->head_dim), need = parts + (size_t)p.B * p.H * p.raw_ld * 4;
     HK_REQUIRE(d->ws && d->ws_bytes >= need, "hk_decode_attn_weights_bf16: workspace of %zu bytes, %zu needed (hk_decode_attn_weights_ws)",
                d->ws ? d->ws_bytes : (size_t)0, need);
@@ -1025,8 +1157,8 @@ extern "C" int hk_decode_attn_weights_bf16(const hk_step_weights_desc* d, void* 
     p.raw = reinterpret_cast<float*>(reinterpret_cast<char*>(d->ws) + parts);
     StepWeights sw = {d->w_in, d->w_out, d->wi_bs, d->wi_hs, d->wo_bs, d->wo_hs};
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    if (d->head_dim == 128) launch_step<128>(p, sw, s);
-    else launch_step<64>(p, sw, s);
+    if (d->head_dim == 128) launch_step<128>(p, m, sw, s);
+    else launch_step<64>(p, m, sw, s);
     HK_CHECK_LAUNCH("hk_decode_attn_weights_bf16");
     return HK_OK;
 }
