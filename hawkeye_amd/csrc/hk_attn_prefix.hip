@@ -546,7 +546,9 @@ __global__ __launch_bounds__(256, 2) void hk_prefix_rows_kernel(const PrefixPara
                 // The ordinary tile, by halves of 32 keys, one matrix instruction after the other with what fits beside it:
                 //   S(0)   |   S(1), exp of half 0   |   P(0) . V, exp of half 1   |   P(1) . V
                 // fragments are read four instructions ahead; sched_barrier keeps the order (left to itself the compiler reads into one
-                // set of registers and waits for every read right before its use).
+                // set of registers and waits for every read right before its use).  A wave that feeds the matrix unit goes before one that does not
+                // (8 x 512 questions' tokens over 1400: 130 us without the priorities, 124 with).
+                __builtin_amdgcn_s_setprio(1);
                 bf16x8 kf[4], vf[4];
                 float e0 = 0.f, e1 = 0.f;
 #pragma unroll
@@ -581,6 +583,7 @@ __global__ __launch_bounds__(256, 2) void hk_prefix_rows_kernel(const PrefixPara
                 if (__builtin_amdgcn_ballot_w64(!(e0 <= OVERFLOW_SUM)) == 0) {
                     l += e0;
                     bf16x8 pf[2] = {pack(0), pack(1)};
+                    __builtin_amdgcn_s_setprio(2);
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int j = 0; j < 2 * NDT; ++j) {
@@ -608,6 +611,7 @@ __global__ __launch_bounds__(256, 2) void hk_prefix_rows_kernel(const PrefixPara
                         from = 64;
                     }
                 }
+                __builtin_amdgcn_s_setprio(0);
             }
             if (from < 64) {
                 // ends, diagonals, biases, rows without a key so far, scores that outgrew m: the tile as a whole, masks and all
