@@ -26,12 +26,9 @@ constexpr float M_NONE = -1.0e30f;   // running maximum of a row that has met no
 constexpr int TK = 32;               // keys per tile
 constexpr int NWV = 4;               // waves per workgroup
 constexpr int MAX_CHUNK = 1024;      // keys per chunk at most: the chunk's bias lives in LDS
-#ifndef HK_ROWS_WANT
-#define HK_ROWS_WANT 320
-#endif
-#ifndef HK_PREFIX_WANT
-#define HK_PREFIX_WANT 1024          // workgroups per launch the chunks are cut for
-#endif
+// Workgroups the chunks are cut for.  256 / 512 / 1024 / 2048 measured within 2 % of each other for shared prefixes, 91 / 91 / 80 / 79 us for 16
+// sequences' own 1500 keys; 128-row blocks: 7 x 37 rows over 1201 keys 42 / 29 / 26 / 36 us at 128 / 256 / 320 / 512, 512 rows over 1400 48 / 37 / 37 / 54.
+constexpr int PART_WANT = 1024, ROWS_WANT = 320;
 
 struct PrefixParams {
     const __bf16 *Q, *KP, *VP, *K, *V;
@@ -891,9 +888,9 @@ int cut(int keys, int64_t per, int64_t want, int unit, int most, int* chunk) {
     return (int)((keys + c - 1) / c);
 }
 
-// Which kernel takes what.  Up to 32 queries per sequence, own keys are bound by reading them: hk_prefix_part_kernel.  So is the prefix up to 64
-// rows in all; beyond, its rows fill 128-row blocks (MIXED).  More queries: hk_prefix_rows_kernel for both, in one workgroup (FUSED) or apart
-// (PACKED), whichever the estimate below finds shorter.
+// Which kernel takes what.  Up to 32 queries per sequence, own keys are bound by reading them: hk_prefix_part_kernel.  So is the prefix as long
+// as few rows share it (SMALL); beyond, its rows fill 128-row blocks (MIXED).  More queries: hk_prefix_rows_kernel for both, in one
+// workgroup (FUSED) or apart (PACKED), whichever the estimate below finds shorter.
 Plan make_plan(PrefixParams& p, int hd, bool raw) {
     Plan m = {};
     p.R = p.B * p.Nq;
@@ -918,14 +915,19 @@ Plan make_plan(PrefixParams& p, int hd, bool raw) {
         return m;
     }
     if (p.Nq <= 32) {
-        m.mode = p.R > 64 && p.P > 0 ? MIXED : SMALL;
-        if (m.mode == SMALL) p.npc = cut(p.P, H * p.nprg, HK_PREFIX_WANT, NWV * TK, MAX_CHUNK, &p.pc);
-        else p.npc = cut(p.P, H * m.rows.npb, HK_ROWS_WANT, KT, all, &p.pc);
-        p.noc = cut(p.Nk, B * H * p.norg, HK_PREFIX_WANT, NWV * TK, MAX_CHUNK, &p.oc);
+        // hk_prefix_part_kernel goes over the prefix again for every 32 rows, hk_prefix_rows_kernel for every 128, but is a launch more and
+        // leaves blocks part empty.  SMALL : MIXED, 32 heads of 128 (us): 64 rows over 1000 / 1985 / 16384 keys 27.5 : 31.5, 36.4 : 34.4, 153 : 136;
+        // 128 rows over 200 / 1000 / 1985 15.0 : 21.4, 27.2 : 27.0, 35.0 : 27.8; 256 over 200 / 1000 19.2 : 29.4, 37.5 : 30.9;
+        // heads of 64, 128 rows over 1000 / 4096 16.9 : 19.0, 31.5 : 25.1.
+        const int64_t again = ((p.R + 31) / 32 - m.rows.npb) * (int64_t)p.P * hd * H;
+        m.mode = again >= 9600000 ? MIXED : SMALL;
+        if (m.mode == SMALL) p.npc = cut(p.P, H * p.nprg, PART_WANT, NWV * TK, MAX_CHUNK, &p.pc);
+        else p.npc = cut(p.P, H * m.rows.npb, ROWS_WANT, KT, all, &p.pc);
+        p.noc = cut(p.Nk, B * H * p.norg, PART_WANT, NWV * TK, MAX_CHUNK, &p.oc);
     } else {
         // time of a 128-row x 64-key tile when 512 workgroups (two per CU) run: about 1 us; a lone workgroup's is not much shorter
-        p.npc = cut(p.P, H * m.rows.npb, HK_ROWS_WANT, KT, all, &p.pc);
-        p.noc = cut(p.Nk, H * B * m.rows.nob, HK_ROWS_WANT, KT, all, &p.oc);
+        p.npc = cut(p.P, H * m.rows.npb, ROWS_WANT, KT, all, &p.pc);
+        p.noc = cut(p.Nk, H * B * m.rows.nob, ROWS_WANT, KT, all, &p.oc);
         const double own = (double)H * B * m.rows.nob * ((p.Nk + KT - 1) / KT), pre = (double)((p.P + KT - 1) / KT);
         const double fused_n = (double)H * B * m.rows.nob;
         double fused = (own + fused_n * pre) / (fused_n < 512 ? fused_n : 512);

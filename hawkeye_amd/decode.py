@@ -21,7 +21,7 @@ import torch
 from . import lib as L
 from . import ops
 from .engine import _Pool
-from .llm import LOG2E, LlamaPrefill, PromptPrefix
+from .llm import LOG2E, MAX_PLANS, LlamaPrefill, PromptPrefix
 
 MAX_ROWS = 16          # sequences per step hk_gemv_bf16 takes
 ROW_GRANULE = 64       # cache rows are allocated in multiples of this, so nearby prompt lengths share one plan
@@ -82,13 +82,17 @@ class LlamaGenerator:
         key = (B, rows, masked, P, weights)
         plan = self.plans.get(key)
         if plan is not None and plan.pool_epoch == self.pool.epoch:
+            self.plans[key] = self.plans.pop(key)      # most recently used last
             return plan
+        self.plans.pop(key, None)
         epoch = self.pool.epoch
         plan = self._build_plan(B, rows, masked, P, weights)
         if self.pool.epoch != epoch:
             self.plans.clear()
         plan.pool_epoch = self.pool.epoch
         self.plans[key] = plan
+        while len(self.plans) > MAX_PLANS:             # every prefix length makes one
+            del self.plans[next(iter(self.plans))]
         return plan
 
     def _build_plan(self, B: int, rows: int, masked: bool, P_rows: int = 0, weights: bool = False) -> _DecodePlan:

@@ -436,6 +436,20 @@ def test_a_bounded_cache_follows_its_definition_step_by_step(lengths):
         gen.generate(src=ask, cache_recent=3, max_new_tokens=2)
 
 
+def test_plans_of_many_prefixes_stay_bounded():
+    from hawkeye_amd.llm import MAX_PLANS
+    cfg, pre, gen = _llm(25)
+    prefix, ask, _, video = _prompt(cfg, 100, [4, 4], 25)
+    first = None
+    for P in list(range(20, 20 + MAX_PLANS + 3)) + [20]:
+        pf = pre.make_prefix(src=prefix[:, :P], video=video)
+        out = gen.generate(src=ask, prefix=pf, max_new_tokens=2, return_logits=True)
+        if P == 20 and first is None:
+            first = out
+    assert len(gen.plans) <= MAX_PLANS and len(pre.plans) <= MAX_PLANS
+    assert torch.equal(out["logits"], first["logits"]) and torch.equal(out["tokens"], first["tokens"])
+
+
 def test_streams_graphs_and_strides():
     """Another stream, a captured call replayed with eager work between, and caches whose offsets pass 2^31 elements."""
     B, H, hd, P, n = 3, 2, 128, 300, 90
