@@ -27,8 +27,8 @@ constexpr int TK = 32;               // keys per tile
 constexpr int NWV = 4;               // waves per workgroup
 constexpr int MAX_CHUNK = 1024;      // keys per chunk at most: the chunk's bias lives in LDS
 // Workgroups the chunks are cut for.  256 / 512 / 1024 / 2048 measured within 2 % of each other for shared prefixes, 91 / 91 / 80 / 79 us for 16
-// sequences' own 1500 keys; 128-row blocks: 7 x 37 rows over 1201 keys 42 / 29 / 26 / 36 us at 128 / 256 / 320 / 512, 512 rows over 1400 48 / 37 / 37 / 54.
-constexpr int PART_WANT = 1024, ROWS_WANT = 320;
+// sequences' own 1500 keys.  128-row blocks (one per CU) want as many as there are CUs: see cut_rows.
+constexpr int PART_WANT = 1024, ROWS_WANT = 256;
 
 struct PrefixParams {
     const __bf16 *Q, *KP, *VP, *K, *V;
@@ -888,6 +888,16 @@ int cut(int keys, int64_t per, int64_t want, int unit, int most, int* chunk) {
     return (int)((keys + c - 1) / c);
 }
 
+// The same for 128-row blocks: the nearest count to ROWS_WANT, but two chunks rather than one wherever a launch leaves CUs without a block.
+// Measured, 32 heads of 128 (us at so many chunks): 1 block of rows over 16384 keys 187 / 158 / 160 / 161 at 4 / 8 / 12 / 16, 2 over 1201
+// 22.9 / 21.8 / 21.8 / 22.9 at 2 / 3 / 4 / 5, 3 over 1985 48 / 33 / 28 / 31 at 1 / 2 / 3 / 4, 5 over 1201 37 / 32 / 36 at 1 / 2 / 3, 6 over
+// 2500 62 / 53 / 65 at 1 / 2 / 3; 8 heads of 64, 13 blocks over 1500 32 / 25 / 27 at 1 / 2 / 3.
+int cut_rows(int keys, int64_t per, int* chunk) {
+    int64_t n = (ROWS_WANT + per / 2) / per;
+    if (n < 2 && per < ROWS_WANT) n = 2;
+    return cut(keys, per, per * n, KT, 1 << 28, chunk);
+}
+
 // Which kernel takes what.  Up to 32 queries per sequence, own keys are bound by reading them: hk_prefix_part_kernel.  So is the prefix as long
 // as few rows share it (SMALL); beyond, its rows fill 128-row blocks (MIXED).  More queries: hk_prefix_rows_kernel for both, in one
 // workgroup (FUSED) or apart (PACKED), whichever the estimate below finds shorter.
@@ -900,7 +910,6 @@ Plan make_plan(PrefixParams& p, int hd, bool raw) {
     p.nprg = (p.R + m.rt * 16 - 1) / (m.rt * 16);
     p.norg = (p.Nq + m.rt * 16 - 1) / (m.rt * 16);
     const int64_t H = p.H, B = p.B;
-    const int all = 1 << 28;
     // One launch, a workgroup per (sequence, head) for all its keys, or chunks and a join?  Measured in a graph, 32 heads of 128 (us, one : two
     // launches).  One sequence, 55 / 372 / 720 keys: 4.6 : 6.3, 7.3 : 6.8, 10.8 : 7.1 - and a launch costs the host 2.6.  The prefix is
     // read once per sequence here: 16 sequences over 352 + 20 keys 13.0 : 8.8.  Without one nothing is read twice, and 256 pairs fill the
@@ -922,12 +931,12 @@ Plan make_plan(PrefixParams& p, int hd, bool raw) {
         const int64_t again = ((p.R + 31) / 32 - m.rows.npb) * (int64_t)p.P * hd * H;
         m.mode = again >= 9600000 ? MIXED : SMALL;
         if (m.mode == SMALL) p.npc = cut(p.P, H * p.nprg, PART_WANT, NWV * TK, MAX_CHUNK, &p.pc);
-        else p.npc = cut(p.P, H * m.rows.npb, ROWS_WANT, KT, all, &p.pc);
+        else p.npc = cut_rows(p.P, H * m.rows.npb, &p.pc);
         p.noc = cut(p.Nk, B * H * p.norg, PART_WANT, NWV * TK, MAX_CHUNK, &p.oc);
     } else {
         // time of a 128-row x 64-key tile when 512 workgroups (two per CU) run: about 1 us; a lone workgroup's is not much shorter
-        p.npc = cut(p.P, H * m.rows.npb, ROWS_WANT, KT, all, &p.pc);
-        p.noc = cut(p.Nk, H * B * m.rows.nob, ROWS_WANT, KT, all, &p.oc);
+        p.npc = cut_rows(p.P, H * m.rows.npb, &p.pc);
+        p.noc = cut_rows(p.Nk, H * B * m.rows.nob, &p.oc);
         const double own = (double)H * B * m.rows.nob * ((p.Nk + KT - 1) / KT), pre = (double)((p.P + KT - 1) / KT);
         const double fused_n = (double)H * B * m.rows.nob;
         double fused = (own + fused_n * pre) / (fused_n < 512 ? fused_n : 512);
