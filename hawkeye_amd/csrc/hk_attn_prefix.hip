@@ -955,7 +955,10 @@ Plan make_plan(PrefixParams& p, int hd, bool raw) {
 
 size_t up16(size_t x) { return (x + 15) / 16 * 16; }
 size_t part_bytes(const PrefixParams& p, int hd) {
-    return p.ns == 0 ? 16 : up16((size_t)p.ns * p.R * p.H * hd * 4) + up16((size_t)p.ns * p.R * p.H * 8);
+    return p.ns == 0 ? HK_NO_WS : up16((size_t)p.ns * p.R * p.H * hd * 4) + up16((size_t)p.ns * p.R * p.H * 8);
+}
+size_t step_bytes(const PrefixParams& p, int hd) {      // chunks, and every key's score (one launch keeps those in LDS)
+    return part_bytes(p, hd) + (p.ns == 0 ? 0 : (size_t)p.B * p.H * p.raw_ld * 4);
 }
 void set_parts(PrefixParams& p, void* ws, int hd) {
     p.part_o = reinterpret_cast<float*>(ws);
@@ -1091,12 +1094,12 @@ extern "C" int hk_prefix_attn_bf16(const hk_prefix_attn_desc* d, void* stream) {
     p.bso = d->bso;
     p.bias_bs = d->bias_bs;
     const Plan m = make_plan(p, d->head_dim, false);
-    HK_REQUIRE(d->ws && d->ws_bytes >= part_bytes(p, d->head_dim),
+    HK_REQUIRE(p.ns == 0 || (d->ws && d->ws_bytes >= part_bytes(p, d->head_dim)),
                "hk_prefix_attn_bf16: workspace of %zu bytes, %zu needed (hk_prefix_attn_ws)", d->ws ? d->ws_bytes : (size_t)0,
                part_bytes(p, d->head_dim));
     HK_REQUIRE(part_grid(p) < (1LL << 31) && rows_grid(p, m) < (1LL << 31), "hk_prefix_attn_bf16: grid too large");
     {
-        const HkSpan o = hk_span(p.O, p.B, p.bso, p.Nq, p.ldo, row, 2), w = hk_span(d->ws, 1, 0, 1, 0, (int64_t)part_bytes(p, d->head_dim), 1);
+        const HkSpan o = hk_span(p.O, p.B, p.bso, p.Nq, p.ldo, row, 2), w = hk_span(p.ns ? d->ws : nullptr, 1, 0, 1, 0, (int64_t)part_bytes(p, d->head_dim), 1);
         const HkSpan in[] = {hk_span(p.KP, 1, 0, p.P, p.ldkp, row, 2), hk_span(p.VP, 1, 0, p.P, p.ldvp, row, 2),
                              hk_span(p.K, p.B, p.bsk, p.Nk, p.ldk, row, 2), hk_span(p.V, p.B, p.bsv, p.Nk, p.ldv, row, 2),
                              hk_span(p.bias, p.B, p.bias_bs, 1, 0, p.Nk, 4), hk_span(p.Q, p.B, p.bsq, p.Nq, p.ldq, row, 2)};
@@ -1119,8 +1122,9 @@ extern "C" size_t hk_decode_attn_weights_ws(int32_t B, int32_t H, int32_t head_d
     p.H = H;
     p.Nq = 1;
     p.Nk = n_keys;
+    p.raw_ld = (n_keys + TK - 1) / TK * TK;
     make_plan(p, head_dim, true);
-    return part_bytes(p, head_dim) + (size_t)B * H * ((n_keys + TK - 1) / TK * TK) * 4;
+    return step_bytes(p, head_dim);
 }
 
 extern "C" int hk_decode_attn_weights_bf16(const hk_step_weights_desc* d, void* stream) {
@@ -1153,13 +1157,13 @@ extern "C" int hk_decode_attn_weights_bf16(const hk_step_weights_desc* d, void* 
     p.bias_hs = d->bias_hs;
     p.raw_ld = (d->n_keys + TK - 1) / TK * TK;
     const Plan m = make_plan(p, d->head_dim, true);
-    const size_t parts = part_bytes(p, d->head_dim), need = parts + (size_t)p.B * p.H * p.raw_ld * 4;
-    HK_REQUIRE(d->ws && d->ws_bytes >= need, "hk_decode_attn_weights_bf16: workspace of %zu bytes, %zu needed (hk_decode_attn_weights_ws)",
+    const size_t need = step_bytes(p, d->head_dim);
+    HK_REQUIRE(p.ns == 0 || (d->ws && d->ws_bytes >= need), "hk_decode_attn_weights_bf16: workspace of %zu bytes, %zu needed (hk_decode_attn_weights_ws)",
                d->ws ? d->ws_bytes : (size_t)0, need);
     HK_REQUIRE(part_grid(p) < (1LL << 31), "hk_decode_attn_weights_bf16: grid too large");
     {
         const HkSpan wo = hk_span(d->w_out, p.B, d->wo_bs, p.H, d->wo_hs, p.Nk, 4), o = hk_span(p.O, p.B, D, 1, 0, D, 2),
-                     w = hk_span(d->ws, 1, 0, 1, 0, (int64_t)need, 1);
+                     w = hk_span(p.ns ? d->ws : nullptr, 1, 0, 1, 0, (int64_t)need, 1);
         const HkSpan in[] = {hk_span(p.Q, p.B, D, 1, 0, D, 2), hk_span(p.K, p.B, p.bsk, p.Nk, D, D, 2), hk_span(p.V, p.B, p.bsv, p.Nk, D, D, 2),
                              hk_span(p.bias, p.B, p.bias_bs, p.H, p.bias_hs, p.Nk, 4),
                              d->w_in == d->w_out ? HkSpan{0, 0} : hk_span(d->w_in, p.B, d->wi_bs, p.H, d->wi_hs, p.Nk, 4)};
@@ -1169,7 +1173,7 @@ extern "C" int hk_decode_attn_weights_bf16(const hk_step_weights_desc* d, void* 
         HK_REQUIRE(!hk_overlap(o, wo) && !hk_overlap(o, w) && !hk_overlap(wo, w), "hk_decode_attn_weights_bf16: outputs and workspace overlap");
     }
     set_parts(p, d->ws, d->head_dim);
-    p.raw = reinterpret_cast<float*>(reinterpret_cast<char*>(d->ws) + parts);
+    p.raw = reinterpret_cast<float*>(reinterpret_cast<char*>(d->ws) + part_bytes(p, d->head_dim));
     StepWeights sw = {d->w_in, d->w_out, d->wi_bs, d->wi_hs, d->wo_bs, d->wo_hs};
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     if (d->head_dim == 128) launch_step<128>(p, m, sw, s);

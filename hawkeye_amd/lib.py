@@ -18,6 +18,7 @@ LIB_PATH = os.environ.get("HK_LIB_PATH") or os.path.join(_HERE, "libhawkeye_hip.
 
 HK_ACT_NONE, HK_ACT_GELU_ERF, HK_ACT_SWIGLU = 0, 1, 2
 HK_DT_BF16, HK_DT_F32 = 0, 1
+HK_NO_WS = 16          # hk_prefix_attn_ws of a call that uses no workspace
 
 
 class HkRows(C.Structure):

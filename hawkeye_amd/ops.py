@@ -494,11 +494,12 @@ def decode_attn_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, po
 # it: a decode loop repeats layouts, and the checks cost the host more than these launches cost the device.  Nothing is kept by a
 # tensor's address; addresses, alignment and overlaps are checked by the library, every time.
 _layouts = {}
+_NUMBERS = (int, bool, type(None))
 
 
 def _layout(check, *args):
     """check(*args), remembered by the layout of the tensors among args."""
-    key = (check, *[(a.shape, a.stride(), a.dtype, a.device) if isinstance(a, torch.Tensor) else a for a in args])
+    key = (check, *[a if a.__class__ in _NUMBERS else (a.shape, a.stride(), a.dtype, a.device) for a in args])
     got = _layouts.get(key)
     if got is None:
         got = check(*args)
@@ -594,11 +595,12 @@ def prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Te
         if out is None:
             out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
         if ws is None:
-            ws = torch.empty((need,), dtype=torch.uint8, device=q.device)
+            if need != L.HK_NO_WS:
+                ws = torch.empty((need,), dtype=torch.uint8, device=q.device)
         elif ws.dtype != torch.uint8 or ws.device != q.device or not ws.is_contiguous():
             raise RuntimeError("prefix_attention: ws must be a contiguous uint8 tensor on q's device")
         d = L.HkPrefixAttnDesc(q.data_ptr(), k_prefix.data_ptr(), v_prefix.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(key_bias),
-                               ws.data_ptr(), ws.numel(), *nums)
+                               _ptr(ws), 0 if ws is None else ws.numel(), *nums)
         L.check(L.load().hk_prefix_attn_bf16(C.byref(d), stream), "hk_prefix_attn_bf16")
     return out
 
@@ -646,9 +648,9 @@ def decode_attn_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     need, nums = _layout(_step_layout, q, k_cache, v_cache, n_keys, H, head_dim, weight, key_bias, weight_out)
     with _On(q.device) as stream:
         out = torch.empty_like(q)
-        ws = torch.empty((need,), dtype=torch.uint8, device=q.device)
+        ws = None if need == L.HK_NO_WS else torch.empty((need,), dtype=torch.uint8, device=q.device)
         d = L.HkStepWeightsDesc(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _ptr(key_bias), _ptr(weight), weight_out.data_ptr(),
-                                out.data_ptr(), ws.data_ptr(), need, *nums)
+                                out.data_ptr(), _ptr(ws), need, *nums)
         L.check(L.load().hk_decode_attn_weights_bf16(C.byref(d), stream), "hk_decode_attn_weights_bf16")
     return out
 

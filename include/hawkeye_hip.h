@@ -429,8 +429,11 @@ int hk_qformer_embed_bwd(const float* dz, const int64_t* input_ids, float* dquer
  *   bs* in elements, head h at column h * hd.  key_bias: optional fp32, own key j of sequence b adds key_bias[b * bias_bs + j] (natural-log
  *   units); a key whose bias is -1e4 or less (hk_qformer_key_bias's mask value, -inf) is removed: its K and V rows may hold anything.
  *   A row that sees no key gives zeros.
- * ws: hk_prefix_attn_ws bytes of the caller's, 16-byte aligned, for this call alone (calls in flight together need one each).
+ * ws: hk_prefix_attn_ws bytes of the caller's, 16-byte aligned, for this call alone (calls in flight together need one each); where that is
+ * HK_NO_WS, one launch does it all and ws may be NULL.  out may not overlap an input or ws; strides are multiples of 8 elements (4: O's),
+ * token strides of K and V below 2^25.
  * Bit-reproducible: chunks are joined in index order. */
+#define HK_NO_WS 16
 typedef struct hk_prefix_attn_desc {
     const void* Q;
     const void* KP;
@@ -451,7 +454,7 @@ size_t hk_prefix_attn_ws(int32_t B, int32_t H, int32_t Nq, int32_t P, int32_t Nk
  *   p_j = softmax_j(q . k_j + bias_j) over cache rows [0, n_keys),  out = sum_j p_j v_j,  w_out[b][h][j] = w_in[b][h][j] + p_j
  * for hk_cache_evict.  q bf16 [B, H*hd] pre-scaled, caches bf16 [B, cache_rows, H*hd], out bf16 [B, H*hd]; w_in (NULL: zeros) and w_out
  * fp32 with strides (wi_bs, wi_hs), (wo_bs, wo_hs), may be one array; key_bias[b * bias_bs + h * bias_hs + j] optional, as in
- * hk_prefix_attn_desc (bias_hs = 0: one row for all heads).  A sequence without a key gives zeros and adds nothing.  ws as above. */
+ * hk_prefix_attn_desc (bias_hs = 0: one row for all heads).  A sequence without a key gives zeros and adds nothing.  ws as above (hk_decode_attn_weights_ws). */
 typedef struct hk_step_weights_desc {
     const void* q;
     const void* k_cache;

@@ -15,7 +15,7 @@ def _refused(rc, text):
 
 
 def _prefix(**kw):
-    H, hd, B, Nq, P, Nk = (kw.get(k, d) for k, d in (("H", 2), ("head_dim", 64), ("B", 2), ("Nq", 1), ("P", 8), ("Nk", 4)))
+    H, hd, B, Nq, P, Nk = (kw.get(k, d) for k, d in (("H", 2), ("head_dim", 64), ("B", 2), ("Nq", 1), ("P", 1000), ("Nk", 4)))      # (keys in chunks: a call with a workspace)
     row = H * hd
     base = dict(Q=A, KP=2 * A, VP=3 * A, K=4 * A, V=5 * A, O=6 * A, key_bias=None, ws=8 * A, ws_bytes=1 << 30, B=B, H=H, Nq=Nq, P=P, Nk=Nk,
                 head_dim=hd, ldq=row, bsq=row * Nq, ldkp=row, ldvp=row, ldk=row, bsk=row * Nk, ldv=row, bsv=row * Nk, ldo=row, bso=row * Nq,
@@ -38,6 +38,7 @@ def test_workspace_queries_refuse_with_zero():
     lib = L.load()
     assert lib.hk_prefix_attn_ws(2, 2, 1, 8, 4, 64) > 0 and lib.hk_decode_attn_weights_ws(2, 2, 128, 5) > 0
     assert lib.hk_prefix_attn_ws(2, 2, 5, 8, 4, 64) == 0 and lib.hk_prefix_attn_ws(2, 2, 1, 8, 4, 80) == 0 and lib.hk_decode_attn_weights_ws(1, 1, 64, 0) == 0
+    assert lib.hk_prefix_attn_ws(2, 2, 1, 8, 4, 64) == lib.hk_decode_attn_weights_ws(2, 2, 128, 5) == L.HK_NO_WS < lib.hk_prefix_attn_ws(2, 2, 1, 1000, 4, 64)
     with pytest.raises(RuntimeError, match="not supported"):
         ops.prefix_attention_ws(2, 2, 1, 8, 0, 64)
 
@@ -49,10 +50,14 @@ def _step(**kw):
     return L.load().hk_decode_attn_weights_bf16(C.byref(L.HkStepWeightsDesc(**base)), None)
 
 
+LONG = dict(cache_rows=1040, wi_bs=2080, wi_hs=1040, wo_bs=2080, wo_hs=1040)      # too long for one launch, which takes no workspace
+
+
 @pytest.mark.parametrize("kw,text", [
     (dict(w_out=None), "null operand"), (dict(n_keys=17), "bad shape"), (dict(n_keys=0), "bad shape"), (dict(head_dim=32), "bad shape"), (dict(q=A + 2), "aligned"),
     (dict(wo_hs=8), "w_out must not overlap"), (dict(wo_bs=24), "w_out must not overlap"), (dict(wi_bs=-1), "negative"), (dict(w_out=4 * A, wo_bs=64), "one layout"),
-    (dict(ws_bytes=16), "workspace"), (dict(w_out=4 * A + 64), "overlaps an input"), (dict(out=2 * A), "overlaps an input"), (dict(ws=5 * A), "overlap")])
+    (dict(n_keys=1030, ws_bytes=1 << 10, **LONG), "workspace"), (dict(n_keys=1030, ws=None, **LONG), "workspace"), (dict(w_out=4 * A + 64), "overlaps an input"),
+    (dict(out=2 * A), "overlaps an input"), (dict(n_keys=1030, ws=5 * A, **LONG), "overlap")])
 def test_decode_attn_weights_refuses(kw, text):
     _refused(_step(**kw), text)
 
