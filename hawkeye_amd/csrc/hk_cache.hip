@@ -15,7 +15,8 @@ constexpr float REMOVED = -1.0e4f;   // a key whose bias is at or below this doe
 //   STATS: queries stay, keys pass: a reference point m and the sum of 2^(s - m) in the lane -> z.  m is the maximum of the row's first keys and
 //     moves only when a tile's partial sum leaves [0, 2^20] (that tile is redone): the common path is exp2 and an addition per score.
 //   SUMS:  keys stay, queries pass: 2^(s - z) added up in 16 registers per lane, over the 32 lanes at the end.
-// No sum crosses workgroups: every order is fixed.
+// GRP = 2: two such groups of four waves share a workgroup, each with stages of its own, and take every other tile; the second's sums
+// join the first's through LDS at the end.  No sum crosses workgroups: every order is fixed.
 struct KeyWeightParams {
     const __bf16 *Q, *K;
     const float* bias;
@@ -31,16 +32,19 @@ constexpr float OVERFLOW_SUM = 1048576.0f;
 constexpr int BLK = 128;             // rows of the operand that stays, per workgroup
 constexpr int TILE = 64;             // rows of the operand that passes, per stage
 
-template <int HD, bool SUMS, bool BIAS>
-__global__ __launch_bounds__(256, 2) void hk_key_weights_kernel(const KeyWeightParams p) {
+template <int HD, bool SUMS, bool BIAS, int GRP>
+__global__ __launch_bounds__(GRP * 256, 2) void hk_key_weights_kernel(const KeyWeightParams p) {
     constexpr int ROWB = HD * 2, CH = HD / 8, NKS = HD / 16;
     constexpr int STAGE = TILE * ROWB;
     constexpr int RPI = 64 / CH;                           // rows one wave-wide LDS-DMA covers
     constexpr int NI = TILE / (4 * RPI);                   // of them per wave and tile
     constexpr bool SIDE = SUMS || BIAS;                    // 64 floats come with a tile: its queries' z (SUMS), its keys' biases (STATS)
     constexpr int PER = NI + (SIDE ? 1 : 0);               // LDS-DMAs per wave and tile
-    extern __shared__ __attribute__((aligned(16))) char smem[];      // NST stages, then [NST][wave][TILE] floats (each wave its own copy)
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    extern __shared__ __attribute__((aligned(16))) char smem[];      // NST stages, then [NST][wave][TILE] floats (each wave its own copy); the same for the next group
+    constexpr int GROUP = NST * (STAGE + 4 * TILE * 4);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane((tid >> 6) & 3);
+    const int grp = GRP == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 8);
+    char* gs = smem + grp * GROUP;
     const int r = lane & 31, h = lane >> 5;
     const int nbh = p.B * p.H;
     // causal: the blocks with the most tiles first (keys at the front, queries at the back)
@@ -69,12 +73,19 @@ __global__ __launch_bounds__(256, 2) void hk_key_weights_kernel(const KeyWeightP
 
     // 16-byte chunk c of row x lives at chunk c ^ swz(x): 16 rows x one chunk touch every bank once
     auto swz = [](int x) { return HD == 128 ? x & 15 : (x >> 1) & 7; };
-    float* side = reinterpret_cast<float*>(smem + NST * STAGE) + wave * TILE;
+    float* side = reinterpret_cast<float*>(gs + NST * STAGE) + wave * TILE;
     const int lx = lane / CH, lc = (lane % CH) ^ swz(lx);  // this lane's row and (source) chunk of a piece of RPI rows from lr:
     // swz(lr + lx) == swz(lr) ^ swz(lx), as RPI is 4 (HD 128) or 8
     const uint32_t lane_off = (uint32_t)((lx * ldp) * 2);
-    auto issue = [&](int t) {
-        char* st = smem + (t & (NST - 1)) * STAGE;
+    int t0 = 0, t1 = (n_pass + TILE - 1) / TILE;
+    if (p.causal) {
+        if (SUMS) t0 = max(0, blk * BLK - off) / TILE;                                       // first query that sees the block's first key
+        else t1 = min(t1, (min(blk * BLK + BLK, p.Nq) - 1 + off) / TILE + 1);                // last key the block's last query sees
+    }
+    auto issue = [&](int u) {                              // the group's tile of step u
+        const int t = t0 + u * GRP + grp;
+        if (GRP > 1 && t >= t1) return;
+        char* st = gs + (u & (NST - 1)) * STAGE;
         if ((t + 1) * TILE <= n_pass) {                    // scalar base + 32-bit lane offset
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
@@ -88,15 +99,10 @@ __global__ __launch_bounds__(256, 2) void hk_key_weights_kernel(const KeyWeightP
                 glds16_v(pbase + (int64_t)min(t * TILE + lr + lx, n_pass - 1) * ldp + (lc ^ swz(lr)) * 8, st + lr * ROWB);
             }
         }
-        if (SIDE) glds4_s(SUMS ? z : bias, (uint32_t)min(t * TILE + lane, n_pass - 1) * 4u, side + (t & (NST - 1)) * 4 * TILE);
+        if (SIDE) glds4_s(SUMS ? z : bias, (uint32_t)min(t * TILE + lane, n_pass - 1) * 4u, side + (u & (NST - 1)) * 4 * TILE);
     };
     const int ro = r * ROWB + ((h ^ swz(r)) << 4);         // chunk 2 s + h: the 2 s joins by exclusive or
 
-    int t0 = 0, t1 = (n_pass + TILE - 1) / TILE;
-    if (p.causal) {
-        if (SUMS) t0 = max(0, blk * BLK - off) / TILE;                                       // first query that sees the block's first key
-        else t1 = min(t1, (min(blk * BLK + BLK, p.Nq) - 1 + off) / TILE + 1);                // last key the block's last query sees
-    }
     float kb[16];                                          // SUMS: the bias of this lane's keys, -inf for removed ones
     bool kplain = true, kall = false;                      // all of the wave's biases are 0, all of its keys are removed
     if (SUMS && BIAS) {
@@ -116,17 +122,19 @@ __global__ __launch_bounds__(256, 2) void hk_key_weights_kernel(const KeyWeightP
     float m = 0.f, l = 0.f;                                // STATS: everything is relative to m
     bool unset = true, pending = true;                     // STATS: this half row / some row of the wave has met no key yet
 
+    const int steps = (t1 - t0 + GRP - 1) / GRP;
 #pragma unroll
     for (int i = 0; i < NST - 1; ++i)
-        if (t0 + i < t1) issue(t0 + i);
-    for (int t = t0; t < t1; ++t) {
-        const int cur = t & (NST - 1);
+        if (i < steps) issue(i);
+    for (int u = 0; u < steps; ++u) {
+        const int cur = u & (NST - 1), t = t0 + u * GRP + grp;
         // this tile's LDS-DMA has arrived, those of the NST - 2 tiles behind it may be on their way (the compiler knows of none)
-        if (t + NST - 2 < t1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 2) * PER) : "memory");
+        if (GRP == 1 && u + NST - 2 < steps) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 2) * PER) : "memory");
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      // tile t stands; everyone has left tile t - 1
-        if (t + NST - 1 < t1) issue(t + NST - 1);
-        const char* ts = smem + cur * STAGE;
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      // tile t stands; everyone has left the tile before
+        if (u + NST - 1 < steps) issue(u + NST - 1);
+        if (GRP > 1 && t >= t1) continue;
+        const char* ts = gs + cur * STAGE;
         const float* sd = side + cur * 4 * TILE;
         // edges: rows of the passing operand that do not exist, keys behind the query's last
         const int p0 = t * TILE;
@@ -232,6 +240,15 @@ __global__ __launch_bounds__(256, 2) void hk_key_weights_kernel(const KeyWeightP
         halve(std::integral_constant<int, 2>{});
         halve(std::integral_constant<int, 1>{});
         acc[0] += __shfl_xor(acc[0], 16, 64);
+        if (GRP > 1) {
+            float* js = reinterpret_cast<float*>(smem) + wave * 64 + lane;
+            __syncthreads();                               // everyone has left the last tiles
+            if (grp) js[(grp - 1) * 256] = acc[0];
+            __syncthreads();
+            if (grp) return;
+#pragma unroll
+            for (int g = 0; g < GRP - 1; ++g) acc[0] += js[g * 256];
+        }
         const int key = s0 + (r & 3) + 8 * ((r & 15) >> 2) + 4 * h;
         if (r < 16 && key < p.Nk) {
             const int64_t at = (int64_t)b * p.wi_bs + (int64_t)head * p.wi_hs + key;
@@ -239,6 +256,22 @@ __global__ __launch_bounds__(256, 2) void hk_key_weights_kernel(const KeyWeightP
         }
     } else {
         if (unset) m = -1.0e30f;                           // this lane half met no key
+        if (GRP > 1) {
+            float* js = reinterpret_cast<float*>(smem) + (wave * 64 + lane) * 2;
+            __syncthreads();                               // everyone has left the last tiles
+            if (grp) {
+                js[(grp - 1) * 512] = m;
+                js[(grp - 1) * 512 + 1] = l;
+            }
+            __syncthreads();
+            if (grp) return;
+#pragma unroll
+            for (int g = 0; g < GRP - 1; ++g) {
+                const float mg = js[g * 512], lg = js[g * 512 + 1], M = fmaxf(m, mg);
+                l = l * __builtin_amdgcn_exp2f(m - M) + lg * __builtin_amdgcn_exp2f(mg - M);
+                m = M;
+            }
+        }
         const float mo = __shfl_xor(m, 32, 64), lo = __shfl_xor(l, 32, 64);
         const float M = fmaxf(m, mo);
         const float sum = l * __builtin_amdgcn_exp2f(m - M) + lo * __builtin_amdgcn_exp2f(mo - M);
@@ -246,18 +279,27 @@ __global__ __launch_bounds__(256, 2) void hk_key_weights_kernel(const KeyWeightP
     }
 }
 
-template <int HD, bool SUMS, bool BIAS>
-int launch_key_weights(KeyWeightParams p, hipStream_t s) {
-    constexpr int LDS = NST * (TILE * HD * 2 + 4 * TILE * 4);
+template <int HD, bool SUMS, bool BIAS, int GRP>
+int launch_groups(const KeyWeightParams& p, hipStream_t s) {
+    constexpr int LDS = GRP * NST * (TILE * HD * 2 + 4 * TILE * 4);
     static std::atomic<unsigned long long> attr_done{0};   // per device
-    const hipError_t e = hk_lds_attr_once(attr_done, reinterpret_cast<const void*>(&hk_key_weights_kernel<HD, SUMS, BIAS>), LDS);
+    const hipError_t e = hk_lds_attr_once(attr_done, reinterpret_cast<const void*>(&hk_key_weights_kernel<HD, SUMS, BIAS, GRP>), LDS);
     if (e != hipSuccess) {
         hk_set_error("hk_attn_key_weights_bf16: hipFuncSetAttribute(%d B LDS): %s", LDS, hipGetErrorString(e));
         return HK_ELAUNCH;
     }
-    p.nblk = ((SUMS ? p.Nk : p.Nq) + BLK - 1) / BLK;
-    hipLaunchKernelGGL((hk_key_weights_kernel<HD, SUMS, BIAS>), dim3((unsigned)((int64_t)p.nblk * p.B * p.H)), dim3(256), LDS, s, p);
+    hipLaunchKernelGGL((hk_key_weights_kernel<HD, SUMS, BIAS, GRP>), dim3((unsigned)((int64_t)p.nblk * p.B * p.H)), dim3(GRP * 256), LDS, s, p);
     return HK_OK;
+}
+template <int HD, bool SUMS, bool BIAS>
+int launch_key_weights(KeyWeightParams p, hipStream_t s) {
+    p.nblk = ((SUMS ? p.Nk : p.Nq) + BLK - 1) / BLK;
+    // A second group where it finds CUs idle and tiles enough.  One : two groups, both launches, heads of 128 (us at so many blocks): 65 rows (32
+    // blocks) 10.0 : 10.1, 128 (32) 10.2 : 11.0, 200 (64) 13.7 : 13.4, 352 (96) 17.0 : 15.7, 1000 (256) 34.4 : 28.0, 2047 (128) 59.9 : 45.1;
+    // 352 (384) 18.7 : 20.3, 500 (512) 23.7 : 25.7, 700 (384) 27.9 : 27.1, 1500 (384) 49.9 : 41.0, 2047 (512) 65.2 : 57.9; 700 (768) 33 : 43.
+    const int64_t blocks = (int64_t)p.nblk * p.B * p.H, n_pass = SUMS ? p.Nq : p.Nk;
+    const bool two = blocks <= 256 ? n_pass > 2 * TILE : blocks <= 512 && n_pass > 10 * TILE;
+    return two ? launch_groups<HD, SUMS, BIAS, 2>(p, s) : launch_groups<HD, SUMS, BIAS, 1>(p, s);
 }
 template <int HD>
 int launch_both(const KeyWeightParams& p, hipStream_t s) {
