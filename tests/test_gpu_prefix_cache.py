@@ -210,6 +210,13 @@ def test_attn_key_weights_matches_its_definition(B, Nq, Nk, H, hd, causal, kind)
         assert bool((got[-1] == 0).all())
 
 
+@pytest.mark.parametrize("B,Nq,Nk,H,hd,causal,kind", [      # more blocks than CUs: one group of waves per workgroup, and (last) two
+    (2, 130, 130, 66, 64, True, "left"), (1, 333, 333, 90, 128, True, None), (3, 700, 700, 30, 64, True, "holes"), (2, 200, 650, 130, 64, False, "add"),
+    (1, 700, 700, 45, 128, True, "add")])
+def test_attn_key_weights_of_many_blocks(B, Nq, Nk, H, hd, causal, kind):
+    test_attn_key_weights_matches_its_definition(B, Nq, Nk, H, hd, causal, kind)
+
+
 def _ref_evict(w, bias, n, budget, recent):
     """kept rows, by Python sorting"""
     B, H = w.shape[:2]
