@@ -62,10 +62,6 @@ __global__ __launch_bounds__(GRP * 256, 2) void hk_key_weights_kernel(const KeyW
 #pragma unroll
         for (int s = 0; s < NKS; ++s) sf[s] = *reinterpret_cast<const bf16x8*>(sp + 16 * s);
     }
-    // The loads above are waited for here: left pending, the compiler would wait for them inside the loop, with counts that take the
-    // LDS-DMA in flight there (which it does not know) along.
-#pragma unroll
-    for (int s = 0; s < NKS; ++s) asm volatile("" : "+v"(sf[s]));
     const __bf16* pbase = (SUMS ? p.Q + (int64_t)b * p.bsq : p.K + (int64_t)b * p.bsk) + head * HD;
     const int64_t ldp = SUMS ? p.ldq : p.ldk;
     const float* bias = BIAS ? p.bias + (int64_t)b * p.bias_bs : nullptr;
@@ -101,6 +97,14 @@ __global__ __launch_bounds__(GRP * 256, 2) void hk_key_weights_kernel(const KeyW
         }
         if (SIDE) glds4_s(SUMS ? z : bias, (uint32_t)min(t * TILE + lane, n_pass - 1) * 4u, side + (u & (NST - 1)) * 4 * TILE);
     };
+    const int steps = (t1 - t0 + GRP - 1) / GRP;
+#pragma unroll
+    for (int i = 0; i < NST - 1; ++i)
+        if (i < steps) issue(i);
+    // The loads above are waited for here: left pending, the compiler would wait for them inside the loop, with counts that take the
+    // LDS-DMA in flight there (which it does not know) along.
+#pragma unroll
+    for (int s = 0; s < NKS; ++s) asm volatile("" : "+v"(sf[s]));
     const int ro = r * ROWB + ((h ^ swz(r)) << 4);         // chunk 2 s + h: the 2 s joins by exclusive or
 
     float kb[16];                                          // SUMS: the bias of this lane's keys, -inf for removed ones
@@ -122,10 +126,6 @@ __global__ __launch_bounds__(GRP * 256, 2) void hk_key_weights_kernel(const KeyW
     float m = 0.f, l = 0.f;                                // STATS: everything is relative to m
     bool unset = true, pending = true;                     // STATS: this half row / some row of the wave has met no key yet
 
-    const int steps = (t1 - t0 + GRP - 1) / GRP;
-#pragma unroll
-    for (int i = 0; i < NST - 1; ++i)
-        if (i < steps) issue(i);
     for (int u = 0; u < steps; ++u) {
         const int cur = u & (NST - 1), t = t0 + u * GRP + grp;
         // this tile's LDS-DMA has arrived, those of the NST - 2 tiles behind it may be on their way (the compiler knows of none)
