@@ -15,7 +15,10 @@
 //   4 q + j of block 0, j < 4, or 4 q + j - 4 of block 1), and V^T comes in that key order from ds_read_b64_tr_b16.
 // K goes from memory straight to the A operand's registers, V through 32 keys of LDS that belong to the wave (no barrier in
 // the loop).  The next tile's K is requested as soon as this one's scores stand, its V as soon as this one's is in LDS: a
-// wave keeps about 16 KB in flight, 8 waves per CU.
+// wave keeps about 16 KB in flight, 8 waves per CU.  Bound by memory: 16 sequences' step over 1500 own keys each (398 MB) 80 us, 5.0 TB/s;
+// 64 sequences' over 512 own keys each beside the prefix 66 us.
+// ONE: a workgroup of eight waves per (sequence, head) for all its keys, the prefix's tiles first; no chunks, no second launch, a step's scores
+// stay in LDS.  Bound by latency (a chain of dependent tiles per wave): one sequence over 353 keys 8 us, and the host needs 10 for the call.
 #include <type_traits>
 #include "hk_common.h"
 
@@ -365,6 +368,13 @@ __global__ __launch_bounds__(NW * 64, 2) void hk_prefix_part_kernel(const Prefix
 // maximum of every tile until it does.
 // Rows are a sequence's (its keys: the prefix, then its own up to the diagonal; or its own alone) or, for the prefix alone, rows of
 // all sequences packed: whichever leaves fewer 128-row blocks part empty (make_plan).
+// A tile with nothing to mask goes by halves, the second half's products among the first half's exponentials.
+// Measured (32 heads of 128): 8 sequences of 512 rows over 1400 shared keys and their own 120 us, 930 TFLOP/s; the matrix unit is busy half of
+// the time.  Copies of the loop without one part, in-bounds and for timing only: without LDS-DMA and barriers 107-116 us, without the reads of
+// K from LDS 84, without those of V too 79, without exp2 101: bound by feeding the matrix unit from LDS (each wave reads every tile), at the clock that the
+// card holds under it.  Slower: 32-key tiles at 3-4 waves per SIMD (10-40 %), LDS-DMA spread over the matrix steps (141), K read before
+// the LDS-DMA is issued (130), four stages instead of two (10-40 % where a CU holds two workgroups, the same elsewhere).  64 sequences' single rows over 16384 shared keys
+// (268 MB, one workgroup per CU): 54-59 us, 4.5-5.0 TB/s.
 struct RowsParams {
     int packed;                      // prefix by packed row blocks and key chunks, own keys apart; else both in one workgroup
     int npb, nob;                    // row blocks: of all rows (packed prefix), of a sequence

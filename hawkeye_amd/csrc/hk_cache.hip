@@ -17,6 +17,11 @@ constexpr float REMOVED = -1.0e4f;   // a key whose bias is at or below this doe
 //   SUMS:  keys stay, queries pass: 2^(s - z) added up in 16 registers per lane, over the 32 lanes at the end.
 // GRP = 2: two such groups of four waves share a workgroup, each with stages of its own, and take every other tile; the second's sums
 // join the first's through LDS at the end.  No sum crosses workgroups: every order is fixed.
+// Measured: 2 x 2047 tokens, 32 heads of 128, padded 77-89 us for both launches (clock), 770-890 TFLOP/s of the products they make (each makes them
+// all).  The matrix unit is busy 21 % of the time, the vector unit 38 %, 1.8 waves per SIMD on average: bound by the chain of a tile within a wave
+// (LDS, 16 matrix instructions, 32 exp2: about 2000 cycles) and the uneven lengths of causal blocks.  No gain: 128-row tiles, their products
+// spread among the exponentials, fragments read 2-8 steps ahead, starting values kept in registers, long and short blocks paired on a CU by
+// their order (each within 3 %); slower: 64 rows per wave, two waves per workgroup (twice the time), 4 and 8 stages.
 struct KeyWeightParams {
     const __bf16 *Q, *K;
     const float* bias;
@@ -364,7 +369,7 @@ __device__ __forceinline__ void move_rows(const EvictParams& p, int b, int head,
 // bit: count the ranks at or above the candidate (a comparison, a ballot and a bit count per slot; the waves add up through LDS), keep the
 // bit if there are enough; done as soon as there are exactly enough.  An ordered pass then keeps the ranks above the threshold and, of those
 // equal to it, the first ones: positions from a scan over the (slot, wave) counts.  Weights and biases move through registers (in place is
-// safe), and MOVE != 0 moves K and V in the same launch.
+// safe), and MOVE moves K and V in the same launch.  Bound by latency without it (512 pairs of 2047 keys 10-15 us), by the moved rows with it.
 template <int T, int KPT, int HD, bool MOVE>
 __global__ __launch_bounds__(T) void hk_evict_kernel(const EvictParams p) {
     constexpr int NW = T / 64, NC = KPT * NW;              // (slot, wave) pairs
@@ -473,7 +478,9 @@ __global__ __launch_bounds__(T) void hk_evict_kernel(const EvictParams p) {
 
 // More keys than registers hold: the budget-th largest rank by four rounds of an 8-bit histogram over the weights in memory, then the ordered
 // pass chunk by chunk (a chunk's values are in registers before any of its stores, and go to places at or below the ones they came from).
+// Bound by the passes' waits for memory: 40000 keys 77 us (one rank in flight per thread and 1024 keys per ordered step: 118).
 __global__ __launch_bounds__(SEL_T) void hk_evict_select_kernel(const EvictParams p) {
+    constexpr int U = 8;                                   // ranks in flight per thread: one at a time, the passes wait for memory
     __shared__ uint32_t hist[256];
     __shared__ uint32_t pick[2];
     __shared__ uint32_t wsum[SEL_T / 64];
@@ -489,9 +496,23 @@ __global__ __launch_bounds__(SEL_T) void hk_evict_select_kernel(const EvictParam
     for (int shift = 24; shift >= 0; shift -= 8) {
         if (tid < 256) hist[tid] = 0;
         __syncthreads();
-        for (int j = tid; j < p.n; j += SEL_T) {
-            const uint32_t k = rank_at(j);
-            if (shift == 24 || (k >> (shift + 8)) == prefix) atomicAdd(&hist[(k >> shift) & 255u], 1u);
+        for (int j0 = tid; j0 < p.n; j0 += SEL_T * U) {
+            uint32_t k[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) k[u] = rank_at(min(j0 + u * SEL_T, p.n - 1));
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const bool in = j0 + u * SEL_T < p.n && (shift == 24 || (k[u] >> (shift + 8)) == prefix);
+                const uint32_t bin = (k[u] >> shift) & 255u;
+                // a wave's ranks often begin alike: the first lane's bin is counted once for all lanes that share it
+                const uint64_t any = __builtin_amdgcn_ballot_w64(in);
+                if (any == 0) continue;
+                const int lead = __ffsll((unsigned long long)any) - 1;
+                const uint32_t b0 = __builtin_amdgcn_readlane(bin, lead);
+                const uint64_t same = __builtin_amdgcn_ballot_w64(in && bin == b0);
+                if (lane == lead) atomicAdd(&hist[b0], (uint32_t)__popcll(same));
+                else if (in && bin != b0) atomicAdd(&hist[bin], 1u);
+            }
         }
         __syncthreads();
         if (wave == 0) {                                   // lane L: bins 255 - 4 L downwards
@@ -523,33 +544,53 @@ __global__ __launch_bounds__(SEL_T) void hk_evict_select_kernel(const EvictParam
     }
     // ---- ordered pass: rank > prefix, and the first `want` of those equal to it ----
     uint32_t above = 0, equal = 0;                         // met so far
-    for (int j0 = 0; j0 < p.n; j0 += SEL_T) {
-        const int j = j0 + tid;
-        const bool in = j < p.n;
-        const uint32_t k = in ? rank_at(j) : 0u;
-        const float wv = in ? w[j] : 0.f, bv = in && bias ? bias[j] : 0.f;
-        const uint64_t ga = __builtin_amdgcn_ballot_w64(in && k > prefix), ge = __builtin_amdgcn_ballot_w64(in && k == prefix);
-        const uint64_t lower = (1ull << lane) - 1;
-        if (lane == 0) wsum[wave] = (uint32_t)__popcll(ga) | (uint32_t)__popcll(ge) << 16;
+    constexpr int W = 4;                                   // consecutive keys per thread and step
+    for (int j0 = 0; j0 < p.n; j0 += SEL_T * W) {
+        uint32_t k[W], c = 0;
+        float wv[W], bv[W];
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            const int j = min(j0 + tid * W + i, p.n - 1);
+            wv[i] = w[j];
+            bv[i] = bias ? bias[j] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            const int j = j0 + tid * W + i;
+            k[i] = rank_of(wv[i], bias && bv[i] <= REMOVED, j >= p.n - p.recent);
+            if (j < p.n) c += (k[i] > prefix ? 1u : 0u) + (k[i] == prefix ? 1u << 16 : 0u);
+        }
+        uint32_t x = c;                                    // above | equal << 16, of the lanes up to this one
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t y = __shfl_up(x, o, 64);
+            if (lane >= o) x += y;
+        }
+        if (lane == 63) wsum[wave] = x;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // wv, bv are in registers before anyone stores
         __syncthreads();
-        uint32_t ba = above, be = equal;
-        for (int x = 0; x < SEL_T / 64; ++x) {
-            const uint32_t s = wsum[x];
-            if (x < wave) {
+        uint32_t ba = above + ((x - c) & 0xffffu), be = equal + ((x - c) >> 16);
+        for (int v = 0; v < SEL_T / 64; ++v) {
+            const uint32_t s = wsum[v];
+            if (v < wave) {
                 ba += s & 0xffffu;
                 be += s >> 16;
             }
             above += s & 0xffffu;
             equal += s >> 16;
         }
-        ba += (uint32_t)__popcll(ga & lower);
-        be += (uint32_t)__popcll(ge & lower);
-        if (in && (k > prefix || (k == prefix && be < want))) {
-            const uint32_t at = ba + min(be, want);
-            kept[at] = j;
-            wo[at] = wv;
-            if (bo) bo[at] = bv;
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            const int j = j0 + tid * W + i;
+            const bool gt = j < p.n && k[i] > prefix, eq = j < p.n && k[i] == prefix;
+            if (gt || (eq && be < want)) {
+                const uint32_t at = ba + min(be, want);
+                kept[at] = j;
+                wo[at] = wv[i];
+                if (bo) bo[at] = bv[i];
+            }
+            ba += gt;
+            be += eq;
         }
         __syncthreads();
     }
@@ -561,7 +602,7 @@ __global__ __launch_bounds__(SEL_T) void hk_evict_select_kernel(const EvictParam
 }
 
 // Rows into another cache: 16 bytes of K and of V per thread and step, neighbouring heads of one destination row next to each other, so
-// that whole destination rows are written; the source rows are HD * 2 byte pieces.
+// that whole destination rows are written; the source rows are HD * 2 byte pieces.  16384 rows of 8 KB, K and V: 99 us, 5.4 TB/s read and written.
 template <int HD>
 __global__ __launch_bounds__(256) void hk_evict_copy_kernel(const EvictParams p) {
     constexpr int CH = HD / 8, U = 2;
@@ -614,9 +655,13 @@ template <int HD>
 int launch_evict_all(const EvictParams& p, hipStream_t s) {
     const unsigned pairs = (unsigned)(p.B * p.H);
     // One launch or two?  A workgroup per pair moves its rows in pieces of one head; the copy kernel writes whole rows with the whole chip
-    // (5.5 TB/s against 4.6) and costs a launch.  128 pairs (353 keys to 256): 12 us against 13.7 and the gap; 512 pairs (2047 to 1024): 119
-    // against 114.5.  In place only the pair's own workgroup knows when a row may be overwritten.
-    if (p.n <= REG_KEYS && (p.in_place || pairs <= 256)) return launch_evict_any<HD, true>(p, s);
+    // (5.5 TB/s against 4.6) and costs a launch (2.6 us of the host's).  One : two, heads of 128 (us).  Budget 256 of 353: 9.5 : 9.2 (32 pairs),
+    // 11.3 : 12.1 (128), 24.5 : 28.5 (512); 500 of 1000: 15.7 : 11.7, 20.0 : 20.0, 51.3 : 52.7; 1024 of 2047: 26 : 15, 31 : 31, 118 : 113; 8000 of
+    // 16000: 200 : 66, 312 : 217.  Heads of 64, 1024 of 2047: 17 : 13 (32 pairs), 28 : 32 (256), 60 : 59 (512).  In place only the pair's own
+    // workgroup knows when a row may be overwritten.
+    const int64_t bytes = (int64_t)p.budget * HD * 2;
+    const bool one = bytes <= (pairs < 128 ? 64 << 10 : 128 << 10);
+    if (p.n <= REG_KEYS && (p.in_place || one)) return launch_evict_any<HD, true>(p, s);
     if (p.n <= REG_KEYS) launch_evict_any<HD, false>(p, s);
     else hipLaunchKernelGGL(hk_evict_select_kernel, dim3(pairs), dim3(SEL_T), 0, s, p);
     if (p.in_place) {
