@@ -9,14 +9,14 @@ constexpr float REMOVED = -1.0e4f;   // a key whose bias is at or below this doe
 
 // ---------------------------------------------------------------- key weights of a prompt
 // w_j = sum_i 2^(s_ij - z_i),  s_ij = q_i . k_j + b_j log2 e,  z_i = log2 sum_j 2^(s_ij).
-// Two launches of one structure: a wave keeps 32 rows of one operand in registers and walks 64-row tiles of the other, which the
+// Two launches of one structure (and a small one between them where few queries take their keys in chunks): a wave keeps 32 rows of one operand in registers and walks 64-row tiles of the other, which the
 // four waves of a workgroup share in LDS (two stages, LDS-DMA one tile ahead).  Both compute S^T = K . Q^T with
 // v_mfma_f32_32x32x16_bf16: lane -> query lane & 31, register i -> key (i & 3) + 8 (i >> 2) + 4 (lane >> 5).
 //   STATS: queries stay, keys pass: a reference point m and the sum of 2^(s - m) in the lane -> z.  m is the maximum of the row's first keys and
 //     moves only when a tile's partial sum leaves [0, 2^20] (that tile is redone): the common path is exp2 and an addition per score.
 //   SUMS:  keys stay, queries pass: 2^(s - z) added up in 16 registers per lane, over the 32 lanes at the end.
 // GRP = 2: two such groups of four waves share a workgroup, each with stages of its own, and take every other tile; the second's sums
-// join the first's through LDS at the end.  No sum crosses workgroups: every order is fixed.
+// join the first's through LDS at the end.  Chunks of keys (key_chunks) leave (m, sum) for a small launch that joins them: every order is fixed.
 // Measured: 2 x 2047 tokens, 32 heads of 128, padded 77-89 us for both launches (clock), 770-890 TFLOP/s of the products they make (each makes them
 // all).  The matrix unit is busy 21 % of the time, the vector unit 38 %, 1.8 waves per SIMD on average: bound by the chain of a tile within a wave
 // (LDS, 16 matrix instructions, 32 exp2: about 2000 cycles) and the uneven lengths of causal blocks.  No gain: 128-row tiles, their products
@@ -26,6 +26,8 @@ struct KeyWeightParams {
     const __bf16 *Q, *K;
     const float* bias;
     float* z;                        // [B][H][Nq]; +inf for a query that sees no key
+    float2* part;                    // STATS by chunks of keys: [chunk][B][H][Nq] of (reference point, sum)
+    int nch, ct;                     // chunks, tiles per chunk
     const float* w_in;
     float* w_out;
     int B, H, Nq, Nk, causal, nblk;
@@ -53,7 +55,10 @@ __global__ __launch_bounds__(GRP * 256, 2) void hk_key_weights_kernel(const KeyW
     const int r = lane & 31, h = lane >> 5;
     const int nbh = p.B * p.H;
     // causal: the blocks with the most tiles first (keys at the front, queries at the back)
-    const int rank = blockIdx.x / nbh, bh = blockIdx.x - rank * nbh;
+    int rank = blockIdx.x / nbh;
+    const int bh = blockIdx.x - rank * nbh;
+    const int c = SUMS ? 0 : rank % p.nch;
+    if (!SUMS) rank /= p.nch;
     const int blk = (!SUMS && p.causal) ? p.nblk - 1 - rank : rank;
     const int b = bh / p.H, head = bh - b * p.H;
     const int off = p.Nk - p.Nq;                           // causal: key <= query + off
@@ -82,6 +87,10 @@ __global__ __launch_bounds__(GRP * 256, 2) void hk_key_weights_kernel(const KeyW
     if (p.causal) {
         if (SUMS) t0 = max(0, blk * BLK - off) / TILE;                                       // first query that sees the block's first key
         else t1 = min(t1, (min(blk * BLK + BLK, p.Nq) - 1 + off) / TILE + 1);                // last key the block's last query sees
+    }
+    if (!SUMS && p.nch > 1) {
+        t0 = c * p.ct;
+        t1 = max(t0, min(t1, t0 + p.ct));
     }
     auto issue = [&](int u) {                              // the group's tile of step u
         const int t = t0 + u * GRP + grp;
@@ -280,8 +289,42 @@ __global__ __launch_bounds__(GRP * 256, 2) void hk_key_weights_kernel(const KeyW
         const float mo = __shfl_xor(m, 32, 64), lo = __shfl_xor(l, 32, 64);
         const float M = fmaxf(m, mo);
         const float sum = l * __builtin_amdgcn_exp2f(m - M) + lo * __builtin_amdgcn_exp2f(mo - M);
-        if (h == 0 && s0 + r < p.Nq) z[s0 + r] = sum == 0.f ? INFINITY : M + __log2f(sum);
+        if (h == 0 && s0 + r < p.Nq) {
+            if (p.nch > 1) p.part[((int64_t)c * nbh + bh) * p.Nq + s0 + r] = make_float2(M, sum);
+            else z[s0 + r] = sum == 0.f ? INFINITY : M + __log2f(sum);
+        }
     }
+}
+
+// z of the queries whose keys went by chunks, in chunk order.
+__global__ __launch_bounds__(256) void hk_key_weights_join_kernel(const KeyWeightParams p) {
+    const int64_t n = (int64_t)p.B * p.H * p.Nq, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    float M = -1.0e30f, sum = 0.f;
+#pragma unroll 4
+    for (int c = 0; c < p.nch; ++c) {
+        const float2 x = p.part[c * n + i];
+        const float N = fmaxf(M, x.x);
+        sum = sum * __builtin_amdgcn_exp2f(M - N) + x.y * __builtin_amdgcn_exp2f(x.x - N);
+        M = N;
+    }
+    p.z[i] = sum == 0.f ? INFINITY : M + __log2f(sum);
+}
+
+// STATS of few queries over many keys: chunks of the keys, a workgroup per CU, four tiles at least.  The last 32 / 512 of so many tokens,
+// 32 heads of 128, without : with chunks (us, all launches): 1000 17.0 : 13.0, 23.8 : 21.7; 2047 27.5 : 15.2, 37.9 : 31.0; 16000 170 : 52, 219 : 164;
+// 4 sequences of 16000 285 : 231 (K is read twice: 216), 665 : 670.  Twice as many chunks: 16000 tokens 57 and 169; eight tiles at least: 1000 tokens 14.8.
+int key_chunks(int64_t blocks, int Nk, int* ct) {
+    const int tiles = (Nk + TILE - 1) / TILE;
+    int64_t n = 256 / blocks < tiles / 4 ? 256 / blocks : tiles / 4;
+    if (n < 1) n = 1;
+    *ct = (int)((tiles + n - 1) / n);
+    return (tiles + *ct - 1) / *ct;
+}
+size_t key_weights_bytes(int64_t B, int64_t H, int64_t Nq, int Nk) {
+    int ct;
+    const int nch = key_chunks((Nq + BLK - 1) / BLK * B * H, Nk, &ct);
+    return (size_t)(B * H * Nq) * (nch > 1 ? 8 * nch + 4 : 4);
 }
 
 template <int HD, bool SUMS, bool BIAS, int GRP>
@@ -293,7 +336,8 @@ int launch_groups(const KeyWeightParams& p, hipStream_t s) {
         hk_set_error("hk_attn_key_weights_bf16: hipFuncSetAttribute(%d B LDS): %s", LDS, hipGetErrorString(e));
         return HK_ELAUNCH;
     }
-    hipLaunchKernelGGL((hk_key_weights_kernel<HD, SUMS, BIAS, GRP>), dim3((unsigned)((int64_t)p.nblk * p.B * p.H)), dim3(GRP * 256), LDS, s, p);
+    hipLaunchKernelGGL((hk_key_weights_kernel<HD, SUMS, BIAS, GRP>), dim3((unsigned)((int64_t)p.nblk * p.B * p.H * (SUMS ? 1 : p.nch))),
+                       dim3(GRP * 256), LDS, s, p);
     return HK_OK;
 }
 template <int HD, bool SUMS, bool BIAS>
@@ -302,7 +346,7 @@ int launch_key_weights(KeyWeightParams p, hipStream_t s) {
     // A second group where it finds CUs idle and tiles enough.  One : two groups, both launches, heads of 128 (us at so many blocks): 65 rows (32
     // blocks) 10.0 : 10.1, 128 (32) 10.2 : 11.0, 200 (64) 13.7 : 13.4, 352 (96) 17.0 : 15.7, 1000 (256) 34.4 : 28.0, 2047 (128) 59.9 : 45.1;
     // 352 (384) 18.7 : 20.3, 500 (512) 23.7 : 25.7, 700 (384) 27.9 : 27.1, 1500 (384) 49.9 : 41.0, 2047 (512) 65.2 : 57.9; 700 (768) 33 : 43.
-    const int64_t blocks = (int64_t)p.nblk * p.B * p.H, n_pass = SUMS ? p.Nq : p.Nk;
+    const int64_t blocks = (int64_t)p.nblk * p.B * p.H * (SUMS ? 1 : p.nch), n_pass = SUMS ? p.Nq : p.nch > 1 ? p.ct * TILE : p.Nk;
     const bool two = blocks <= 256 ? n_pass > 2 * TILE : blocks <= 512 && n_pass > 10 * TILE;
     return two ? launch_groups<HD, SUMS, BIAS, 2>(p, s) : launch_groups<HD, SUMS, BIAS, 1>(p, s);
 }
@@ -310,6 +354,7 @@ template <int HD>
 int launch_both(const KeyWeightParams& p, hipStream_t s) {
     const int rc = p.bias ? launch_key_weights<HD, false, true>(p, s) : launch_key_weights<HD, false, false>(p, s);
     if (rc != HK_OK) return rc;
+    if (p.nch > 1) hipLaunchKernelGGL(hk_key_weights_join_kernel, dim3((unsigned)(((int64_t)p.B * p.H * p.Nq + 255) / 256)), dim3(256), 0, s, p);
     return p.bias ? launch_key_weights<HD, true, true>(p, s) : launch_key_weights<HD, true, false>(p, s);
 }
 
@@ -676,6 +721,11 @@ int launch_evict_all(const EvictParams& p, hipStream_t s) {
 
 }  // namespace
 
+extern "C" size_t hk_attn_key_weights_ws(int32_t B, int32_t H, int32_t Nq, int32_t Nk) {
+    if (B < 1 || B >= 65536 || H < 1 || H >= 65536 || Nq < 1 || Nk < 1 || Nq >= (1 << 26) || Nk >= (1 << 26)) return 0;
+    return key_weights_bytes(B, H, Nq, Nk);
+}
+
 extern "C" int hk_attn_key_weights_bf16(const hk_key_weights_desc* d, void* stream) {
     HK_REQUIRE(d && d->Q && d->K && d->w_out, "hk_attn_key_weights_bf16: null operand");
     HK_REQUIRE(d->B >= 1 && d->B < 65536 && d->H >= 1 && d->H < 65536 && d->Nq >= 1 && d->Nk >= 1 && d->Nq < (1 << 26) && d->Nk < (1 << 26) &&
@@ -685,16 +735,16 @@ extern "C" int hk_attn_key_weights_bf16(const hk_key_weights_desc* d, void* stre
     HK_REQUIRE(((d->ldq | d->bsq | d->ldk | d->bsk) & 7) == 0 && d->ldq >= 0 && d->bsq >= 0 && d->ldk >= 0 && d->bsk >= 0,
                "hk_attn_key_weights_bf16: strides must be multiples of 8 elements, not negative");
     HK_REQUIRE(d->ldq < (1 << 25) && d->ldk < (1 << 25), "hk_attn_key_weights_bf16: token strides of 2^25 elements and more are not supported");
-    HK_REQUIRE(((uintptr_t)d->Q | (uintptr_t)d->K) % 16 == 0 &&
-                   ((uintptr_t)d->key_bias | (uintptr_t)d->w_in | (uintptr_t)d->w_out | (uintptr_t)d->ws) % 4 == 0,
+    HK_REQUIRE(((uintptr_t)d->Q | (uintptr_t)d->K | (uintptr_t)d->ws) % 16 == 0 &&
+                   ((uintptr_t)d->key_bias | (uintptr_t)d->w_in | (uintptr_t)d->w_out) % 4 == 0,
                "hk_attn_key_weights_bf16: operands must be 16-byte aligned");
     HK_REQUIRE((d->H == 1 || d->wo_hs >= d->Nk) && (d->B == 1 || d->wo_bs >= (d->H - 1) * d->wo_hs + d->Nk) && d->wi_bs >= 0 && d->wi_hs >= 0 &&
                    d->bias_bs >= 0,
                "hk_attn_key_weights_bf16: rows of w_out must not overlap, strides must not be negative");
     HK_REQUIRE(d->w_in != d->w_out || (d->wi_bs == d->wo_bs && d->wi_hs == d->wo_hs),
                "hk_attn_key_weights_bf16: weights updated in place must have one layout");
-    const size_t need = (size_t)d->B * d->H * d->Nq * 4;
-    HK_REQUIRE(d->ws && d->ws_bytes >= need, "hk_attn_key_weights_bf16: workspace of %zu bytes, B * H * Nq floats = %zu needed",
+    const size_t need = key_weights_bytes(d->B, d->H, d->Nq, d->Nk);
+    HK_REQUIRE(d->ws && d->ws_bytes >= need, "hk_attn_key_weights_bf16: workspace of %zu bytes, %zu needed (hk_attn_key_weights_ws)",
                d->ws ? d->ws_bytes : (size_t)0, need);
     {
         const int64_t row = (int64_t)d->H * d->head_dim;
@@ -706,13 +756,15 @@ extern "C" int hk_attn_key_weights_bf16(const hk_key_weights_desc* d, void* stre
             HK_REQUIRE(!hk_overlap(wo, in[i]) && !hk_overlap(w, in[i]), "hk_attn_key_weights_bf16: the output or the workspace overlaps an input");
         HK_REQUIRE(!hk_overlap(wo, w), "hk_attn_key_weights_bf16: the output overlaps the workspace");
     }
-    const int64_t most = ((d->Nq > d->Nk ? d->Nq : d->Nk) + BLK - 1) / BLK;
-    HK_REQUIRE(most * d->B * d->H < (1LL << 31), "hk_attn_key_weights_bf16: grid too large");
+    const int64_t most = ((d->Nq > d->Nk ? d->Nq : d->Nk) + BLK - 1) / BLK;      // (chunks only where that leaves few workgroups)
+    HK_REQUIRE(most * d->B * d->H < (1LL << 31) && (int64_t)d->B * d->H * d->Nq < (1LL << 38), "hk_attn_key_weights_bf16: grid too large");
     KeyWeightParams p = {};
     p.Q = reinterpret_cast<const __bf16*>(d->Q);
     p.K = reinterpret_cast<const __bf16*>(d->K);
     p.bias = d->key_bias;
-    p.z = reinterpret_cast<float*>(d->ws);
+    p.nch = key_chunks(((int64_t)d->Nq + BLK - 1) / BLK * d->B * d->H, d->Nk, &p.ct);
+    p.part = reinterpret_cast<float2*>(d->ws);             // z behind it (8-byte aligned)
+    p.z = reinterpret_cast<float*>(d->ws) + (p.nch > 1 ? (int64_t)2 * p.nch * d->B * d->H * d->Nq : 0);
     p.w_in = d->w_in;
     p.w_out = d->w_out;
     p.B = d->B;

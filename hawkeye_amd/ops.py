@@ -670,7 +670,10 @@ def _key_weights_layout(q, k, key_bias, causal, weight, weight_out):
     bias_bs, _ = _per_key(key_bias, "key_bias", B, 1, Nk, False)
     wi = _per_key(weight, "weight", B, H, Nk, True)
     wo = (H * Nk, Nk) if weight_out is None else _per_key(weight_out, "weight_out", B, H, Nk, True)
-    return B * H * Nq * 4, (B, H, Nq, Nk, hd, 1 if causal else 0, ldq, bsq, ldk, bsk, bias_bs, *wi, *wo)
+    need = L.load().hk_attn_key_weights_ws(B, H, Nq, Nk)
+    if need == 0:
+        raise RuntimeError(f"attn_key_weights: shape B={B} H={H} Nq={Nq} Nk={Nk} is not supported")
+    return need, (B, H, Nq, Nk, hd, 1 if causal else 0, ldq, bsq, ldk, bsk, bias_bs, *wi, *wo)
 
 
 def attn_key_weights(q: torch.Tensor, k: torch.Tensor, key_bias: Optional[torch.Tensor] = None, causal: bool = True,

@@ -210,6 +210,13 @@ def test_attn_key_weights_matches_its_definition(B, Nq, Nk, H, hd, causal, kind)
         assert bool((got[-1] == 0).all())
 
 
+@pytest.mark.parametrize("B,Nq,Nk,H,hd,causal,kind", [      # few queries, many keys: row sums by chunks of keys
+    (1, 3, 16411, 1, 64, True, "left"), (2, 130, 4100, 2, 128, True, "holes"), (3, 40, 2000, 1, 128, False, "all"), (1, 700, 700, 1, 128, True, None),
+    (2, 1, 513, 3, 64, True, "add"), (1, 129, 1025, 40, 128, True, "left")])
+def test_attn_key_weights_of_few_queries(B, Nq, Nk, H, hd, causal, kind):
+    test_attn_key_weights_matches_its_definition(B, Nq, Nk, H, hd, causal, kind)
+
+
 @pytest.mark.parametrize("B,Nq,Nk,H,hd,causal,kind", [      # more blocks than CUs: one group of waves per workgroup, and (last) two
     (2, 130, 130, 66, 64, True, "left"), (1, 333, 333, 90, 128, True, None), (3, 700, 700, 30, 64, True, "holes"), (2, 200, 650, 130, 64, False, "add"),
     (1, 700, 700, 45, 128, True, "add")])

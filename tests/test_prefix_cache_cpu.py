@@ -38,6 +38,7 @@ def test_workspace_queries_refuse_with_zero():
     lib = L.load()
     assert lib.hk_prefix_attn_ws(2, 2, 1, 8, 4, 64) > 0 and lib.hk_decode_attn_weights_ws(2, 2, 128, 5) > 0
     assert lib.hk_prefix_attn_ws(2, 2, 5, 8, 4, 64) == 0 and lib.hk_prefix_attn_ws(2, 2, 1, 8, 4, 80) == 0 and lib.hk_decode_attn_weights_ws(1, 1, 64, 0) == 0
+    assert lib.hk_attn_key_weights_ws(1, 1, 0, 4) == 0 and lib.hk_attn_key_weights_ws(2, 3, 5, 7) == 2 * 3 * 5 * 4 < lib.hk_attn_key_weights_ws(2, 3, 5, 7000)
     assert lib.hk_prefix_attn_ws(2, 2, 1, 8, 4, 64) == lib.hk_decode_attn_weights_ws(2, 2, 128, 5) == L.HK_NO_WS < lib.hk_prefix_attn_ws(2, 2, 1, 1000, 4, 64)
     with pytest.raises(RuntimeError, match="not supported"):
         ops.prefix_attention_ws(2, 2, 1, 8, 0, 64)
