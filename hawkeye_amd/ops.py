@@ -494,37 +494,32 @@ def decode_attn_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, po
 # it: a decode loop repeats layouts, and the checks cost the host more than these launches cost the device.  Nothing is kept by a
 # tensor's address; addresses, alignment and overlaps are checked by the library, every time.
 _layouts = {}
-_NUMBERS = (int, bool, type(None))
 
 
-def _layout(check, *args):
-    """check(*args), remembered by the layout of the tensors among args."""
-    key = (check, *[a if a.__class__ in _NUMBERS else (a.shape, a.stride(), a.dtype, a.device) for a in args])
-    got = _layouts.get(key)
-    if got is None:
-        got = check(*args)
-        if len(_layouts) >= 4096:
-            _layouts.clear()
-        _layouts[key] = got
+def _lay(t: Optional[torch.Tensor]):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+def _checked(key, check, *args):
+    """check(*args), which the layout `key` passes, kept for the calls that follow."""
+    got = check(*args)
+    if len(_layouts) >= 4096:
+        _layouts.clear()
+    _layouts[key] = got
     return got
 
 
-class _On:
-    """with _On(dev) as stream: the current device is dev and stream its current stream's handle (a device switch only if there is one)."""
-    __slots__ = ("dev", "back")
-
-    def __init__(self, dev: torch.device):
-        self.dev = dev
-
-    def __enter__(self) -> int:
-        self.back = torch.cuda.current_device()
-        if self.back != self.dev.index:
-            torch.cuda.set_device(self.dev.index)
-        return torch._C._cuda_getCurrentRawStream(self.dev.index)    # current_stream() builds a Stream object: 2.7 us a call against 0.1
-
-    def __exit__(self, *exc):
-        if self.back != self.dev.index:
-            torch.cuda.set_device(self.back)
+def _launch(entry, d, name: str, dev: int):
+    """entry(d) on the current stream of device dev, which is current meanwhile (current_stream() builds a Stream object: 2.7 us a call, 0.1 here)."""
+    back = torch._C._cuda_getDevice()
+    if back == dev:
+        L.check(entry(C.byref(d), torch._C._cuda_getCurrentRawStream(dev)), name)
+        return
+    torch.cuda.set_device(dev)
+    try:
+        L.check(entry(C.byref(d), torch._C._cuda_getCurrentRawStream(dev)), name)
+    finally:
+        torch.cuda.set_device(back)
 
 
 def _strides(t: torch.Tensor, name: str, H: int, hd: int):
@@ -578,7 +573,7 @@ def _prefix_layout(q, k_prefix, v_prefix, k, v, key_bias, out):
         if out.shape != q.shape:
             raise RuntimeError(f"prefix_attention: out must be {tuple(q.shape)}")
         ldo, bso = _strides(out, "out", H, hd)
-    return prefix_attention_ws(B, H, Nq, P, Nk, hd), (B, H, Nq, P, Nk, hd, ldq, bsq, ldkp, ldvp, ldk, bsk, ldv, bsv, ldo, bso, bias_bs)
+    return prefix_attention_ws(B, H, Nq, P, Nk, hd), q.device.index, q.is_contiguous(), (B, H, Nq, P, Nk, hd, ldq, bsq, ldkp, ldvp, ldk, bsk, ldv, bsv, ldo, bso, bias_bs)
 
 
 def prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -590,18 +585,21 @@ def prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Te
     [B,Nq,H,hd] bf16.  key_bias: optional fp32 [B, >= Nk] of the own keys (natural-log units); -1e4 or less removes the key.  A row that sees
     no key gives zeros.  out may not overlap an input.  ws: uint8 of at least prefix_attention_ws(...) bytes (default: allocated),
     for this call alone."""
-    need, nums = _layout(_prefix_layout, q, k_prefix, v_prefix, k, v, key_bias, out)
-    with _On(q.device) as stream:
-        if out is None:
-            out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
-        if ws is None:
-            if need != L.HK_NO_WS:
-                ws = torch.empty((need,), dtype=torch.uint8, device=q.device)
-        elif ws.dtype != torch.uint8 or ws.device != q.device or not ws.is_contiguous():
-            raise RuntimeError("prefix_attention: ws must be a contiguous uint8 tensor on q's device")
-        d = L.HkPrefixAttnDesc(q.data_ptr(), k_prefix.data_ptr(), v_prefix.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(key_bias),
-                               _ptr(ws), 0 if ws is None else ws.numel(), *nums)
-        L.check(L.load().hk_prefix_attn_bf16(C.byref(d), stream), "hk_prefix_attn_bf16")
+    key = (q.shape, q.stride(), q.dtype, q.device, k_prefix.shape, k_prefix.stride(), k_prefix.dtype, k_prefix.device, v_prefix.shape,
+           v_prefix.stride(), v_prefix.dtype, v_prefix.device, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device,
+           _lay(key_bias), _lay(out), "prefix_attention")
+    got = _layouts.get(key)
+    need, dev, dense, nums = got if got else _checked(key, _prefix_layout, q, k_prefix, v_prefix, k, v, key_bias, out)
+    if out is None:
+        out = torch.empty_like(q) if dense else torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+    if ws is None:
+        if need != L.HK_NO_WS:
+            ws = torch.empty((need,), dtype=torch.uint8, device=q.device)
+    elif ws.dtype != torch.uint8 or ws.device != q.device or not ws.is_contiguous():
+        raise RuntimeError("prefix_attention: ws must be a contiguous uint8 tensor on q's device")
+    d = L.HkPrefixAttnDesc(q.data_ptr(), k_prefix.data_ptr(), v_prefix.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(key_bias),
+                           _ptr(ws), 0 if ws is None else ws.numel(), *nums)
+    _launch(L.load().hk_prefix_attn_bf16, d, "hk_prefix_attn_bf16", dev)
     return out
 
 
@@ -632,7 +630,7 @@ def _step_layout(q, k_cache, v_cache, n_keys, H, head_dim, weight, key_bias, wei
     need = L.load().hk_decode_attn_weights_ws(B, H, head_dim, n_keys)
     if need == 0:
         raise RuntimeError(f"decode_attn_weights: shape B={B} H={H} n_keys={n_keys} head size {head_dim} is not supported")
-    return need, (B, H, head_dim, n_keys, k_cache.shape[1], *bias, *wi, *wo)
+    return need, q.device.index, (B, H, head_dim, n_keys, k_cache.shape[1], *bias, *wi, *wo)
 
 
 def decode_attn_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, n_keys: int, H: int, head_dim: int,
@@ -645,13 +643,15 @@ def decode_attn_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     if weight_out is None:
         weight_out = weight
     n_keys, H, head_dim = index(n_keys), index(H), index(head_dim)
-    need, nums = _layout(_step_layout, q, k_cache, v_cache, n_keys, H, head_dim, weight, key_bias, weight_out)
-    with _On(q.device) as stream:
-        out = torch.empty_like(q)
-        ws = None if need == L.HK_NO_WS else torch.empty((need,), dtype=torch.uint8, device=q.device)
-        d = L.HkStepWeightsDesc(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _ptr(key_bias), _ptr(weight), weight_out.data_ptr(),
-                                out.data_ptr(), _ptr(ws), need, *nums)
-        L.check(L.load().hk_decode_attn_weights_bf16(C.byref(d), stream), "hk_decode_attn_weights_bf16")
+    key = (q.shape, q.stride(), q.dtype, q.device, k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.device, v_cache.shape,
+           v_cache.stride(), v_cache.dtype, v_cache.device, n_keys, H, head_dim, _lay(weight), _lay(key_bias), _lay(weight_out), "decode_attn_weights")
+    got = _layouts.get(key)
+    need, dev, nums = got if got else _checked(key, _step_layout, q, k_cache, v_cache, n_keys, H, head_dim, weight, key_bias, weight_out)
+    out = torch.empty_like(q)
+    ws = None if need == L.HK_NO_WS else torch.empty((need,), dtype=torch.uint8, device=q.device)
+    d = L.HkStepWeightsDesc(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _ptr(key_bias), _ptr(weight), weight_out.data_ptr(),
+                            out.data_ptr(), _ptr(ws), need, *nums)
+    _launch(L.load().hk_decode_attn_weights_bf16, d, "hk_decode_attn_weights_bf16", dev)
     return out
 
 
@@ -673,7 +673,7 @@ def _key_weights_layout(q, k, key_bias, causal, weight, weight_out):
     need = L.load().hk_attn_key_weights_ws(B, H, Nq, Nk)
     if need == 0:
         raise RuntimeError(f"attn_key_weights: shape B={B} H={H} Nq={Nq} Nk={Nk} is not supported")
-    return need, (B, H, Nq, Nk, hd, 1 if causal else 0, ldq, bsq, ldk, bsk, bias_bs, *wi, *wo)
+    return need, q.device.index, (B, H, Nq, Nk, hd, 1 if causal else 0, ldq, bsq, ldk, bsk, bias_bs, *wi, *wo)
 
 
 def attn_key_weights(q: torch.Tensor, k: torch.Tensor, key_bias: Optional[torch.Tensor] = None, causal: bool = True,
@@ -684,13 +684,16 @@ def attn_key_weights(q: torch.Tensor, k: torch.Tensor, key_bias: Optional[torch.
     key_bias fp32 [B, >= Nk] (-1e4 or less removes the key).  A query that sees no key adds nothing."""
     if weight_out is None:
         weight_out = weight
-    need, nums = _layout(_key_weights_layout, q, k, key_bias, bool(causal), weight, weight_out)
-    with _On(q.device) as stream:
-        if weight_out is None:
-            weight_out = torch.empty((nums[0], nums[1], nums[3]), dtype=torch.float32, device=q.device)
-        ws = torch.empty((need,), dtype=torch.uint8, device=q.device)
-        d = L.HkKeyWeightsDesc(q.data_ptr(), k.data_ptr(), _ptr(key_bias), _ptr(weight), weight_out.data_ptr(), ws.data_ptr(), need, *nums)
-        L.check(L.load().hk_attn_key_weights_bf16(C.byref(d), stream), "hk_attn_key_weights_bf16")
+    causal = bool(causal)
+    key = (q.shape, q.stride(), q.dtype, q.device, k.shape, k.stride(), k.dtype, k.device, _lay(key_bias), causal, _lay(weight), _lay(weight_out),
+           "attn_key_weights")
+    got = _layouts.get(key)
+    need, dev, nums = got if got else _checked(key, _key_weights_layout, q, k, key_bias, causal, weight, weight_out)
+    if weight_out is None:
+        weight_out = torch.empty((nums[0], nums[1], nums[3]), dtype=torch.float32, device=q.device)
+    ws = torch.empty((need,), dtype=torch.uint8, device=q.device)
+    d = L.HkKeyWeightsDesc(q.data_ptr(), k.data_ptr(), _ptr(key_bias), _ptr(weight), weight_out.data_ptr(), ws.data_ptr(), need, *nums)
+    _launch(L.load().hk_attn_key_weights_bf16, d, "hk_attn_key_weights_bf16", dev)
     return weight_out
 
 
@@ -706,7 +709,7 @@ def _evict_layout(k, v, weight, n_keys, budget, recent, key_bias, ko, vo, wo, bo
     _one_device("cache_evict", k, v, weight, key_bias, ko, vo, wo, bo)
     if ko.dim() != 4 or vo.dim() != 4 or ko.shape[0] != B or vo.shape[0] != B or ko.shape[1] < budget or vo.shape[1] < budget:
         raise RuntimeError(f"cache_evict: k_out and v_out must be [{B},>= {budget},{H},{hd}]")
-    return (B, H, hd, n_keys, budget, recent, *_strides(k, "k", H, hd), *_strides(v, "v", H, hd), *_strides(ko, "k_out", H, hd),
+    return k.device.index, (B, H, hd, n_keys, budget, recent, *_strides(k, "k", H, hd), *_strides(v, "v", H, hd), *_strides(ko, "k_out", H, hd),
             *_strides(vo, "v_out", H, hd), *_per_key(weight, "weight", B, H, n_keys, True), *_per_key(wo, "weight_out", B, H, budget, True),
             *_per_key(key_bias, "key_bias", B, H, n_keys, True), *_per_key(bo, "key_bias_out", B, H, budget, True))
 
@@ -721,12 +724,15 @@ def cache_evict(k: torch.Tensor, v: torch.Tensor, weight: torch.Tensor, n_keys: 
     other tensors that overlap no input, rows behind budget left alone.  key_bias fp32 [B,H,>=n_keys]: per head, as heads keep different rows."""
     ko, vo, wo, bo = (k, v, weight, key_bias) if out is None else out
     n_keys, budget, recent = index(n_keys), index(budget), index(recent)
-    nums = _layout(_evict_layout, k, v, weight, n_keys, budget, recent, key_bias, ko, vo, wo, bo)
-    with _On(k.device) as stream:
-        kept = torch.empty((nums[0], nums[1], budget), dtype=torch.int32, device=k.device)
-        d = L.HkCacheEvictDesc(k.data_ptr(), v.data_ptr(), ko.data_ptr(), vo.data_ptr(), weight.data_ptr(), wo.data_ptr(), _ptr(key_bias), _ptr(bo),
-                               kept.data_ptr(), *nums)
-        L.check(L.load().hk_cache_evict_bf16(C.byref(d), stream), "hk_cache_evict_bf16")
+    key = (k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device, weight.shape, weight.stride(), weight.dtype, weight.device,
+           n_keys, budget, recent, _lay(key_bias), "cache_evict" if out is None else
+           (ko.shape, ko.stride(), ko.dtype, ko.device, vo.shape, vo.stride(), vo.dtype, vo.device, wo.shape, wo.stride(), wo.dtype, wo.device, _lay(bo)))
+    got = _layouts.get(key)
+    dev, nums = got if got else _checked(key, _evict_layout, k, v, weight, n_keys, budget, recent, key_bias, ko, vo, wo, bo)
+    kept = torch.empty((nums[0], nums[1], budget), dtype=torch.int32, device=k.device)
+    d = L.HkCacheEvictDesc(k.data_ptr(), v.data_ptr(), ko.data_ptr(), vo.data_ptr(), weight.data_ptr(), wo.data_ptr(), _ptr(key_bias), _ptr(bo),
+                           kept.data_ptr(), *nums)
+    _launch(L.load().hk_cache_evict_bf16, d, "hk_cache_evict_bf16", dev)
     return kept
 
 
