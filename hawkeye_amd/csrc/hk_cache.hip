@@ -9,7 +9,7 @@ constexpr float REMOVED = -1.0e4f;   // a key whose bias is at or below this doe
 
 // ---------------------------------------------------------------- key weights of a prompt
 // w_j = sum_i 2^(s_ij - z_i),  s_ij = q_i . k_j + b_j log2 e,  z_i = log2 sum_j 2^(s_ij).
-// Two launches of one structure (and a small one between them where few queries take their keys in chunks): a wave keeps 32 rows of one operand in registers and walks 64-row tiles of the other, which the
+// Beyond few keys (hk_key_weights_few_kernel), two launches of one structure (and a small one between them where few queries take their keys in chunks): a wave keeps 32 rows of one operand in registers and walks 64-row tiles of the other, which the
 // four waves of a workgroup share in LDS (two stages, LDS-DMA one tile ahead).  Both compute S^T = K . Q^T with
 // v_mfma_f32_32x32x16_bf16: lane -> query lane & 31, register i -> key (i & 3) + 8 (i >> 2) + 4 (lane >> 5).
 //   STATS: queries stay, keys pass: a reference point m and the sum of 2^(s - m) in the lane -> z.  m is the maximum of the row's first keys and
@@ -38,6 +38,25 @@ constexpr int NST = 2;               // stages (a power of two): a tile is reque
 constexpr float OVERFLOW_SUM = 1048576.0f;
 constexpr int BLK = 128;             // rows of the operand that stays, per workgroup
 constexpr int TILE = 64;             // rows of the operand that passes, per stage
+
+// a[0] of lane r & 15 <- the sum of a[r & 15] over the 32 lanes of a half: each step sends the half of the values that the partner lane keeps.
+// Partners differ in the bit that picks the half and share those before it: lane ^ 8, ^ 7, ^ 2, ^ 1 (all within 16 lanes), at last ^ 16.
+__device__ __forceinline__ void sum_over_queries(float (&a)[16], int r) {
+    auto halve = [&](auto o_c, auto dpp_c) __attribute__((always_inline)) {
+        constexpr int o = decltype(o_c)::value;
+        const bool up = (r & o) != 0;
+#pragma unroll
+        for (int i = 0; i < o; ++i) {
+            const float keep = up ? a[i + o] : a[i], send = up ? a[i] : a[i + o];
+            a[i] = keep + __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, send), decltype(dpp_c)::value, 0xf, 0xf, true));
+        }
+    };
+    halve(std::integral_constant<int, 8>{}, std::integral_constant<int, 0x128>{});      // row_ror:8
+    halve(std::integral_constant<int, 4>{}, std::integral_constant<int, 0x141>{});      // row_half_mirror
+    halve(std::integral_constant<int, 2>{}, std::integral_constant<int, 0x4e>{});       // quad_perm [2,3,0,1]
+    halve(std::integral_constant<int, 1>{}, std::integral_constant<int, 0xb1>{});       // quad_perm [1,0,3,2]
+    a[0] += __shfl_xor(a[0], 16, 64);
+}
 
 template <int HD, bool SUMS, bool BIAS, int GRP>
 __global__ __launch_bounds__(GRP * 256, 2) void hk_key_weights_kernel(const KeyWeightParams p) {
@@ -239,21 +258,7 @@ __global__ __launch_bounds__(GRP * 256, 2) void hk_key_weights_kernel(const KeyW
         }
     }
     if (SUMS) {
-        // over the 32 lanes of a half: each step sends the half of the values that the partner lane keeps; value r & 15 ends in lane r
-        auto halve = [&](auto o_c) {
-            constexpr int o = decltype(o_c)::value;
-            const bool up = (r & o) != 0;
-#pragma unroll
-            for (int i = 0; i < o; ++i) {
-                const float keep = up ? acc[i + o] : acc[i], send = up ? acc[i] : acc[i + o];
-                acc[i] = keep + __shfl_xor(send, o, 64);
-            }
-        };
-        halve(std::integral_constant<int, 8>{});
-        halve(std::integral_constant<int, 4>{});
-        halve(std::integral_constant<int, 2>{});
-        halve(std::integral_constant<int, 1>{});
-        acc[0] += __shfl_xor(acc[0], 16, 64);
+        sum_over_queries(acc, r);
         if (GRP > 1) {
             float* js = reinterpret_cast<float*>(smem) + wave * 64 + lane;
             __syncthreads();                               // everyone has left the last tiles
@@ -311,6 +316,126 @@ __global__ __launch_bounds__(256) void hk_key_weights_join_kernel(const KeyWeigh
     p.z[i] = sum == 0.f ? INFINITY : M + __log2f(sum);
 }
 
+// Few keys: one launch, a workgroup per (sequence, head), no second pass over the products.  A wave takes 32 queries at a time and keeps their
+// scores of ALL keys in registers (NB blocks of 32; S^T = K . Q^T as above), so the softmax is the plain one: maximum, exponentials, sum.
+// K lies in LDS as the fragments that the matrix instruction takes.  A block's weights are added over its 32 queries by halving exchanges (as
+// above) into the wave's own sums in LDS; the eight waves' sums are added in order at the end.
+template <int HD, int NB, bool BIAS>
+__global__ __launch_bounds__(512, 2) void hk_key_weights_few_kernel(const KeyWeightParams p) {
+    constexpr int NKS = HD / 16, NW = 8;
+    extern __shared__ __attribute__((aligned(16))) char smem[];      // fragments [NB][NKS][64 lanes] of 16 bytes, then sums [NW][NB * 32], biases [NB * 32]
+    bf16x8* kl = reinterpret_cast<bf16x8*>(smem);
+    float* sums = reinterpret_cast<float*>(smem + NB * NKS * 1024);
+    float* bl = sums + NW * NB * 32;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 31, h = lane >> 5;
+    const int b = blockIdx.x / p.H, head = blockIdx.x - b * p.H;
+    const int off = p.Nk - p.Nq, nkb = (p.Nk + 31) / 32, nqb = (p.Nq + 31) / 32;
+    const __bf16* kp = p.K + (int64_t)b * p.bsk + head * HD + 8 * h;
+    const __bf16* qp = p.Q + (int64_t)b * p.bsq + head * HD + 8 * h;
+    bf16x8 qf[NKS];
+    auto load_q = [&](int qb) {
+        const __bf16* x = qp + (int64_t)min(qb * 32 + r, p.Nq - 1) * p.ldq;
+#pragma unroll
+        for (int s = 0; s < NKS; ++s) qf[s] = *reinterpret_cast<const bf16x8*>(x + 16 * s);
+    };
+    if (wave < nqb) load_q(nqb - 1 - wave);
+    for (int g = wave; g < nkb; g += NW) {
+        const __bf16* x = kp + (int64_t)min(g * 32 + r, p.Nk - 1) * p.ldk;
+        bf16x8 kf[NKS];
+#pragma unroll
+        for (int s = 0; s < NKS; ++s) kf[s] = *reinterpret_cast<const bf16x8*>(x + 16 * s);
+#pragma unroll
+        for (int s = 0; s < NKS; ++s) kl[(g * NKS + s) * 64 + lane] = kf[s];
+    }
+    for (int j = tid; j < NW * NB * 32; j += NW * 64) sums[j] = 0.f;
+    if (BIAS)
+        for (int j = tid; j < nkb * 32; j += NW * 64) {
+            const float v = p.bias[(int64_t)b * p.bias_bs + min(j, p.Nk - 1)];
+            bl[j] = v <= REMOVED ? -INFINITY : v * HK_LOG2E;
+        }
+    __syncthreads();
+    for (int u = 0; u * NW < nqb; ++u) {                   // causal: the longest blocks first, to and fro over the waves
+        const int qb = nqb - 1 - (u * NW + (u & 1 ? NW - 1 - wave : wave));
+        if (qb < 0) break;
+        if (u) load_q(qb);
+        const int q = qb * 32 + r, last = p.causal ? min(p.Nk - 1, q + off) : p.Nk - 1;      // the last key the lane's query sees
+        const int gn = p.causal ? min(nkb, (qb * 32 + 31 + off) / 32 + 1) : nkb;
+        const int clear = p.causal ? min(p.Nk - 1, qb * 32 + off) : p.Nk - 1;                // keys up to here every query of the block sees
+        f32x16 st[NB];
+        float mx = -INFINITY;
+#pragma unroll
+        for (int g0 = 0; g0 < NB; g0 += 2)
+            if (g0 < gn) {                                 // two blocks: independent chains (one behind the keys: its scores are masked, all of them)
+#pragma unroll
+                for (int g = g0; g < g0 + 2; ++g)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) st[g][i] = 0.f;
+#pragma unroll
+                for (int s = 0; s < NKS; ++s)
+#pragma unroll
+                    for (int g = g0; g < g0 + 2; ++g)
+                        st[g] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kl[(g * NKS + s) * 64 + lane], qf[s], st[g], 0, 0, 0);
+#pragma unroll
+                for (int g = g0; g < g0 + 2; ++g) {
+                    if (BIAS) {
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {      // register 4 x + j <-> key 32 g + 8 x + 4 h + j
+                            const f32x4 v = *reinterpret_cast<const f32x4*>(bl + g * 32 + 8 * x + 4 * h);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) st[g][4 * x + j] = v[j] == -INFINITY ? -INFINITY : st[g][4 * x + j] + v[j];
+                        }
+                    }
+                    if (g * 32 + 31 > clear) {
+                        const int lim = last - g * 32 - 4 * h;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if ((i & 3) + 8 * (i >> 2) > lim) st[g][i] = -INFINITY;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[g][i]);
+                }
+            }
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        if (mx == -INFINITY) mx = 0.f;                     // no key: every exponential is 0
+        float l = 0.f;
+#pragma unroll
+        for (int g0 = 0; g0 < NB; g0 += 2)
+            if (g0 < gn) {
+                float x[2] = {0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        st[g0 + g][i] = __builtin_amdgcn_exp2f(st[g0 + g][i] - mx);
+                        x[g] += st[g0 + g][i];
+                    }
+                l += x[0] + x[1];
+            }
+        l += __shfl_xor(l, 32, 64);
+        float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);       // NaN stays
+        if (q >= p.Nq) inv = 0.f;
+#pragma unroll
+        for (int g = 0; g < NB; ++g)
+            if (g < gn) {
+                float a[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) a[i] = st[g][i] * inv;
+                sum_over_queries(a, r);
+                if (r < 16) sums[wave * NB * 32 + g * 32 + (r & 3) + 8 * (r >> 2) + 4 * h] += a[0];
+            }
+    }
+    __syncthreads();
+    const float* wi = p.w_in ? p.w_in + (int64_t)b * p.wi_bs + (int64_t)head * p.wi_hs : nullptr;
+    float* wo = p.w_out + (int64_t)b * p.wo_bs + (int64_t)head * p.wo_hs;
+    for (int j = tid; j < p.Nk; j += NW * 64) {
+        float x = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) x += sums[w * NB * 32 + j];
+        wo[j] = (wi ? wi[j] : 0.f) + x;
+    }
+}
+
 // STATS of few queries over many keys: chunks of the keys, a workgroup per CU, four tiles at least.  The last 32 / 512 of so many tokens,
 // 32 heads of 128, without : with chunks (us, all launches): 1000 17.0 : 13.0, 23.8 : 21.7; 2047 27.5 : 15.2, 37.9 : 31.0; 16000 170 : 52, 219 : 164;
 // 4 sequences of 16000 285 : 231 (K is read twice: 216), 665 : 670.  Twice as many chunks: 16000 tokens 57 and 169; eight tiles at least: 1000 tokens 14.8.
@@ -321,7 +446,16 @@ int key_chunks(int64_t blocks, int Nk, int* ct) {
     *ct = (int)((tiles + n - 1) / n);
     return (tiles + *ct - 1) / *ct;
 }
-size_t key_weights_bytes(int64_t B, int64_t H, int64_t Nq, int Nk) {
+// hk_key_weights_few_kernel or two launches?  The former as long as its waves have up to 12 blocks of 32 x 32 products each.  Few : two, 32 heads of 128
+// (us): prompts of 20 / 65 / 128 / 256 / 352 tokens 4.2 : 7.6, 5.6 : 9.9, 6.5 : 10.2, 10.5 : 13.6, 14.6 : 15.8, 32 of them 7 : 13, 13 : 20, 17 : 28, 44 : 57,
+// 61 : 88; without a diagonal, 128 keys and 400 / 800 / 1600 queries 9.9 : 13.3, 15.6 : 16.6, 23.4 : 24.5, 256 keys and 200 / 400 11.5 : 13.5, 17.0 : 15.3,
+// 384 keys and 200 15.3 : 14.6; heads of 64, 256 keys and 400 14.2 : 11.9.
+bool few_keys(int64_t Nq, int64_t Nk, bool causal) {
+    const int64_t nqb = (Nq + 31) / 32, nkb = (Nk + 31) / 32;
+    return Nk <= 384 && nqb * nkb - (causal ? nqb * (nqb - 1) / 2 : 0) <= 96;
+}
+size_t key_weights_bytes(int64_t B, int64_t H, int64_t Nq, int Nk, bool causal) {
+    if (few_keys(Nq, Nk, causal)) return HK_NO_WS;
     int ct;
     const int nch = key_chunks((Nq + BLK - 1) / BLK * B * H, Nk, &ct);
     return (size_t)(B * H * Nq) * (nch > 1 ? 8 * nch + 4 : 4);
@@ -350,8 +484,25 @@ int launch_key_weights(KeyWeightParams p, hipStream_t s) {
     const bool two = blocks <= 256 ? n_pass > 2 * TILE : blocks <= 512 && n_pass > 10 * TILE;
     return two ? launch_groups<HD, SUMS, BIAS, 2>(p, s) : launch_groups<HD, SUMS, BIAS, 1>(p, s);
 }
+template <int HD, int NB, bool BIAS>
+int launch_few(const KeyWeightParams& p, hipStream_t s) {
+    constexpr int LDS = NB * 32 * (HD * 2 + 9 * 4);
+    static std::atomic<unsigned long long> attr_done{0};   // per device
+    const hipError_t e = hk_lds_attr_once(attr_done, reinterpret_cast<const void*>(&hk_key_weights_few_kernel<HD, NB, BIAS>), LDS);
+    if (e != hipSuccess) {
+        hk_set_error("hk_attn_key_weights_bf16: hipFuncSetAttribute(%d B LDS): %s", LDS, hipGetErrorString(e));
+        return HK_ELAUNCH;
+    }
+    hipLaunchKernelGGL((hk_key_weights_few_kernel<HD, NB, BIAS>), dim3((unsigned)(p.B * p.H)), dim3(512), LDS, s, p);
+    return HK_OK;
+}
 template <int HD>
 int launch_both(const KeyWeightParams& p, hipStream_t s) {
+    if (few_keys(p.Nq, p.Nk, p.causal)) {
+        if (p.Nk <= 128) return p.bias ? launch_few<HD, 4, true>(p, s) : launch_few<HD, 4, false>(p, s);
+        if (p.Nk <= 256) return p.bias ? launch_few<HD, 8, true>(p, s) : launch_few<HD, 8, false>(p, s);
+        return p.bias ? launch_few<HD, 12, true>(p, s) : launch_few<HD, 12, false>(p, s);
+    }
     const int rc = p.bias ? launch_key_weights<HD, false, true>(p, s) : launch_key_weights<HD, false, false>(p, s);
     if (rc != HK_OK) return rc;
     if (p.nch > 1) hipLaunchKernelGGL(hk_key_weights_join_kernel, dim3((unsigned)(((int64_t)p.B * p.H * p.Nq + 255) / 256)), dim3(256), 0, s, p);
@@ -721,9 +872,9 @@ int launch_evict_all(const EvictParams& p, hipStream_t s) {
 
 }  // namespace
 
-extern "C" size_t hk_attn_key_weights_ws(int32_t B, int32_t H, int32_t Nq, int32_t Nk) {
-    if (B < 1 || B >= 65536 || H < 1 || H >= 65536 || Nq < 1 || Nk < 1 || Nq >= (1 << 26) || Nk >= (1 << 26)) return 0;
-    return key_weights_bytes(B, H, Nq, Nk);
+extern "C" size_t hk_attn_key_weights_ws(int32_t B, int32_t H, int32_t Nq, int32_t Nk, int32_t causal) {
+    if (B < 1 || B >= 65536 || H < 1 || H >= 65536 || Nq < 1 || Nk < 1 || Nq >= (1 << 26) || Nk >= (1 << 26) || (causal && Nk < Nq)) return 0;
+    return key_weights_bytes(B, H, Nq, Nk, causal != 0);
 }
 
 extern "C" int hk_attn_key_weights_bf16(const hk_key_weights_desc* d, void* stream) {
@@ -743,12 +894,13 @@ extern "C" int hk_attn_key_weights_bf16(const hk_key_weights_desc* d, void* stre
                "hk_attn_key_weights_bf16: rows of w_out must not overlap, strides must not be negative");
     HK_REQUIRE(d->w_in != d->w_out || (d->wi_bs == d->wo_bs && d->wi_hs == d->wo_hs),
                "hk_attn_key_weights_bf16: weights updated in place must have one layout");
-    const size_t need = key_weights_bytes(d->B, d->H, d->Nq, d->Nk);
-    HK_REQUIRE(d->ws && d->ws_bytes >= need, "hk_attn_key_weights_bf16: workspace of %zu bytes, %zu needed (hk_attn_key_weights_ws)",
+    const size_t need = key_weights_bytes(d->B, d->H, d->Nq, d->Nk, d->causal != 0);
+    const bool few = need == HK_NO_WS;
+    HK_REQUIRE(few || (d->ws && d->ws_bytes >= need), "hk_attn_key_weights_bf16: workspace of %zu bytes, %zu needed (hk_attn_key_weights_ws)",
                d->ws ? d->ws_bytes : (size_t)0, need);
     {
         const int64_t row = (int64_t)d->H * d->head_dim;
-        const HkSpan wo = hk_span(d->w_out, d->B, d->wo_bs, d->H, d->wo_hs, d->Nk, 4), w = hk_span(d->ws, 1, 0, 1, 0, (int64_t)need, 1);
+        const HkSpan wo = hk_span(d->w_out, d->B, d->wo_bs, d->H, d->wo_hs, d->Nk, 4), w = hk_span(few ? nullptr : d->ws, 1, 0, 1, 0, (int64_t)need, 1);
         const HkSpan in[] = {hk_span(d->Q, d->B, d->bsq, d->Nq, d->ldq, row, 2), hk_span(d->K, d->B, d->bsk, d->Nk, d->ldk, row, 2),
                              hk_span(d->key_bias, d->B, d->bias_bs, 1, 0, d->Nk, 4),
                              d->w_in == d->w_out ? HkSpan{0, 0} : hk_span(d->w_in, d->B, d->wi_bs, d->H, d->wi_hs, d->Nk, 4)};

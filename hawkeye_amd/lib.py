@@ -162,7 +162,7 @@ SYMBOLS = {
     "hk_decode_attn_weights_bf16": (C.c_int, [C.POINTER(HkStepWeightsDesc), C.c_void_p]),
     "hk_decode_attn_weights_ws": (C.c_size_t, [C.c_int32] * 4),
     "hk_attn_key_weights_bf16": (C.c_int, [C.POINTER(HkKeyWeightsDesc), C.c_void_p]),
-    "hk_attn_key_weights_ws": (C.c_size_t, [C.c_int32] * 4),
+    "hk_attn_key_weights_ws": (C.c_size_t, [C.c_int32] * 5),
     "hk_cache_evict_bf16": (C.c_int, [C.POINTER(HkCacheEvictDesc), C.c_void_p]),
     "hk_argmax_f32": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int64, C.c_void_p]),
     "hk_silu_mul_bf16": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p]),

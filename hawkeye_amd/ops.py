@@ -670,7 +670,7 @@ def _key_weights_layout(q, k, key_bias, causal, weight, weight_out):
     bias_bs, _ = _per_key(key_bias, "key_bias", B, 1, Nk, False)
     wi = _per_key(weight, "weight", B, H, Nk, True)
     wo = (H * Nk, Nk) if weight_out is None else _per_key(weight_out, "weight_out", B, H, Nk, True)
-    need = L.load().hk_attn_key_weights_ws(B, H, Nq, Nk)
+    need = L.load().hk_attn_key_weights_ws(B, H, Nq, Nk, 1 if causal else 0)
     if need == 0:
         raise RuntimeError(f"attn_key_weights: shape B={B} H={H} Nq={Nq} Nk={Nk} is not supported")
     return need, q.device.index, (B, H, Nq, Nk, hd, 1 if causal else 0, ldq, bsq, ldk, bsk, bias_bs, *wi, *wo)
@@ -691,8 +691,8 @@ def attn_key_weights(q: torch.Tensor, k: torch.Tensor, key_bias: Optional[torch.
     need, dev, nums = got if got else _checked(key, _key_weights_layout, q, k, key_bias, causal, weight, weight_out)
     if weight_out is None:
         weight_out = torch.empty((nums[0], nums[1], nums[3]), dtype=torch.float32, device=q.device)
-    ws = torch.empty((need,), dtype=torch.uint8, device=q.device)
-    d = L.HkKeyWeightsDesc(q.data_ptr(), k.data_ptr(), _ptr(key_bias), _ptr(weight), weight_out.data_ptr(), ws.data_ptr(), need, *nums)
+    ws = None if need == L.HK_NO_WS else torch.empty((need,), dtype=torch.uint8, device=q.device)
+    d = L.HkKeyWeightsDesc(q.data_ptr(), k.data_ptr(), _ptr(key_bias), _ptr(weight), weight_out.data_ptr(), _ptr(ws), need, *nums)
     _launch(L.load().hk_attn_key_weights_bf16, d, "hk_attn_key_weights_bf16", dev)
     return weight_out
 

@@ -476,7 +476,8 @@ size_t hk_decode_attn_weights_ws(int32_t B, int32_t H, int32_t head_dim, int32_t
  * Q [B,Nq,H,hd] (carrying softmax_scale * log2(e)) and K [B,Nk,H,hd] bf16 through strides as in hk_attn_desc; weights fp32 with strides
  * (*_bs, *_hs), w_in NULL = zeros, may be w_out; key_bias[b * bias_bs + j] as in hk_prefix_attn_desc; a query that sees no key adds nothing.
  * ws: hk_attn_key_weights_ws bytes of the caller's, 16-byte aligned (the rows' log2 sums; few queries take theirs in chunks of keys, joined in
- * index order).  Strides as in hk_prefix_attn_desc.  Two or three launches: row sums, their join, weights; bit-reproducible. */
+ * index order; HK_NO_WS: few keys, one launch, ws may be NULL).  Strides as in hk_prefix_attn_desc.  Else two or three launches: row sums, their
+ * join, weights.  Bit-reproducible. */
 typedef struct hk_key_weights_desc {
     const void* Q;
     const void* K;
@@ -489,7 +490,7 @@ typedef struct hk_key_weights_desc {
     int64_t ldq, bsq, ldk, bsk, bias_bs, wi_bs, wi_hs, wo_bs, wo_hs;
 } hk_key_weights_desc;
 int hk_attn_key_weights_bf16(const hk_key_weights_desc* d, void* stream);
-size_t hk_attn_key_weights_ws(int32_t B, int32_t H, int32_t Nq, int32_t Nk); /* 0: refused shape */
+size_t hk_attn_key_weights_ws(int32_t B, int32_t H, int32_t Nq, int32_t Nk, int32_t causal); /* 0: refused shape */
 
 /* Eviction by accumulated attention weight: for every (sequence, head) the last `recent` of n_keys cache rows and, of the rest, the
  * budget - recent with the largest weight (equal weights: the lowest index) move, in ascending order, to rows [0, budget) of the output:

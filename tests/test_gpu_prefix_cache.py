@@ -217,6 +217,14 @@ def test_attn_key_weights_of_few_queries(B, Nq, Nk, H, hd, causal, kind):
     test_attn_key_weights_matches_its_definition(B, Nq, Nk, H, hd, causal, kind)
 
 
+@pytest.mark.parametrize("B,Nq,Nk,H,hd,causal,kind", [      # few keys: one launch; beyond (last two): two
+    (2, 1, 33, 3, 128, True, "add"), (3, 31, 97, 2, 64, True, "holes"), (2, 128, 128, 3, 128, True, "left"), (2, 129, 161, 2, 128, True, "all"),
+    (1, 256, 256, 2, 64, True, "left"), (2, 200, 256, 2, 128, False, "add"), (2, 353, 384, 3, 128, True, "left"), (1, 384, 384, 2, 64, True, None),
+    (1, 800, 65, 3, 128, False, "holes"), (40, 70, 70, 20, 64, True, "add"), (2, 385, 385, 2, 128, True, "left"), (1, 300, 384, 2, 64, False, "add")])
+def test_attn_key_weights_of_few_keys(B, Nq, Nk, H, hd, causal, kind):
+    test_attn_key_weights_matches_its_definition(B, Nq, Nk, H, hd, causal, kind)
+
+
 @pytest.mark.parametrize("B,Nq,Nk,H,hd,causal,kind", [      # more blocks than CUs: one group of waves per workgroup, and (last) two
     (2, 130, 130, 66, 64, True, "left"), (1, 333, 333, 90, 128, True, None), (3, 700, 700, 30, 64, True, "holes"), (2, 200, 650, 130, 64, False, "add"),
     (1, 700, 700, 45, 128, True, "add")])

@@ -38,7 +38,8 @@ def test_workspace_queries_refuse_with_zero():
     lib = L.load()
     assert lib.hk_prefix_attn_ws(2, 2, 1, 8, 4, 64) > 0 and lib.hk_decode_attn_weights_ws(2, 2, 128, 5) > 0
     assert lib.hk_prefix_attn_ws(2, 2, 5, 8, 4, 64) == 0 and lib.hk_prefix_attn_ws(2, 2, 1, 8, 4, 80) == 0 and lib.hk_decode_attn_weights_ws(1, 1, 64, 0) == 0
-    assert lib.hk_attn_key_weights_ws(1, 1, 0, 4) == 0 and lib.hk_attn_key_weights_ws(2, 3, 5, 7) == 2 * 3 * 5 * 4 < lib.hk_attn_key_weights_ws(2, 3, 5, 7000)
+    assert lib.hk_attn_key_weights_ws(1, 1, 0, 4, 0) == 0 == lib.hk_attn_key_weights_ws(1, 1, 5, 4, 1) and lib.hk_attn_key_weights_ws(2, 3, 5, 7, 1) == L.HK_NO_WS
+    assert lib.hk_attn_key_weights_ws(30, 30, 500, 500, 1) == 30 * 30 * 500 * 4 and lib.hk_attn_key_weights_ws(2, 3, 5, 7000, 1) > 2 * 3 * 5 * 4
     assert lib.hk_prefix_attn_ws(2, 2, 1, 8, 4, 64) == lib.hk_decode_attn_weights_ws(2, 2, 128, 5) == L.HK_NO_WS < lib.hk_prefix_attn_ws(2, 2, 1, 1000, 4, 64)
     with pytest.raises(RuntimeError, match="not supported"):
         ops.prefix_attention_ws(2, 2, 1, 8, 0, 64)
@@ -70,10 +71,13 @@ def _weights(**kw):
     return L.load().hk_attn_key_weights_bf16(C.byref(L.HkKeyWeightsDesc(**base)), None)
 
 
+MANY = dict(Nq=500, Nk=500, bsq=64000, bsk=64000, wo_bs=1000, wo_hs=500)      # too many products for one launch, which takes no workspace
+
+
 @pytest.mark.parametrize("kw,text", [
     (dict(K=None), "null operand"), (dict(Nq=10), "bad shape"), (dict(Nq=0), "bad shape"), (dict(head_dim=256), "bad shape"), (dict(ldq=100), "strides"),
-    (dict(Q=A + 4), "aligned"), (dict(wo_hs=8), "w_out must not overlap"), (dict(ws_bytes=63), "workspace"), (dict(w_in=3 * A, wi_bs=20, wi_hs=10), "one layout"),
-    (dict(w_out=A), "overlaps an input"), (dict(ws=3 * A), "overlaps the workspace")])
+    (dict(Q=A + 4), "aligned"), (dict(wo_hs=8), "w_out must not overlap"), (dict(ws_bytes=63, **MANY), "workspace"), (dict(ws=None, **MANY), "workspace"), (dict(w_in=3 * A, wi_bs=20, wi_hs=10), "one layout"),
+    (dict(w_out=A), "overlaps an input"), (dict(ws=3 * A, **MANY), "overlaps the workspace")])
 def test_attn_key_weights_refuses(kw, text):
     _refused(_weights(**kw), text)
 
