@@ -368,6 +368,8 @@ __global__ __launch_bounds__(NW * 64, 2) void hk_prefix_part_kernel(const Prefix
 // maximum of every tile until it does.
 // Rows are a sequence's (its keys: the prefix, then its own up to the diagonal; or its own alone) or, for the prefix alone, rows of
 // all sequences packed: whichever leaves fewer 128-row blocks part empty (make_plan).
+// GRP = 2: two such groups of waves share a workgroup, each with stages of its own, and take every other tile; the second's (m, l, o) joins the
+// first's through LDS at the end (where CUs would be idle: make_plan).
 // A tile with nothing to mask goes by halves, the second half's products among the first half's exponentials.
 // Measured (32 heads of 128): 8 sequences of 512 rows over 1400 shared keys and their own 120 us, 930 TFLOP/s; the matrix unit is busy half of
 // the time.  Copies of the loop without one part, in-bounds and for timing only: without LDS-DMA and barriers 107-116 us, without the reads of
@@ -391,15 +393,17 @@ __device__ __forceinline__ float half_max(float x) {    // the larger of the two
     return fmaxf(a, b);
 }
 
-template <int HD, bool BIAS>
-__global__ __launch_bounds__(256, 2) void hk_prefix_rows_kernel(const PrefixParams p, const RowsParams q) {
+template <int HD, bool BIAS, int GRP>
+__global__ __launch_bounds__(GRP * 256, 2) void hk_prefix_rows_kernel(const PrefixParams p, const RowsParams q) {
     constexpr int ROWB = HD * 2, CH = HD / 8, NKS = HD / 16, NDT = HD / 32;
     constexpr int STAGE = 2 * KT * ROWB;
     constexpr int RPP = 256 / CH;                          // key rows one workgroup-wide LDS-DMA covers
     constexpr int NP = KT / RPP;                           // of them per operand and tile
-    extern __shared__ __attribute__((aligned(16))) char smem[];      // [2][K | V][KT keys][ROWB], then [2][KT] biases
-    float* blds = reinterpret_cast<float*>(smem + 2 * STAGE);
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    extern __shared__ __attribute__((aligned(16))) char smem[];      // per group: [2][K | V][KT keys][ROWB]; then per group [2][KT] biases
+    const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int grp = GRP == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+    char* gs = smem + grp * 2 * STAGE;
+    float* blds = reinterpret_cast<float*>(smem + GRP * 2 * STAGE) + grp * 2 * KT;
     const int r = lane & 31, h = lane >> 5;
 
     // ---- which rows, which keys (blockIdx = ... * H + head: the row blocks of a head share an XCD's L2 where H is a multiple of 8) ----
@@ -467,7 +471,7 @@ __global__ __launch_bounds__(256, 2) void hk_prefix_rows_kernel(const PrefixPara
     float br = 0.f;
     auto load_tile = [&](const __bf16* kb, const __bf16* vb, int64_t ldk, int64_t ldv, uint32_t kl, uint32_t vl, int kt, int n, int stage)
         __attribute__((always_inline)) {
-        char* ks = smem + stage * STAGE + wave * (64 / CH) * ROWB;
+        char* ks = gs + stage * STAGE + wave * (64 / CH) * ROWB;
         char* vs = ks + KT * ROWB;
         // the swizzle goes on the source chunk (the LDS image is lane-linear); RPP is a multiple of every swizzle's period
         if (kt + KT <= n) {
@@ -486,6 +490,7 @@ __global__ __launch_bounds__(256, 2) void hk_prefix_rows_kernel(const PrefixPara
         }
     };
     auto issue = [&](int t, int stage) __attribute__((always_inline)) {
+        if (GRP > 1 && t >= NT) return;
         if (t < nA) {
             load_tile(kA, vA, p.ldkp, p.ldvp, klA, vlA, t * KT, a1 - a0, stage);
         } else {
@@ -508,20 +513,20 @@ __global__ __launch_bounds__(256, 2) void hk_prefix_rows_kernel(const PrefixPara
     bool unset = true, pending = true;                     // this row / some row of the wave has met no key yet
 
     if (NT > 0) {
-        issue(0, 0);
+        issue(grp, 0);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        if (BIAS && nA == 0 && tid < KT) blds[tid] = br;
+        if (BIAS && grp >= nA && tid < KT) blds[tid] = br;
         __syncthreads();
     }
-    for (int t = 0; t < NT; ++t) {
-        const int cur = t & 1;
-        if (t + 1 < NT) issue(t + 1, cur ^ 1);
+    for (int u = 0; u * GRP < NT; ++u) {
+        const int cur = u & 1, t = u * GRP + grp;
+        if (t + GRP < NT) issue(t + GRP, cur ^ 1);
         const bool own = t >= nA;
         const int kt = (own ? t - nA : t) * KT, n = own ? k1 : a1 - a0;
-        if (active && (!own || kt <= q0 + 31 + off)) {
+        if (active && (GRP == 1 || t < NT) && (!own || kt <= q0 + 31 + off)) {
             int ko = koff0, vo = voff0;
             asm volatile("" : "+v"(ko), "+v"(vo));          // the offsets are made from these here, not kept across tiles in registers
-            const char* ks = smem + cur * STAGE;
+            const char* ks = gs + cur * STAGE;
             const char* vs = ks + KT * ROWB;
             uint64_t gone = 0;                             // keys of this tile that no row has
             bool biased = false;
@@ -722,10 +727,32 @@ __global__ __launch_bounds__(256, 2) void hk_prefix_rows_kernel(const PrefixPara
             }
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the next tile's LDS-DMA, unknown to the compiler
-        if (BIAS && t + 1 >= nA && t + 1 < NT && tid < KT) blds[(cur ^ 1) * KT + tid] = br;
+        if (BIAS && t + GRP >= nA && t + GRP < NT && tid < KT) blds[(cur ^ 1) * KT + tid] = br;
         __syncthreads();
     }
 
+    if (GRP > 1) {                                         // the second group's part joins the first's (everyone has left the last tiles)
+        float* js = reinterpret_cast<float*>(smem) + tid;  // [NDT * 16 + 2][256 threads]
+        if (unset) m = M_NONE;
+        if (grp) {
+            js[0] = m;
+            js[256] = l;
+#pragma unroll
+            for (int d = 0; d < NDT; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) js[(2 + 16 * d + i) * 256] = ot[d][i];
+        }
+        __syncthreads();
+        if (grp) return;
+        const float m1 = js[0], M = fmaxf(m, m1), f0 = __builtin_amdgcn_exp2f(m - M), f1 = __builtin_amdgcn_exp2f(m1 - M);
+        l = l * f0 + js[256] * f1;
+#pragma unroll
+        for (int d = 0; d < NDT; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) ot[d][i] = ot[d][i] * f0 + js[(2 + 16 * d + i) * 256] * f1;
+        unset = M <= M_NONE;
+        m = M;
+    }
     l += __shfl_xor(l, 32, 64);
     if (q0 + r >= nrows) return;
     const int row = row0 + q0 + r;
@@ -881,7 +908,7 @@ __global__ __launch_bounds__(256) void hk_step_join_kernel(const PrefixParams p,
 // ---------------------------------------------------------------- host side
 enum { ONCE, SMALL, MIXED, PACKED, FUSED };
 struct Plan {
-    int mode, rt;
+    int mode, rt, groups;            // groups: of four waves per workgroup of hk_prefix_rows_kernel, if two
     RowsParams rows;
 };
 
@@ -951,11 +978,16 @@ Plan make_plan(PrefixParams& p, int hd, bool raw) {
         const double own = (double)H * B * m.rows.nob * ((p.Nk + KT - 1) / KT), pre = (double)((p.P + KT - 1) / KT);
         const double fused_n = (double)H * B * m.rows.nob;
         double fused = (own + fused_n * pre) / (fused_n < 512 ? fused_n : 512);
+        // Two groups of waves where CUs would be idle.  One : two, 32 heads of 128 (us): one sequence's 37 rows over 100 / 350 / 1201 9.5 : 9.7, 13.8 : 13.1,
+        // 28.2 : 22.9, 200 over 350 18.9 : 16.7, 512 over 1400 43.5 : 36.2; chunks of a prefix (PACKED), 37 rows over 350 / 1201 11.2 : 12.5, 13.4 : 14.5.
+        const bool two = fused_n <= 256 && (p.P + KT - 1) / KT + (p.Nk + KT - 1) / KT >= 6;
+        if (two) fused = 0.8 * fused + 1.0;
         const double packed_n = (double)H * m.rows.npb * p.npc + (double)H * B * m.rows.nob * p.noc;
         double packed = (own + (double)H * m.rows.npb * pre) / (packed_n < 512 ? packed_n : 512);
         packed += 4.0 + (double)p.R * H * (p.npc + p.noc) * hd * 8 / 4.5e6;      // the join: a launch, partial sums written and read at 4.5 TB/s
         m.mode = p.P > 0 && packed < fused ? PACKED : FUSED;
         if (p.P == 0 && packed < fused && p.noc > 1) m.mode = PACKED;
+        if (m.mode == FUSED && two) m.groups = 2;
     }
     m.rows.packed = m.mode != FUSED;
     m.rows.pjobs = m.mode == MIXED || m.mode == PACKED ? H * m.rows.npb * p.npc : 0;
@@ -991,17 +1023,21 @@ void launch_once(const PrefixParams& p, const StepWeights& sw, hipStream_t s) {
     if (p.bias) hipLaunchKernelGGL((hk_prefix_part_kernel<HD, 1, true, RAW, 8, true>), grid, dim3(512), 0, s, p, sw);
     else hipLaunchKernelGGL((hk_prefix_part_kernel<HD, 1, false, RAW, 8, true>), grid, dim3(512), 0, s, p, sw);
 }
-template <int HD, bool BIAS>
-int launch_rows(const PrefixParams& p, const Plan& m, hipStream_t s) {
-    constexpr int LDS = 2 * 2 * KT * HD * 2 + (BIAS ? 2 * KT * 4 : 0);
+template <int HD, bool BIAS, int GRP>
+int launch_rows_groups(const PrefixParams& p, const Plan& m, hipStream_t s) {
+    constexpr int LDS = GRP * (2 * 2 * KT * HD * 2 + (BIAS ? 2 * KT * 4 : 0));
     static std::atomic<unsigned long long> attr_done{0};   // per device
-    const hipError_t e = hk_lds_attr_once(attr_done, reinterpret_cast<const void*>(&hk_prefix_rows_kernel<HD, BIAS>), LDS);
+    const hipError_t e = hk_lds_attr_once(attr_done, reinterpret_cast<const void*>(&hk_prefix_rows_kernel<HD, BIAS, GRP>), LDS);
     if (e != hipSuccess) {
         hk_set_error("hk_prefix_attn_bf16: hipFuncSetAttribute(%d B LDS): %s", LDS, hipGetErrorString(e));
         return HK_ELAUNCH;
     }
-    hipLaunchKernelGGL((hk_prefix_rows_kernel<HD, BIAS>), dim3((unsigned)rows_grid(p, m)), dim3(256), LDS, s, p, m.rows);
+    hipLaunchKernelGGL((hk_prefix_rows_kernel<HD, BIAS, GRP>), dim3((unsigned)rows_grid(p, m)), dim3(GRP * 256), LDS, s, p, m.rows);
     return HK_OK;
+}
+template <int HD, bool BIAS>
+int launch_rows(const PrefixParams& p, const Plan& m, hipStream_t s) {
+    return m.groups == 2 ? launch_rows_groups<HD, BIAS, 2>(p, m, s) : launch_rows_groups<HD, BIAS, 1>(p, m, s);
 }
 template <int HD, int SG>
 void launch_join(const PrefixParams& p, hipStream_t s) {

@@ -130,6 +130,13 @@ def test_prefix_attention_matches_its_definition(B, Nq, P, Nk, H, hd, kind):
         assert bool((got[-1] == 0).all())
 
 
+@pytest.mark.parametrize("B,Nq,P,Nk,H,hd,kind", [           # one workgroup for prefix and own keys: two groups of waves, and (last three) one
+    (2, 130, 300, 130, 6, 128, "left"), (1, 512, 333, 512, 5, 64, "add"), (3, 200, 0, 450, 4, 128, "all"), (1, 257, 0, 460, 8, 128, "holes"),
+    (4, 64, 385, 64, 16, 64, None), (2, 385, 0, 385, 3, 128, "left"), (3, 40, 100, 41, 90, 64, "left"), (2, 150, 200, 150, 70, 128, "add"), (5, 33, 64, 33, 60, 128, "all")])
+def test_prefix_attention_in_one_launch_of_row_blocks(B, Nq, P, Nk, H, hd, kind):
+    test_prefix_attention_matches_its_definition(B, Nq, P, Nk, H, hd, kind)
+
+
 def test_prefix_attention_large_scores_and_late_maximum():
     """Scores that grow along the keys by far more than the lazily moved maximum's 8 bits, up to 2^10 apart."""
     B, P, Nk, H, hd = 3, 400, 50, 2, 128
