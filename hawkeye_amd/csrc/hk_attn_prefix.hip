@@ -948,13 +948,14 @@ Plan make_plan(PrefixParams& p, int hd, bool raw) {
     p.norg = (p.Nq + m.rt * 16 - 1) / (m.rt * 16);
     const int64_t H = p.H, B = p.B;
     // One launch, a workgroup per (sequence, head) for all its keys, or chunks and a join?  Measured in a graph, 32 heads of 128 (us, one : two
-    // launches).  One sequence, 55 / 372 / 720 keys: 4.6 : 6.3, 7.3 : 6.8, 10.8 : 7.1 - and a launch costs the host 2.6.  The prefix is
+    // launches).  One sequence, 55 / 372 / 520 / 720 keys: 4.6 : 6.3, 7.3 : 6.8, 8.8 : 7.0, 10.8 : 7.1 - and the second launch and the workspace
+    // cost the host 4.3, so up to 1.5 are given for them.  The prefix is
     // read once per sequence here: 16 sequences over 352 + 20 keys 13.0 : 8.8.  Heads of 64, 55 / 520 / 700 / 907 keys: 4.0 : 5.8, 6.0 : 6.5, 6.9 : 6.6,
     // 8.0 : 6.7 (16 waves instead of eight: 0.2 more).  Without one nothing is read twice, and 256 pairs fill the
     // chip: 8 sequences' step over 353 / 1000 keys 11.3 : 15.8, 23.5 : 26.3; 4 sequences' over 1000 15.9 : 18.4, one's 13.7 : 8.0; 32 sequences'
     // over 100 20.7 : 16.6.
     const int64_t pairs = H * B, keys = (int64_t)p.P + p.Nk;
-    if (p.Nq <= 16 && (p.P > 0 ? pairs <= 256 && keys * hd <= 384 * 128 : pairs <= 512 && (keys <= 384 || (pairs >= 128 && keys <= MAX_CHUNK)))) {
+    if (p.Nq <= 16 && (p.P > 0 ? pairs <= 256 && keys * hd <= 480 * 128 : pairs <= 512 && (keys <= 384 || (pairs >= 128 && keys <= MAX_CHUNK)))) {
         m.mode = ONCE;
         m.rt = 1;
         p.norg = 1;
