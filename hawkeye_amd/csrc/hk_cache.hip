@@ -218,6 +218,7 @@ __global__ __launch_bounds__(GRP * 256, 2) void hk_key_weights_kernel(const KeyW
                     int lim = p.causal ? min(p.Nk - 1, q + off) : p.Nk - 1;                  // last key it sees
                     if (SUMS && q >= p.Nq) lim = -1;
                     lim -= (SUMS ? s0 : p0 + g * 32) + 4 * h;                                // register i: key (i & 3) + 8 (i >> 2) from here
+                    asm volatile("" : "+v"(lim));     // (left to itself the compiler makes the comparisons for every tile)
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
                         if ((i & 3) + 8 * (i >> 2) > lim) st[g][i] = -INFINITY;
