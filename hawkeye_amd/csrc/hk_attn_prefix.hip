@@ -971,6 +971,10 @@ Plan make_plan(PrefixParams& p, int hd, bool raw) {
         m.mode = again >= 9600000 ? MIXED : SMALL;
         if (m.mode == SMALL) p.npc = cut(p.P, H * p.nprg, PART_WANT, NWV * TK, MAX_CHUNK, &p.pc);
         else p.npc = cut_rows(p.P, H * m.rows.npb, &p.pc);
+        if (m.mode == MIXED && p.Nq <= 16) {               // 16 rows are enough for the own keys then
+            m.rt = 1;
+            p.norg = 1;
+        }
         p.noc = cut(p.Nk, B * H * p.norg, PART_WANT, NWV * TK, MAX_CHUNK, &p.oc);
     } else {
         // time of a 128-row x 64-key tile when 512 workgroups (two per CU) run: about 1 us; a lone workgroup's is not much shorter
