@@ -17,6 +17,7 @@
 // the loop).  The next tile's K is requested as soon as this one's scores stand, its V as soon as this one's is in LDS: a
 // wave keeps about 16 KB in flight, 8 waves per CU.  Bound by memory: 16 sequences' step over 1500 own keys each (398 MB) 80 us, 5.0 TB/s;
 // 64 sequences' over 512 own keys each beside the prefix 66 us.
+// Many sequences with few own keys each: a wave takes a sequence's keys alone (by_wave).
 // ONE: a workgroup of eight waves per (sequence, head) for all its keys, the prefix's tiles first; no chunks, no second launch, a step's scores
 // stay in LDS.  Bound by latency (a chain of dependent tiles per wave): one sequence over 353 keys 8 us, and the host needs 10 for the call.
 #include <type_traits>
@@ -45,6 +46,7 @@ struct PrefixParams {
     int pc, npc, nprg;               // prefix: keys per chunk, chunks, row groups
     int oc, noc, norg;               // own keys: the same, per sequence
     int ns;                          // slots of a row: npc + noc
+    int by_wave;                     // own keys: a (sequence, head, row group) per wave instead of per workgroup (noc = 1)
     int64_t pjobs;                   // workgroups of the prefix: H * npc * nprg (below 2^31 once checked)
 };
 
@@ -84,14 +86,14 @@ __global__ __launch_bounds__(NW * 64, 2) void hk_prefix_part_kernel(const Prefix
     __shared__ __attribute__((aligned(16))) float blds[BIAS ? MAX_CHUNK : 4];
     __shared__ __attribute__((aligned(16))) float rawl[ONE && RAW ? MAX_CHUNK : 4];
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l15 = lane & 15, quad = lane >> 4;
 
     // ---- which rows, which keys ----
     int head, row0, nrows, k0, k1, slot, lim0 = 0x3fffffff, brow = 0;
     const __bf16 *kb, *vb;
     int64_t ldk, ldv;
-    bool shared_keys;
+    bool shared_keys, alone = false, live = true;          // alone: this wave has keys and rows of its own, if live
     const int pA = ONE ? p.P : 0, nA = (pA + TK - 1) / TK;      // ONE: tiles [0, nA) are the prefix's, the own keys' follow
     if (!ONE && blockIdx.x < p.pjobs) {      // row groups of one (head, chunk) follow each other: the later ones find K and V in L2
         const int rg = blockIdx.x % p.nprg, hc = blockIdx.x / p.nprg;
@@ -108,6 +110,13 @@ __global__ __launch_bounds__(NW * 64, 2) void hk_prefix_part_kernel(const Prefix
         shared_keys = true;
     } else {
         int j = (int)(blockIdx.x - (ONE ? 0 : p.pjobs));
+        if (!ONE && !RAW && p.by_wave) {
+            const int jobs = p.B * p.H * p.norg;
+            alone = true;
+            j = j * NW + wave;
+            live = j < jobs;
+            j = min(j, jobs - 1);
+        }
         const int rg = j % p.norg;
         j /= p.norg;
         head = j % p.H;
@@ -129,9 +138,14 @@ __global__ __launch_bounds__(NW * 64, 2) void hk_prefix_part_kernel(const Prefix
         shared_keys = false;
     }
     const bool has_bias = BIAS && !shared_keys;
+    const float* bls = blds + (alone ? wave * (MAX_CHUNK / NW) : 0);
     if (has_bias) {
         const float* bp = p.bias + (int64_t)brow * p.bias_bs + (int64_t)head * p.bias_hs;
-        for (int i = tid; i < MAX_CHUNK && k0 + i < k1; i += NW * 64) blds[i] = bp[k0 + i];
+        if (alone) {
+            for (int i = lane; i < MAX_CHUNK / NW && k0 + i < k1; i += 64) blds[wave * (MAX_CHUNK / NW) + i] = bp[k0 + i];
+        } else {
+            for (int i = tid; i < MAX_CHUNK && k0 + i < k1; i += NW * 64) blds[i] = bp[k0 + i];
+        }
         __syncthreads();
     }
 
@@ -188,12 +202,13 @@ __global__ __launch_bounds__(NW * 64, 2) void hk_prefix_part_kernel(const Prefix
 #pragma unroll
     for (int d = 0; d < DT; ++d) toff[d] = trow * HD * 2 + (((2 * d + ((lane & 3) >> 1)) ^ swz(trow)) << 4) + 8 * (lane & 1);
 
-    const int nt = nA + (k1 > k0 ? (k1 - k0 + TK - 1) / TK : 0);
-    if (wave < nt) {
-        load_k(wave);
-        load_v(wave);
+    const int nt = live ? nA + (k1 > k0 ? (k1 - k0 + TK - 1) / TK : 0) : 0;
+    const int tf = alone ? 0 : wave, ts = alone ? 1 : NW;  // the wave's tiles: tf, tf + ts, ...
+    if (tf < nt) {
+        load_k(tf);
+        load_v(tf);
     }
-    for (int t = wave; t < nt; t += NW) {
+    for (int t = tf; t < nt; t += ts) {
         f32x4 st[RT][2];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
@@ -203,14 +218,14 @@ __global__ __launch_bounds__(NW * 64, 2) void hk_prefix_part_kernel(const Prefix
 #pragma unroll
                 for (int s = 0; s < KS; ++s) st[rt][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kr[g][s], qf[rt][s], st[rt][g], 0, 0, 0);
             }
-        const bool more = t + NW < nt;
-        if (more) load_k(t + NW);
+        const bool more = t + ts < nt;
+        if (more) load_k(t + ts);
         // ---- bias, removed and invisible keys ----
         const bool pre = ONE && t < nA;
         const int kt = pre ? t * TK : k0 + (t - nA) * TK, ke = pre ? pA : k1;
         uint32_t gone = 0;                                // keys of this tile that no row has: their V rows are made zero
         if (has_bias && !pre) {
-            const float* bl = blds + (t - nA) * TK;
+            const float* bl = bls + (t - nA) * TK;
             const bool rem = lane < TK && (kt + lane >= ke || bl[lane] <= REMOVED);
             gone = (uint32_t)__builtin_amdgcn_ballot_w64(rem);
 #pragma unroll
@@ -286,7 +301,7 @@ __global__ __launch_bounds__(NW * 64, 2) void hk_prefix_part_kernel(const Prefix
             *reinterpret_cast<u32x4*>(vw + r * HD * 2 + ((vch ^ swz(r)) << 4)) = vr[i];
         }
         wave_lds_sync();
-        if (more) load_v(t + NW);
+        if (more) load_v(t + ts);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
             const bf16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(vw + toff[d]));
@@ -319,6 +334,18 @@ __global__ __launch_bounds__(NW * 64, 2) void hk_prefix_part_kernel(const Prefix
     }
     __syncthreads();
     constexpr int TPR = HD / 4;                            // threads per row, four dims each
+    if (alone) {
+        for (int r = lane / TPR; live && r < nrows; r += 64 / TPR) {
+            const int c = lane % TPR;
+            const int64_t at = ((int64_t)(row0 + r) * p.H + head) * p.ns + slot;
+            *reinterpret_cast<f32x4*>(p.part_o + at * HD + 4 * c) = *reinterpret_cast<const f32x4*>(ow + r * HD + ((c ^ (r & 7)) << 2));
+            if (c == 0) {
+                p.part_ml[at * 2] = ml[wave][r][0];
+                p.part_ml[at * 2 + 1] = ml[wave][r][1];
+            }
+        }
+        return;
+    }
     for (int r = tid / TPR; r < nrows; r += NW * 64 / TPR) {
         const int c = tid % TPR;
         float M = ml[0][r][0];
@@ -349,7 +376,8 @@ __global__ __launch_bounds__(NW * 64, 2) void hk_prefix_part_kernel(const Prefix
             p.part_ml[at * 2] = M;
             p.part_ml[at * 2 + 1] = ls;
         }
-    }    if (ONE && RAW) {                                      // the weights of the one row
+    }
+    if (ONE && RAW) {                                      // the weights of the one row
         float M = ml[0][0][0], ls = 0.f;
 #pragma unroll
         for (int w = 1; w < NW; ++w) M = fmaxf(M, ml[w][0][0]);
@@ -976,6 +1004,10 @@ Plan make_plan(PrefixParams& p, int hd, bool raw) {
             p.norg = 1;
         }
         p.noc = cut(p.Nk, B * H * p.norg, PART_WANT, NWV * TK, MAX_CHUNK, &p.oc);
+        // Own keys by wave: nothing of a workgroup is idle where they are few, but a wave walks them alone.  By workgroup : by wave, 32 heads of 128, prefix of
+        // 1985 (us): 16 sequences' 20 / 61 / 100 own keys 14.1 : 13.7, 15.3 : 15.3, 16.6 : 17.6, 32 sequences' 21.6 : 17.3, 22.1 : 19.9, 25.0 : 24.3, 64
+        // sequences' 35 : 28, 36 : 33, 41 : 40; 128 own keys 43 : 44; heads of 64, 32 sequences' 14.1 : 11.7, 14.3 : 12.4, 15.5 : 14.5.
+        p.by_wave = !raw && p.noc == 1 && p.Nk <= 96 && B * H * p.norg >= 1024;
     } else {
         // time of a 128-row x 64-key tile when 512 workgroups (two per CU) run: about 1 us; a lone workgroup's is not much shorter
         p.npc = cut_rows(p.P, H * m.rows.npb, &p.pc);
@@ -1012,7 +1044,10 @@ void set_parts(PrefixParams& p, void* ws, int hd) {
     p.part_o = reinterpret_cast<float*>(ws);
     p.part_ml = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + up16((size_t)p.ns * p.R * p.H * hd * 4));
 }
-int64_t part_grid(const PrefixParams& p) { return p.ns == 0 ? (int64_t)p.B * p.H : p.pjobs + (int64_t)p.B * p.noc * p.H * p.norg; }
+int64_t part_grid(const PrefixParams& p) {
+    const int64_t own = (int64_t)p.B * p.H * p.norg;
+    return p.ns == 0 ? (int64_t)p.B * p.H : p.pjobs + (p.by_wave ? (own + NWV - 1) / NWV : own * p.noc);
+}
 int64_t rows_grid(const PrefixParams& p, const Plan& m) {
     const int64_t own = (int64_t)p.B * m.rows.nob * p.H;
     return m.mode == MIXED ? m.rows.pjobs : m.mode == PACKED ? m.rows.pjobs + own * p.noc : own;

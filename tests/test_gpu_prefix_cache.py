@@ -137,6 +137,13 @@ def test_prefix_attention_in_one_launch_of_row_blocks(B, Nq, P, Nk, H, hd, kind)
     test_prefix_attention_matches_its_definition(B, Nq, P, Nk, H, hd, kind)
 
 
+@pytest.mark.parametrize("B,Nq,P,Nk,H,hd,kind", [           # many sequences with few own keys: a wave per (sequence, head)
+    (33, 1, 500, 61, 32, 64, "left"), (130, 1, 400, 20, 9, 128, "add"), (70, 3, 300, 33, 15, 64, "holes"), (40, 20, 200, 70, 30, 128, "all"),
+    (257, 1, 33, 96, 5, 128, "left"), (1030, 1, 700, 1, 1, 64, None), (26, 1, 2100, 97, 40, 128, "left"), (128, 2, 6000, 31, 9, 128, "holes")])
+def test_prefix_attention_of_many_short_sequences(B, Nq, P, Nk, H, hd, kind):
+    test_prefix_attention_matches_its_definition(B, Nq, P, Nk, H, hd, kind)
+
+
 def test_prefix_attention_large_scores_and_late_maximum():
     """Scores that grow along the keys by far more than the lazily moved maximum's 8 bits, up to 2^10 apart."""
     B, P, Nk, H, hd = 3, 400, 50, 2, 128
