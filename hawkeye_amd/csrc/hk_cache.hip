@@ -535,10 +535,11 @@ __device__ __forceinline__ uint32_t rank_of(float w, bool removed, bool recent) 
 
 // Kept rows within one (sequence, head), walked upwards by a workgroup of T threads.  Row `at` comes from src(at) >= at, so a step's stores
 // can only hit sources of the same or an earlier step: all of a step's loads have arrived before its first store.  Not in place: copied.
-template <int HD, int T, typename Src>
-__device__ __forceinline__ void move_rows(const EvictParams& p, int b, int head, bool is_v, Src src) {
-    constexpr int CH = HD / 8, RPS = T / CH, U = 8;
-    const int col = head * HD + ((int)threadIdx.x % CH) * 8, g = threadIdx.x / CH;
+// (W of the head's HD values, from w0 on: what different workgroups move does not meet.)
+template <int HD, int T, int W, typename Src>
+__device__ __forceinline__ void move_rows(const EvictParams& p, int b, int head, bool is_v, int w0, Src src) {
+    constexpr int CH = W / 8, RPS = T / CH, U = 8;
+    const int col = head * HD + w0 + ((int)threadIdx.x % CH) * 8, g = threadIdx.x / CH;
     const __bf16* from = is_v ? p.V + (int64_t)b * p.bsv + col : p.K + (int64_t)b * p.bsk + col;
     __bf16* to = is_v ? p.VO + (int64_t)b * p.bsvo + col : p.KO + (int64_t)b * p.bsko + col;
     const int64_t ldf = is_v ? p.ldv : p.ldk, ldt = is_v ? p.ldvo : p.ldko;
@@ -668,8 +669,8 @@ __global__ __launch_bounds__(T) void hk_evict_kernel(const EvictParams p) {
     if (MOVE) {
         __syncthreads();
         auto src = [&](int at) { return (int)rows[at]; };
-        move_rows<HD, T>(p, b, head, false, src);
-        move_rows<HD, T>(p, b, head, true, src);
+        move_rows<HD, T, HD>(p, b, head, false, 0, src);
+        move_rows<HD, T, HD>(p, b, head, true, 0, src);
     }
 }
 
@@ -828,12 +829,13 @@ __global__ __launch_bounds__(256) void hk_evict_copy_kernel(const EvictParams p)
         }
 }
 
-// Rows within the cache, the kept list in memory: one workgroup per (sequence, head, K or V).
-template <int HD>
+// Rows within the cache, the kept list in memory: a workgroup per (sequence, head, K or V, W values of the head).
+template <int HD, int W>
 __global__ __launch_bounds__(512) void hk_evict_move_kernel(const EvictParams p) {
-    const int bh = blockIdx.x >> 1, b = bh / p.H, head = bh - b * p.H;
+    constexpr int N = HD / W;
+    const int bh = blockIdx.x / (2 * N), part = blockIdx.x % (2 * N), b = bh / p.H, head = bh - b * p.H;
     const int32_t* kept = p.kept + (int64_t)bh * p.budget;
-    move_rows<HD, 512>(p, b, head, blockIdx.x & 1, [&](int at) { return kept[at]; });
+    move_rows<HD, 512, W>(p, b, head, part & 1, (part >> 1) * W, [&](int at) { return kept[at]; });
 }
 
 template <int T, int KPT, int HD, bool MOVE>
@@ -855,15 +857,19 @@ int launch_evict_all(const EvictParams& p, hipStream_t s) {
     // One launch or two?  A workgroup per pair moves its rows in pieces of one head; the copy kernel writes whole rows with the whole chip
     // (5.5 TB/s against 4.6) and costs a launch (2.6 us of the host's).  One : two, heads of 128 (us).  Budget 256 of 353: 9.5 : 9.2 (32 pairs),
     // 11.3 : 12.1 (128), 24.5 : 28.5 (512); 500 of 1000: 15.7 : 11.7, 20.0 : 20.0, 51.3 : 52.7; 1024 of 2047: 26 : 15, 31 : 31, 118 : 113; 8000 of
-    // 16000: 200 : 66, 312 : 217.  Heads of 64, 1024 of 2047: 17 : 13 (32 pairs), 28 : 32 (256), 60 : 59 (512).  In place only the pair's own
-    // workgroup knows when a row may be overwritten.
+    // 16000: 200 : 66, 312 : 217.  Heads of 64, 1024 of 2047: 17 : 13 (32 pairs), 28 : 32 (256), 60 : 59 (512).
     const int64_t bytes = (int64_t)p.budget * HD * 2;
     const bool one = bytes <= (pairs < 128 ? 64 << 10 : 128 << 10);
-    if (p.n <= REG_KEYS && (p.in_place || one)) return launch_evict_any<HD, true>(p, s);
+    // In place, rows may only move within what one workgroup walks, but slices of the head's values are apart: few pairs spread over the CUs by
+    // slices of 32, and many lose by their 64-byte pieces.  One : two launches, 1024 of 2047 rows 14.0 : 12.7 (32 pairs), 18.1 : 21.2 (64), 23.5 : 33.4 (128);
+    // 8000 of 16000 97 : 63 (32), 201 : 253 (128); 500 of 1000 8.9 : 8.2 (32).
+    const bool sliced = pairs <= 32;
+    if (p.n <= REG_KEYS && (p.in_place ? one || !sliced : one)) return launch_evict_any<HD, true>(p, s);
     if (p.n <= REG_KEYS) launch_evict_any<HD, false>(p, s);
     else hipLaunchKernelGGL(hk_evict_select_kernel, dim3(pairs), dim3(SEL_T), 0, s, p);
     if (p.in_place) {
-        hipLaunchKernelGGL((hk_evict_move_kernel<HD>), dim3(pairs * 2), dim3(512), 0, s, p);
+        if (sliced) hipLaunchKernelGGL((hk_evict_move_kernel<HD, 32>), dim3(pairs * 2 * (HD / 32)), dim3(512), 0, s, p);
+        else hipLaunchKernelGGL((hk_evict_move_kernel<HD, HD>), dim3(pairs * 2), dim3(512), 0, s, p);
     } else {
         const int64_t pieces = (int64_t)p.B * p.H * p.budget, per = 256 / (HD / 8) * 2;
         HK_REQUIRE((pieces + per - 1) / per < (1LL << 31), "hk_cache_evict_bf16: grid too large");

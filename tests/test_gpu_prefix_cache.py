@@ -302,6 +302,11 @@ def test_cache_evict_keeps_the_heaviest_rows(B, n, budget, recent, H, hd, masked
         assert torch.equal(k, k0) and torch.equal(v, v0) and torch.equal(w.view(torch.int32), w0.view(torch.int32))
 
 
+@pytest.mark.parametrize("inplace", [False, True])
+def test_cache_evict_of_many_long_caches(inplace):
+    test_cache_evict_keeps_the_heaviest_rows(1, 16400, 60, 7, 34, 64, True, inplace)
+
+
 # ---------------------------------------------------------------- the paths that use them: prompts that continue a prefix, bounded caches
 def _llm(seed, **kw):
     from dataclasses import replace
