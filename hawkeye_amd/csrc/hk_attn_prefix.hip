@@ -274,7 +274,7 @@ __global__ __launch_bounds__(NW * 64, 2) void hk_prefix_part_kernel(const Prefix
                     for (int i = 0; i < 4; ++i) ot[rt][d][i] *= a;
             }
         }
-        // P in bf16 (the matrix instruction's operand): half a step of 2^-9 each; the sum l is of the unrounded values
+        // P in bf16 (the matrix instruction's operand): half a step each, 2^-8 of the value; the sum l is of the unrounded values
         bf16x8 pf[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
