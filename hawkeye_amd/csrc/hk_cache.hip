@@ -455,11 +455,13 @@ bool few_keys(int64_t Nq, int64_t Nk, bool causal) {
     const int64_t nqb = (Nq + 31) / 32, nkb = (Nk + 31) / 32;
     return Nk <= 384 && nqb * nkb - (causal ? nqb * (nqb - 1) / 2 : 0) <= 96;
 }
+// Whole multiples of 64 bytes: the sums of a few rows could otherwise come to HK_NO_WS, which says that there are none.
 size_t key_weights_bytes(int64_t B, int64_t H, int64_t Nq, int Nk, bool causal) {
+    static_assert(HK_NO_WS % 64 != 0, "a workspace's size must not be the value that stands for none");
     if (few_keys(Nq, Nk, causal)) return HK_NO_WS;
     int ct;
     const int nch = key_chunks((Nq + BLK - 1) / BLK * B * H, Nk, &ct);
-    return (size_t)(B * H * Nq) * (nch > 1 ? 8 * nch + 4 : 4);
+    return ((size_t)(B * H * Nq) * (nch > 1 ? 8 * nch + 4 : 4) + 63) / 64 * 64;
 }
 
 template <int HD, bool SUMS, bool BIAS, int GRP>
@@ -903,7 +905,7 @@ extern "C" int hk_attn_key_weights_bf16(const hk_key_weights_desc* d, void* stre
     HK_REQUIRE(d->w_in != d->w_out || (d->wi_bs == d->wo_bs && d->wi_hs == d->wo_hs),
                "hk_attn_key_weights_bf16: weights updated in place must have one layout");
     const size_t need = key_weights_bytes(d->B, d->H, d->Nq, d->Nk, d->causal != 0);
-    const bool few = need == HK_NO_WS;
+    const bool few = few_keys(d->Nq, d->Nk, d->causal != 0);
     HK_REQUIRE(few || (d->ws && d->ws_bytes >= need), "hk_attn_key_weights_bf16: workspace of %zu bytes, %zu needed (hk_attn_key_weights_ws)",
                d->ws ? d->ws_bytes : (size_t)0, need);
     {

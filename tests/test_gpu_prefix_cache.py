@@ -554,3 +554,9 @@ def test_streams_graphs_and_strides():
     assert bool((kept[..., -20:] == torch.arange(rows - 20, rows, device=DEV)).all()) and bool((kept >= rows - n).all())
     src = (kept.long() - (rows - n)).transpose(1, 2)[..., None].expand(-1, -1, -1, hd)
     assert torch.equal(big[:, :50].unflatten(2, (H, hd)), kk.unflatten(2, (H, hd)).gather(1, src))
+
+
+@pytest.mark.parametrize("B,Nq,Nk,H,hd,causal,kind", [      # keys too many for one launch, too few for chunks, few rows: the smallest workspaces
+    (1, 1, 400, 4, 64, True, None), (2, 1, 400, 2, 128, True, "left"), (1, 4, 385, 1, 128, True, None), (4, 1, 430, 1, 64, False, "holes"), (1, 1, 448, 4, 128, True, "add")])
+def test_attn_key_weights_with_the_smallest_workspaces(B, Nq, Nk, H, hd, causal, kind):
+    test_attn_key_weights_matches_its_definition(B, Nq, Nk, H, hd, causal, kind)

@@ -116,3 +116,27 @@ def test_wrappers_refuse_tensors_that_are_not_on_the_gpu():
         ops.prefix_attention(t.expand(1, 2, 2, 64), t[0], t[0], t, t)
     with pytest.raises(RuntimeError, match="budget"):
         ops.cache_evict(t, t, w, 1, 2)
+
+
+# keys too many for one launch, too few for chunks, and so few rows that their sums' bytes are few
+@pytest.mark.parametrize("B,H,Nq,Nk", [(1, 4, 1, 400), (2, 2, 1, 400), (1, 1, 4, 385), (1, 4, 1, 448), (1, 1, 1, 385), (1, 5, 1, 400), (4, 1, 1, 430)])
+def test_attn_key_weights_of_few_rows_need_their_workspace(B, H, Nq, Nk):
+    need = L.load().hk_attn_key_weights_ws(B, H, Nq, Nk, 1)
+    assert need != L.HK_NO_WS and need >= 4 * B * H * Nq
+    row = H * 64
+    kw = dict(B=B, H=H, Nq=Nq, Nk=Nk, ldq=row, bsq=row * Nq, ldk=row, bsk=row * Nk, wo_bs=H * Nk, wo_hs=Nk)
+    _refused(_weights(ws=None, **kw), "workspace")
+    _refused(_weights(ws_bytes=need - 1, **kw), "workspace")
+    _refused(_weights(ws=3 * A, ws_bytes=need, **kw), "overlaps the workspace")
+
+
+def test_no_real_workspace_has_the_size_that_stands_for_none():
+    lib = L.load()
+    for B in (1, 2, 3, 8):
+        for H in (1, 2, 4, 5):
+            for Nq in (1, 2, 4, 33):
+                for Nk in (33, 384, 385, 400, 448, 449, 1000, 1500, 5000):
+                    row, few = H * 64, lib.hk_attn_key_weights_ws(B, H, Nq, Nk, 1) == L.HK_NO_WS
+                    assert few == (Nk <= 384), (B, H, Nq, Nk)
+                    if not few:
+                        _refused(_weights(ws=None, B=B, H=H, Nq=Nq, Nk=Nk, ldq=row, bsq=row * Nq, ldk=row, bsk=row * Nk, wo_bs=H * Nk, wo_hs=Nk), "workspace")
