@@ -1151,7 +1151,7 @@ extern "C" int hk_prefix_attn_bf16(const hk_prefix_attn_desc* d, void* stream) {
     HK_REQUIRE(d->ldkp < (1 << 25) && d->ldvp < (1 << 25) && d->ldk < (1 << 25) && d->ldv < (1 << 25),
                "hk_prefix_attn_bf16: token strides of 2^25 elements and more are not supported");
     HK_REQUIRE(d->ldq >= 0 && d->ldkp >= 0 && d->ldvp >= 0 && d->ldk >= 0 && d->ldv >= 0 && d->bsq >= 0 && d->bsk >= 0 && d->bsv >= 0 &&
-                   (d->Nq == 1 || d->ldo >= row) && (d->B == 1 || d->bso >= row) && d->bias_bs >= 0,
+                   hk_rows_apart(d->B, d->bso, d->Nq, d->ldo, row) && d->bias_bs >= 0,
                "hk_prefix_attn_bf16: strides must not be negative, output rows must not overlap");
     HK_REQUIRE(((uintptr_t)d->Q | (uintptr_t)d->KP | (uintptr_t)d->VP | (uintptr_t)d->K | (uintptr_t)d->V | (uintptr_t)d->ws) % 16 == 0 &&
                    (uintptr_t)d->O % 8 == 0 && (uintptr_t)d->key_bias % 4 == 0,
@@ -1222,8 +1222,7 @@ extern "C" int hk_decode_attn_weights_bf16(const hk_step_weights_desc* d, void* 
     HK_REQUIRE(((uintptr_t)d->q | (uintptr_t)d->k_cache | (uintptr_t)d->v_cache | (uintptr_t)d->ws) % 16 == 0 && (uintptr_t)d->out % 8 == 0 &&
                    ((uintptr_t)d->w_in | (uintptr_t)d->w_out | (uintptr_t)d->key_bias) % 4 == 0,
                "hk_decode_attn_weights_bf16: operands must be 16-byte aligned");
-    HK_REQUIRE((d->H == 1 || d->wo_hs >= d->n_keys) && (d->B == 1 || d->wo_bs >= (d->H - 1) * d->wo_hs + d->n_keys) && d->wi_bs >= 0 &&
-                   d->wi_hs >= 0 && d->bias_bs >= 0 && d->bias_hs >= 0,
+    HK_REQUIRE(hk_rows_apart(d->B, d->wo_bs, d->H, d->wo_hs, d->n_keys) && d->wi_bs >= 0 && d->wi_hs >= 0 && d->bias_bs >= 0 && d->bias_hs >= 0,
                "hk_decode_attn_weights_bf16: rows of w_out must not overlap, strides must not be negative");
     HK_REQUIRE(d->w_in != d->w_out || (d->wi_bs == d->wo_bs && d->wi_hs == d->wo_hs),
                "hk_decode_attn_weights_bf16: weights updated in place must have one layout");

@@ -899,8 +899,7 @@ extern "C" int hk_attn_key_weights_bf16(const hk_key_weights_desc* d, void* stre
     HK_REQUIRE(((uintptr_t)d->Q | (uintptr_t)d->K | (uintptr_t)d->ws) % 16 == 0 &&
                    ((uintptr_t)d->key_bias | (uintptr_t)d->w_in | (uintptr_t)d->w_out) % 4 == 0,
                "hk_attn_key_weights_bf16: operands must be 16-byte aligned");
-    HK_REQUIRE((d->H == 1 || d->wo_hs >= d->Nk) && (d->B == 1 || d->wo_bs >= (d->H - 1) * d->wo_hs + d->Nk) && d->wi_bs >= 0 && d->wi_hs >= 0 &&
-                   d->bias_bs >= 0,
+    HK_REQUIRE(hk_rows_apart(d->B, d->wo_bs, d->H, d->wo_hs, d->Nk) && d->wi_bs >= 0 && d->wi_hs >= 0 && d->bias_bs >= 0,
                "hk_attn_key_weights_bf16: rows of w_out must not overlap, strides must not be negative");
     HK_REQUIRE(d->w_in != d->w_out || (d->wi_bs == d->wo_bs && d->wi_hs == d->wo_hs),
                "hk_attn_key_weights_bf16: weights updated in place must have one layout");
@@ -961,8 +960,6 @@ extern "C" int hk_cache_evict_bf16(const hk_cache_evict_desc* d, void* stream) {
     HK_REQUIRE(((d->ldk | d->bsk | d->ldv | d->bsv | d->ldko | d->bsko | d->ldvo | d->bsvo) & 7) == 0 && d->ldk >= 0 && d->bsk >= 0 && d->ldv >= 0 &&
                    d->bsv >= 0 && d->w_bs >= 0 && d->w_hs >= 0 && d->b_bs >= 0 && d->b_hs >= 0,
                "hk_cache_evict_bf16: strides must be multiples of 8 elements, not negative");
-    HK_REQUIRE(d->ldko >= row && d->ldvo >= row && (d->B == 1 || (d->bsko >= row && d->bsvo >= row)),
-               "hk_cache_evict_bf16: output rows must not overlap");
     HK_REQUIRE(((uintptr_t)d->K | (uintptr_t)d->V | (uintptr_t)d->k_out | (uintptr_t)d->v_out) % 16 == 0 &&
                    ((uintptr_t)d->weight | (uintptr_t)d->weight_out | (uintptr_t)d->key_bias | (uintptr_t)d->key_bias_out | (uintptr_t)d->kept) % 4 == 0,
                "hk_cache_evict_bf16: caches must be 16-byte aligned");
@@ -974,9 +971,10 @@ extern "C" int hk_cache_evict_bf16(const hk_cache_evict_desc* d, void* stream) {
     HK_REQUIRE(!in_place || (d->ldk == d->ldko && d->bsk == d->bsko && d->ldv == d->ldvo && d->bsv == d->bsvo && d->w_bs == d->wo_bs &&
                              d->w_hs == d->wo_hs && d->b_bs == d->bo_bs && d->b_hs == d->bo_hs),
                "hk_cache_evict_bf16: in place, input and output must have one layout");
-    const int64_t wlen = in_place ? d->n_keys : d->budget;
-    HK_REQUIRE((d->H == 1 || d->wo_hs >= wlen) && (d->B == 1 || d->wo_bs >= (d->H - 1) * d->wo_hs + wlen) &&
-                   (d->key_bias == nullptr || ((d->H == 1 || d->bo_hs >= wlen) && (d->B == 1 || d->bo_bs >= (d->H - 1) * d->bo_hs + wlen))),
+    const int64_t wlen = in_place ? d->n_keys : d->budget;       // in place, what one sequence writes another must not read either
+    HK_REQUIRE(hk_rows_apart(d->B, d->bsko, wlen, d->ldko, row) && hk_rows_apart(d->B, d->bsvo, wlen, d->ldvo, row),
+               "hk_cache_evict_bf16: output rows must not overlap");
+    HK_REQUIRE(hk_rows_apart(d->B, d->wo_bs, d->H, d->wo_hs, wlen) && (d->key_bias == nullptr || hk_rows_apart(d->B, d->bo_bs, d->H, d->bo_hs, wlen)),
                "hk_cache_evict_bf16: rows of the weights and biases written must not overlap");
     {
         const HkSpan out[] = {hk_span(d->k_out, d->B, d->bsko, d->budget, d->ldko, row, 2), hk_span(d->v_out, d->B, d->bsvo, d->budget, d->ldvo, row, 2),

@@ -89,6 +89,12 @@ static inline HkSpan hk_span(const void* ptr, int64_t n1, int64_t s1, int64_t n2
 }
 static inline bool hk_overlap(HkSpan x, HkSpan y) { return x.a < y.b && y.a < x.b; }
 
+// Rows of `row` elements at i1 * s1 + i2 * s2 (i1 < n1, i2 < n2) that a call writes: no two share an element, the one index within the other's steps.
+static inline bool hk_rows_apart(int64_t n1, int64_t s1, int64_t n2, int64_t s2, int64_t row) {
+    if ((n1 > 1 && s1 < row) || (n2 > 1 && s2 < row)) return false;
+    return n1 <= 1 || n2 <= 1 || s1 >= (n2 - 1) * s2 + row || s2 >= (n1 - 1) * s1 + row;
+}
+
 #define HK_REQUIRE(cond, ...)            \
     do {                                 \
         if (!(cond)) {                   \

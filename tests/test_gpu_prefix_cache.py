@@ -560,3 +560,25 @@ def test_streams_graphs_and_strides():
     (1, 1, 400, 4, 64, True, None), (2, 1, 400, 2, 128, True, "left"), (1, 4, 385, 1, 128, True, None), (4, 1, 430, 1, 64, False, "holes"), (1, 1, 448, 4, 128, True, "add")])
 def test_attn_key_weights_with_the_smallest_workspaces(B, Nq, Nk, H, hd, causal, kind):
     test_attn_key_weights_matches_its_definition(B, Nq, Nk, H, hd, causal, kind)
+
+
+def test_outputs_in_other_orders_of_their_dims():
+    """Tokens outside sequences, heads outside sequences: the results of the plain layouts."""
+    B, Nq, P, Nk, H, hd = 3, 5, 600, 40, 4, 64
+    q, kp, vp = _rand((B, Nq, H, hd), 1, 0.2), _rand((P, H, hd), 2), _rand((P, H, hd), 3)
+    k, v = _rand((B, Nk, H, hd), 4), _rand((B, Nk, H, hd), 5)
+    out = torch.full((Nq, B, H, hd), 7.0, dtype=torch.bfloat16, device=DEV)
+    want = ops.prefix_attention(q, kp, vp, k, v)
+    assert torch.equal(ops.prefix_attention(q, kp, vp, k, v, out=out.transpose(0, 1)), want)
+    w = ops.attn_key_weights(q, k)
+    wt = torch.zeros((H, B, Nk), device=DEV)
+    assert torch.equal(ops.attn_key_weights(q, k, weight_out=wt.transpose(0, 1)), w)
+    kc, vc, q1 = k.reshape(B, Nk, H * hd), v.reshape(B, Nk, H * hd), q[:, 0].reshape(B, H * hd).contiguous()
+    w2 = w.clone()
+    o = ops.decode_attn_weights(q1, kc, vc, Nk, H, hd, w2)
+    assert torch.equal(ops.decode_attn_weights(q1, kc, vc, Nk, H, hd, wt.transpose(0, 1)), o) and torch.equal(wt.transpose(0, 1), w2)
+    ko, vo = torch.empty((11, B, H, hd), dtype=torch.bfloat16, device=DEV), torch.empty((11, B, H, hd), dtype=torch.bfloat16, device=DEV)
+    wo = torch.empty((H, B, 11), device=DEV)
+    kept = ops.cache_evict(k, v, wt.transpose(0, 1), Nk, 11, 3, out=(ko.transpose(0, 1), vo.transpose(0, 1), wo.transpose(0, 1), None))
+    assert torch.equal(ops.cache_evict(k, v, w2, Nk, 11, 3), kept)            # in place
+    assert torch.equal(ko.transpose(0, 1), k[:, :11]) and torch.equal(vo.transpose(0, 1), v[:, :11]) and torch.equal(wo.transpose(0, 1), w2[..., :11])

@@ -140,3 +140,13 @@ def test_no_real_workspace_has_the_size_that_stands_for_none():
                     assert few == (Nk <= 384), (B, H, Nq, Nk)
                     if not few:
                         _refused(_weights(ws=None, B=B, H=H, Nq=Nq, Nk=Nk, ldq=row, bsq=row * Nq, ldk=row, bsk=row * Nk, wo_bs=H * Nk, wo_hs=Nk), "workspace")
+
+
+@pytest.mark.parametrize("call,kw,text", [          # rows of different sequences (or tokens) that share elements, though each stride alone holds a row
+    (_prefix, dict(Nq=3, ldo=128, bso=128), "rows must not overlap"), (_prefix, dict(Nq=3, ldo=256, bso=384), "rows must not overlap"),
+    (_evict, dict(bsko=128), "rows must not overlap"), (_evict, dict(bsvo=384), "rows must not overlap"), (_evict, dict(B=3, ldko=256, bsko=128), "rows must not overlap"),
+    (_evict, dict(k_out=A, v_out=2 * A, weight_out=5 * A, ldko=128, bsk=128 * 4, bsko=128 * 4, bsvo=128 * 9, wo_bs=18, wo_hs=9), "rows must not overlap"),
+    (_step, dict(wo_hs=16, wo_bs=16), "w_out must not overlap"), (_weights, dict(wo_hs=9, wo_bs=9), "w_out must not overlap"),
+    (_evict, dict(wo_bs=4, wo_hs=4), "written must not overlap"), (_evict, dict(key_bias=8 * A, key_bias_out=9 * A, b_bs=18, b_hs=9, bo_bs=4, bo_hs=4), "written must not overlap")])
+def test_outputs_whose_rows_share_elements_are_refused(call, kw, text):
+    _refused(call(**kw), text)
