@@ -186,13 +186,16 @@ __global__ __launch_bounds__(GRP * 256, 2) void hk_key_weights_kernel(const KeyW
         }
         for (bool take = !SUMS && pending;; take = true) { // STATS: a second time if a partial sum left the range; SUMS: once
             f32x16 st[2];                                  // the half tiles' products: two independent chains
+            // The products start from -m only where they are of its size: added to a reference point far away, or one that biases make large, they
+            // would lose bits at every step.  base: what the biases, added afterwards, are taken relative to.
+            const float base = SUMS || take ? 0.f : m, start = plain ? -base : 0.f;
 #pragma unroll
             for (int s = 0; s < NKS; ++s)
 #pragma unroll
                 for (int g = 0; g < 2; ++g) {
                     if (s == 0) {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) st[g][i] = SUMS ? 0.f : -m;
+                        for (int i = 0; i < 16; ++i) st[g][i] = SUMS ? 0.f : start;
                     }
                     const bf16x8 pf = *reinterpret_cast<const bf16x8*>(ts + g * 32 * ROWB + (ro ^ (32 * s)));
                     st[g] = SUMS ? __builtin_amdgcn_mfma_f32_32x32x16_bf16(sf[s], pf, st[g], 0, 0, 0)
@@ -207,7 +210,7 @@ __global__ __launch_bounds__(GRP * 256, 2) void hk_key_weights_kernel(const KeyW
                             st[g][i] = kb[i] == -INFINITY ? -INFINITY : st[g][i] + kb[i];
                         } else {
                             const float v = sd[g * 32 + 4 * h + (i & 3) + 8 * (i >> 2)];
-                            st[g][i] = v <= REMOVED ? -INFINITY : st[g][i] + v * HK_LOG2E;
+                            st[g][i] = v <= REMOVED ? -INFINITY : st[g][i] + fmaf(v, HK_LOG2E, -base);
                         }
                     }
             }
@@ -237,15 +240,15 @@ __global__ __launch_bounds__(GRP * 256, 2) void hk_key_weights_kernel(const KeyW
                 float mx = fmaxf(st[0][0], st[1][0]);
 #pragma unroll
                 for (int i = 1; i < 16; ++i) mx = fmaxf(mx, fmaxf(st[0][i], st[1][i]));
-                const float delta = unset ? (mx == -INFINITY ? 0.f : mx) : fmaxf(mx, 0.f);
-                l *= unset ? 0.f : __builtin_amdgcn_exp2f(-delta);
+                const float mn = unset ? (mx == -INFINITY ? 0.f : mx) : fmaxf(m, mx);
+                l *= unset ? 0.f : __builtin_amdgcn_exp2f(m - mn);
                 unset = unset && mx == -INFINITY;
                 pending = __builtin_amdgcn_ballot_w64(unset) != 0;
-                m += delta;
+                m = mn;
 #pragma unroll
                 for (int g = 0; g < 2; ++g)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) st[g][i] -= delta;
+                    for (int i = 0; i < 16; ++i) st[g][i] -= mn;
             }
             float rs = 0.f;
 #pragma unroll

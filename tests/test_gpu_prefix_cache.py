@@ -582,3 +582,37 @@ def test_outputs_in_other_orders_of_their_dims():
     kept = ops.cache_evict(k, v, wt.transpose(0, 1), Nk, 11, 3, out=(ko.transpose(0, 1), vo.transpose(0, 1), wo.transpose(0, 1), None))
     assert torch.equal(ops.cache_evict(k, v, w2, Nk, 11, 3), kept)            # in place
     assert torch.equal(ko.transpose(0, 1), k[:, :11]) and torch.equal(vo.transpose(0, 1), v[:, :11]) and torch.equal(wo.transpose(0, 1), w2[..., :11])
+
+
+def _deep(B, n, first, seed):
+    """Biases of about -9000 (far below all scores, and still there) on the first `first` keys, 0 on the others."""
+    b = torch.zeros((B, n), device=DEV)
+    b[:, :first] = -9000.0 + _rand((B, first), seed, 2.0, torch.float32)
+    return b
+
+
+# Two sizes of reference points in one row.  A row that sees an ordinary key has nothing left of the others: the tolerance is the usual one.  (Few
+# ordinary keys and queries: errors of many would cancel.)
+@pytest.mark.parametrize("B,Nq,Nk,H,hd,causal,first", [
+    (2, 3, 460, 4, 128, True, 448), (3, 2, 700, 5, 64, False, 690), (2, 7, 500, 3, 128, False, 450), (70, 2, 450, 5, 64, True, 440), (2, 5, 5000, 2, 128, True, 4990),
+    (40, 3, 700, 64, 128, False, 699), (2, 500, 700, 70, 64, True, 150), (2, 100, 300, 2, 128, True, 100), (1, 20, 100, 2, 64, False, 70)])
+def test_attn_key_weights_behind_keys_with_large_biases(B, Nq, Nk, H, hd, causal, first):
+    q, k = _rand((B, Nq, H, hd), 1, 0.05 * hd ** -0.5), _rand((B, Nk, H, hd), 2)
+    # (small scores: a small d)
+    bias = _deep(B, Nk, first, 3)
+    got = ops.attn_key_weights(q, k, key_bias=bias, causal=causal)
+    p, d = _ref_weights(q, k, bias, causal)
+    ref = p.sum(2)
+    _near(got, ref, ref * (2 * d + (Nq + 128) * 2.0 ** -24) + Nq * 1e-37)
+
+
+# A row that sees biased keys alone: its scores lie below 2^14 and are held in 32 bits with the bias in them, 2^-11 for each of five roundings (the
+# product with log2 e, the addition, in both passes; the row's sum).
+@pytest.mark.parametrize("B,Nq,Nk,H,hd,first", [(2, 500, 500, 2, 128, 300), (1, 130, 600, 2, 64, 600), (2, 100, 100, 3, 128, 50), (1, 30, 3000, 1, 64, 3000)])
+def test_attn_key_weights_of_rows_with_large_biases_alone(B, Nq, Nk, H, hd, first):
+    q, k = _rand((B, Nq, H, hd), 1, 1.5 * hd ** -0.5 * LOG2E), _rand((B, Nk, H, hd), 2)
+    bias = _deep(B, Nk, first, 3)
+    got = ops.attn_key_weights(q, k, key_bias=bias)
+    p, d = _ref_weights(q, k, bias, True)
+    ref = p.sum(2)
+    _near(got, ref, ref * (2 * d + (Nq + 128) * 2.0 ** -24 + 5 * math.log(2.0) * 2.0 ** -11) + Nq * 1e-37)
