@@ -557,11 +557,12 @@ __global__ __launch_bounds__(GRP * 256, 2) void hk_prefix_rows_kernel(const Pref
             const char* ks = gs + cur * STAGE;
             const char* vs = ks + KT * ROWB;
             uint64_t gone = 0;                             // keys of this tile that no row has
-            bool biased = false;
+            bool biased = false, added = false;            // some key is biased or removed / some key that stays is biased
             if (BIAS && own) {
                 const float v = blds[cur * KT + lane];
                 gone = __builtin_amdgcn_ballot_w64(kt + lane >= n || v <= REMOVED);
                 biased = __builtin_amdgcn_ballot_w64(v != 0.f) != 0;
+                added = __builtin_amdgcn_ballot_w64(v != 0.f && !(v <= REMOVED)) != 0;
             }
             const bool edge = kt + KT > n || (own && kt + KT - 1 > q0 + off);
             f32x16 st[2];
@@ -656,27 +657,35 @@ __global__ __launch_bounds__(GRP * 256, 2) void hk_prefix_rows_kernel(const Pref
             if (from < 64) {
                 // ends, diagonals, biases, rows without a key so far, scores that outgrew m: the tile as a whole, masks and all
                 float rs;
-                auto scores = [&]() __attribute__((always_inline)) {
+                // base: what the scores are relative to.  The products start from it only where they are of its size: added to a reference point far
+                // away, or one that biases make large, they would lose bits at every step.
+                auto scores = [&](float base) __attribute__((always_inline)) {
+                    int kz = ko, bz = cur * KT + 4 * h;
+                    uint64_t gz = gone;
+                    asm volatile("" : "+v"(kz), "+v"(bz), "+s"(gz));        // read again each time: kept, the fragments, biases and masks of a tile fill the registers
                     f32x16 c0;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) c0[i] = -m;
+                    for (int i = 0; i < 16; ++i) c0[i] = BIAS && biased ? 0.f : -base;
 #pragma unroll
                     for (int s = 0; s < NKS; ++s)              // two independent chains
 #pragma unroll
-                        for (int g = 0; g < 2; ++g) st[g] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kread(g * NKS + s), qf[s], s == 0 ? c0 : st[g], 0, 0, 0);
+                        for (int g = 0; g < 2; ++g)
+                            st[g] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(ks + g * 32 * ROWB + (kz ^ (32 * s))), qf[s],
+                                                                            s == 0 ? c0 : st[g], 0, 0, 0);
                     if (BIAS && biased) {                      // register 4 x + j of st[g] <-> key 32 g + 8 x + 4 h + j
 #pragma unroll
                         for (int g = 0; g < 2; ++g)
 #pragma unroll
                             for (int x = 0; x < 4; ++x) {
-                                const f32x4 bv = *reinterpret_cast<const f32x4*>(blds + cur * KT + 32 * g + 8 * x + 4 * h);
-                                const uint32_t gb = (uint32_t)(gone >> (32 * g + 8 * x)) >> (4 * h);
+                                const f32x4 bv = *reinterpret_cast<const f32x4*>(blds + bz + 32 * g + 8 * x);
+                                const uint32_t gb = (uint32_t)(gz >> (32 * g + 8 * x)) >> (4 * h);
 #pragma unroll
-                                for (int j = 0; j < 4; ++j) st[g][4 * x + j] = (gb >> j) & 1 ? -INFINITY : st[g][4 * x + j] + bv[j] * HK_LOG2E;
+                                for (int j = 0; j < 4; ++j) st[g][4 * x + j] = (gb >> j) & 1 ? -INFINITY : st[g][4 * x + j] + fmaf(bv[j], HK_LOG2E, -base);
                             }
                     }
                     if (edge || from) {
-                        const int lim = min(n - 1, own ? q0 + r + off : n - 1) - kt - 4 * h;
+                        int lim = min(n - 1, own ? q0 + r + off : n - 1) - kt - 4 * h;
+                        asm volatile("" : "+v"(lim));
 #pragma unroll
                         for (int g = 0; g < 2; ++g)
 #pragma unroll
@@ -700,20 +709,16 @@ __global__ __launch_bounds__(GRP * 256, 2) void hk_prefix_rows_kernel(const Pref
 #pragma unroll
                     for (int i = 1; i < 16; ++i) mx = fmaxf(mx, fmaxf(st[0][i], st[1][i]));
                     mx = half_max(mx);
-                    const float delta = unset ? (mx == -INFINITY ? 0.f : mx) : fmaxf(mx, 0.f);
-                    const float a = unset ? 0.f : __builtin_amdgcn_exp2f(-delta);
+                    const float mn = unset ? (mx == -INFINITY ? 0.f : mx) : fmaxf(m, mx);
+                    const float a = unset ? 0.f : __builtin_amdgcn_exp2f(m - mn);
                     unset = unset && mx == -INFINITY;
                     pending = __builtin_amdgcn_ballot_w64(unset) != 0;
-                    m += delta;
+                    m = mn;
                     l *= a;
 #pragma unroll
                     for (int d = 0; d < NDT; ++d)
 #pragma unroll
                         for (int i = 0; i < 16; ++i) ot[d][i] *= a;
-#pragma unroll
-                    for (int g = 0; g < 2; ++g)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) st[g][i] -= delta;
                 };
                 auto pv = [&](const bf16x8* pf, auto masked_c) __attribute__((always_inline)) {
 #pragma unroll
@@ -736,8 +741,18 @@ __global__ __launch_bounds__(GRP * 256, 2) void hk_prefix_rows_kernel(const Pref
                     }
                 };
                 for (bool take = pending || plain;; take = true) {      // at most twice
-                    scores();
-                    if (take) move_max();
+                    scores(take ? 0.f : m);
+                    if (take) {
+                        move_max();
+                        if (BIAS && added) {               // once more, relative to the new m: beside their biases the scores have lost bits
+                            scores(m);
+                        } else {
+#pragma unroll
+                            for (int g = 0; g < 2; ++g)
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) st[g][i] -= m;
+                        }
+                    }
                     exp_sum();
                     if (take || __builtin_amdgcn_ballot_w64(!(rs <= OVERFLOW_SUM)) == 0) break;
                 }

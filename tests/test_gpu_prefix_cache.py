@@ -616,3 +616,20 @@ def test_attn_key_weights_of_rows_with_large_biases_alone(B, Nq, Nk, H, hd, firs
     p, d = _ref_weights(q, k, bias, True)
     ref = p.sum(2)
     _near(got, ref, ref * (2 * d + (Nq + 128) * 2.0 ** -24 + 5 * math.log(2.0) * 2.0 ** -11) + Nq * 1e-37)
+
+
+
+# Questions whose own keys all carry large biases, or begin with them: what the biases have in common drops out of a softmax, and takes no bit along.
+@pytest.mark.parametrize("B,Nq,P,Nk,H,hd,first,rest", [
+    (2, 70, 0, 200, 3, 128, 1e5, 1e5), (3, 130, 300, 130, 4, 64, 1e5, 1e5), (2, 40, 0, 400, 90, 128, 1e5, 1e5), (1, 257, 0, 460, 8, 64, 3e4, 1e5), (2, 100, 64, 300, 2, 128, -9000.0, 0.0),
+    (1, 64, 0, 3000, 1, 64, 1e5, 1e5)])
+def test_prefix_attention_of_questions_with_large_biases(B, Nq, P, Nk, H, hd, first, rest):
+    q, kp, vp = _rand((B, Nq, H, hd), 1, 1.5 * hd ** -0.5 * LOG2E), _rand((P, H, hd), 2), _rand((P, H, hd), 3)
+    k, v = _rand((B, Nk, H, hd), 4), _rand((B, Nk, H, hd), 5)
+    bias = torch.full((B, Nk), float(rest), device=DEV)
+    bias[:, :Nk - Nq - 1] = float(first)
+    bias += _rand((B, Nk), 6, 2.0, torch.float32)
+    v[..., ::2] = 3.0 * torch.sign(q[:1, :1, :, ::2]) + v[..., ::2]           # (outputs far from zero)
+    got = ops.prefix_attention(q, kp, vp, k, v, key_bias=bias)
+    ref, tol = _ref_prefix(q, kp, vp, k, v, bias)
+    _near(got, ref, tol)
