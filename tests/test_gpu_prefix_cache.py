@@ -633,3 +633,32 @@ def test_prefix_attention_of_questions_with_large_biases(B, Nq, P, Nk, H, hd, fi
     got = ops.prefix_attention(q, kp, vp, k, v, key_bias=bias)
     ref, tol = _ref_prefix(q, kp, vp, k, v, bias)
     _near(got, ref, tol)
+
+
+# Steps and a few tokens: P is two bf16 numbers, off by 2^-16 of itself.  What is left beside the output's own rounding: scores (d), sums of n terms in
+# 32 bits in numerator and denominator, exp2 of the terms, chunks and waves (2^-20 covers eight of them).
+def _near_32(got, ref, A, d, n):
+    _near(got, ref, 2.0 ** -8 * ref.abs() + 1.01 * A * (2.0 ** -16 + 2 * d + 2 * (n + 64) * 2.0 ** -24 + 2.0 ** -20) + 1e-37)
+
+
+@pytest.mark.parametrize("B,Nq,P,Nk,H,hd,kind", [
+    (4, 1, 352, 20, 32, 128, None), (16, 1, 1985, 61, 8, 128, "left"), (16, 1, 1985, 61, 8, 128, None), (5, 3, 777, 130, 12, 64, "add"), (1, 1, 5000, 300, 4, 128, "holes"),
+    (4, 16, 1500, 16, 4, 64, None), (3, 1, 0, 90, 4, 128, "left"), (40, 1, 100, 33, 3, 128, "left"), (2, 32, 300, 32, 3, 64, None)])
+def test_steps_keep_the_bits_of_their_probabilities(B, Nq, P, Nk, H, hd, kind):
+    q, kp, vp = _rand((B, Nq, H, hd), 1, 0.2 * hd ** -0.5 * LOG2E), _rand((P, H, hd), 2), _rand((P, H, hd), 3)
+    k, v, bias = _rand((B, Nk, H, hd), 4), _rand((B, Nk, H, hd), 5), _bias(kind, B, Nk, 6)
+    got = ops.prefix_attention(q, kp, vp, k, v, key_bias=bias)
+    p = _softmax(_h(q), [_h(kp[None]).expand(B, -1, -1, -1), _h(k)], [None, None if bias is None else bias.double()[:, None, None]], Nq)
+    vs = torch.cat([_h(vp[None]).expand(B, -1, -1, -1), _h(v)], 2)
+    d = _d(_h(q), [_h(kp[None]).expand(B, -1, -1, -1), _h(k)], hd)
+    _near_32(got.transpose(1, 2), p @ vs, p @ vs.abs(), d, P + Nk)
+
+
+@pytest.mark.parametrize("B,n,H,hd,kind", [(1, 353, 8, 128, None), (4, 1500, 4, 128, "left"), (2, 1500, 4, 128, None), (3, 700, 5, 64, "add"), (1, 9000, 2, 64, None)])
+def test_weighted_steps_keep_the_bits_of_their_probabilities(B, n, H, hd, kind):
+    q = _rand((B, H * hd), 1, 0.2 * hd ** -0.5 * LOG2E)
+    k, v, bias = _rand((B, n, H * hd), 2), _rand((B, n, H * hd), 3), _bias(kind, B, n, 4)
+    out = ops.decode_attn_weights(q, k, v, n, H, hd, torch.zeros((B, H, n), device=DEV), key_bias=bias)
+    p, d = _ref_weights(q.view(B, 1, H, hd), k.view(B, n, H, hd), bias, False)
+    vd = _h(v.view(B, n, H, hd))
+    _near_32(out.view(B, H, hd), (p @ vd)[:, :, 0], (p @ vd.abs())[:, :, 0], d, n)
