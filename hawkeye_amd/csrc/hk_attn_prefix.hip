@@ -1283,7 +1283,7 @@ extern "C" int hk_decode_attn_weights_bf16(const hk_step_weights_desc* d, void* 
                      w = hk_span(p.ns ? d->ws : nullptr, 1, 0, 1, 0, (int64_t)need, 1);
         const HkSpan in[] = {hk_span(p.Q, p.B, D, 1, 0, D, 2), hk_span(p.K, p.B, p.bsk, p.Nk, D, D, 2), hk_span(p.V, p.B, p.bsv, p.Nk, D, D, 2),
                              hk_span(p.bias, p.B, p.bias_bs, p.H, p.bias_hs, p.Nk, 4),
-                             d->w_in == d->w_out ? HkSpan{0, 0} : hk_span(d->w_in, p.B, d->wi_bs, p.H, d->wi_hs, p.Nk, 4)};
+                             d->w_in == d->w_out ? HkSpan{} : hk_span(d->w_in, p.B, d->wi_bs, p.H, d->wi_hs, p.Nk, 4)};
         for (int i = 0; i < 5; ++i)
             HK_REQUIRE(!hk_overlap(wo, in[i]) && !hk_overlap(o, in[i]) && !hk_overlap(w, in[i]),
                        "hk_decode_attn_weights_bf16: an output or the workspace overlaps an input");

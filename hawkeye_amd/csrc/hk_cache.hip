@@ -915,7 +915,7 @@ extern "C" int hk_attn_key_weights_bf16(const hk_key_weights_desc* d, void* stre
         const HkSpan wo = hk_span(d->w_out, d->B, d->wo_bs, d->H, d->wo_hs, d->Nk, 4), w = hk_span(few ? nullptr : d->ws, 1, 0, 1, 0, (int64_t)need, 1);
         const HkSpan in[] = {hk_span(d->Q, d->B, d->bsq, d->Nq, d->ldq, row, 2), hk_span(d->K, d->B, d->bsk, d->Nk, d->ldk, row, 2),
                              hk_span(d->key_bias, d->B, d->bias_bs, 1, 0, d->Nk, 4),
-                             d->w_in == d->w_out ? HkSpan{0, 0} : hk_span(d->w_in, d->B, d->wi_bs, d->H, d->wi_hs, d->Nk, 4)};
+                             d->w_in == d->w_out ? HkSpan{} : hk_span(d->w_in, d->B, d->wi_bs, d->H, d->wi_hs, d->Nk, 4)};
         for (int i = 0; i < 4; ++i)
             HK_REQUIRE(!hk_overlap(wo, in[i]) && !hk_overlap(w, in[i]), "hk_attn_key_weights_bf16: the output or the workspace overlaps an input");
         HK_REQUIRE(!hk_overlap(wo, w), "hk_attn_key_weights_bf16: the output overlaps the workspace");

@@ -721,7 +721,7 @@ def cache_evict(k: torch.Tensor, v: torch.Tensor, weight: torch.Tensor, n_keys: 
     or less, rank below all; NaN below numbers) move, in ascending order, to rows [0, budget), with their weights and biases.
     Returns kept int32 [B,H,budget], the rows they came from.  1 <= budget <= n_keys, 0 <= recent <= budget.
     out None: in place (weights and biases of rows [budget, n_keys) become 0); out = (k_out, v_out, weight_out, key_bias_out or None):
-    other tensors that overlap no input, rows behind budget left alone.  key_bias fp32 [B,H,>=n_keys]: per head, as heads keep different rows."""
+    other tensors that overlap no input, rows behind budget left alone.  k and v may be views of one tensor.  key_bias fp32 [B,H,>=n_keys]: per head, as heads keep different rows."""
     ko, vo, wo, bo = (k, v, weight, key_bias) if out is None else out
     n_keys, budget, recent = index(n_keys), index(budget), index(recent)
     key = (k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device, weight.shape, weight.stride(), weight.dtype, weight.device,

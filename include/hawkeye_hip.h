@@ -499,6 +499,7 @@ size_t hk_attn_key_weights_ws(int32_t B, int32_t H, int32_t Nq, int32_t Nk, int3
  * Removed keys (bias -1e4 or less) rank below all others, NaN weights below numbers; -0 equals 0.  0 <= recent <= budget <= n_keys, budget >= 1.
  * The output is the input itself (every pointer and stride the same; weights and biases of rows [budget, n_keys) become 0, K and V
  * there keep what they held) or other memory that overlaps none of it (rows behind budget are left alone).
+ * K and V may be interleaved in one tensor ([B, rows, 2, H, hd] or [B, 2, rows, H, hd]).
  * K / V [B, rows, H, hd] through strides ld*, bs*; weights [B, H, rows] through (w_bs, w_hs) in and (wo_bs, wo_hs) out; biases, which
  * are per head here because heads keep different rows, through (b_bs, b_hs) and (bo_bs, bo_hs), or both NULL. */
 typedef struct hk_cache_evict_desc {

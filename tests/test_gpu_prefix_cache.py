@@ -662,3 +662,39 @@ def test_weighted_steps_keep_the_bits_of_their_probabilities(B, n, H, hd, kind):
     p, d = _ref_weights(q.view(B, 1, H, hd), k.view(B, n, H, hd), bias, False)
     vd = _h(v.view(B, n, H, hd))
     _near_32(out.view(B, H, hd), (p @ vd)[:, :, 0], (p @ vd.abs())[:, :, 0], d, n)
+
+
+@pytest.mark.parametrize("form", ["rows", "blocks", "qkv"])
+@pytest.mark.parametrize("B,n,budget,H,hd", [(2, 300, 100, 3, 64), (3, 700, 513, 2, 128), (12, 1500, 900, 3, 128), (1, 17000, 300, 2, 64)])
+def test_cache_evict_of_interleaved_caches(form, B, n, budget, H, hd):
+    """K and V as views of one tensor, in place and into views of one tensor: the results of two tensors."""
+    rows = n + 2
+    kv = _rand((B, 2, rows, H, hd) if form == "blocks" else (B, rows, 2 if form == "rows" else 3, H, hd), 1)
+    k, v = (kv[:, 0], kv[:, 1]) if form == "blocks" else (kv[:, :, -2], kv[:, :, -1])
+    w = _rand((B, H, rows), 3, 1.0, torch.float32).abs()
+    k1, v1, w1, kv0 = k.clone(), v.clone(), w.clone(), kv.clone()
+    want = ops.cache_evict(k1, v1, w1, n, budget, 20)
+    new = torch.full((B, 2, budget + 1, H, hd) if form == "blocks" else (B, budget + 1, 2, H, hd), 7.0, dtype=torch.bfloat16, device=DEV)
+    ko, vo = (new[:, 0], new[:, 1]) if form == "blocks" else (new[:, :, 0], new[:, :, 1])
+    wo = torch.empty((B, H, budget), device=DEV)
+    assert torch.equal(ops.cache_evict(k, v, w, n, budget, 20, out=(ko, vo, wo, None)), want)
+    assert torch.equal(kv, kv0)
+    for a, b, c in ((ko, k1, vo), (vo, v1, ko)):
+        assert torch.equal(a[:, :budget], b[:, :budget]) and bool((a[:, budget:] == 7.0).all())
+    assert torch.equal(wo, w1[..., :budget])
+    assert torch.equal(ops.cache_evict(k, v, w, n, budget, 20), want)
+    assert torch.equal(k, k1) and torch.equal(v, v1) and torch.equal(w, w1)
+    if form == "qkv":
+        assert torch.equal(kv[:, :, 0], kv0[:, :, 0])
+
+
+def test_prefix_attention_into_a_column_of_its_inputs_tensor():
+    B, n, H, hd = 3, 40, 2, 128
+    x = _rand((B, n, 4, H, hd), 1, 0.3)
+    kp, vp = _rand((500, H, hd), 2), _rand((500, H, hd), 3)
+    x0 = x.clone()
+    want = ops.prefix_attention(x0[:, :, 0], kp, vp, x0[:, :, 1], x0[:, :, 2])
+    got = ops.prefix_attention(x[:, :, 0], kp, vp, x[:, :, 1], x[:, :, 2], out=x[:, :, 3])
+    assert torch.equal(got, want) and torch.equal(x[:, :, :3], x0[:, :, :3])
+    with pytest.raises(RuntimeError, match="overlaps an input"):
+        ops.prefix_attention(x[:, :, 0], kp, vp, x[:, :, 1], x[:, :, 2], out=x[:, :, 2])

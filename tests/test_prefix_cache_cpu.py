@@ -150,3 +150,17 @@ def test_no_real_workspace_has_the_size_that_stands_for_none():
     (_evict, dict(wo_bs=4, wo_hs=4), "written must not overlap"), (_evict, dict(key_bias=8 * A, key_bias_out=9 * A, b_bs=18, b_hs=9, bo_bs=4, bo_hs=4), "written must not overlap")])
 def test_outputs_whose_rows_share_elements_are_refused(call, kw, text):
     _refused(call(**kw), text)
+
+
+KV = dict(K=A, V=A + 256, ldk=256, bsk=256 * 9, ldv=256, bsv=256 * 9)                              # [B, 9, 2, 2, 64]: rows of 256 bytes, side by side
+SAME = dict(k_out=A, v_out=A + 256, weight_out=5 * A, ldko=256, bsko=256 * 9, ldvo=256, bsvo=256 * 9, wo_bs=18, wo_hs=9)
+
+
+@pytest.mark.parametrize("kw,text", [               # interleaved, and a piece into each other; interleaved with another period
+    (dict(KV, **dict(SAME, v_out=A + 240, V=A + 240)), "an output overlaps an input"), (dict(KV, **dict(SAME, V=A + 272, v_out=A + 272)), "an output overlaps an input"),
+    (dict(KV, **dict(SAME, ldv=264, bsv=264 * 9, ldvo=264, bsvo=264 * 9)), "an output overlaps an input"), (dict(KV, k_out=A + 128, ldko=256, bsko=256 * 9), "an output overlaps an input"),
+    (dict(KV, **dict(SAME, bsv=256 * 9 + 128, bsvo=256 * 9 + 128)), "an output overlaps an input"), (dict(k_out=3 * A, v_out=3 * A + 128, ldko=256, ldvo=256, bsko=1024, bsvo=1024), "two outputs overlap"),
+    (dict(KV, k_out=A + 512 * 18 - 256, v_out=4 * A, ldko=256, bsko=1024), "an output overlaps an input"),
+    (dict(k_out=3 * A, v_out=3 * A + 128 * 2 * 3, bsko=1024, bsvo=1024), "two outputs overlap")])
+def test_interleaved_caches_that_meet_are_refused(kw, text):
+    _refused(_evict(**kw), text)
