@@ -698,3 +698,62 @@ def test_prefix_attention_into_a_column_of_its_inputs_tensor():
     assert torch.equal(got, want) and torch.equal(x[:, :, :3], x0[:, :, :3])
     with pytest.raises(RuntimeError, match="overlaps an input"):
         ops.prefix_attention(x[:, :, 0], kp, vp, x[:, :, 1], x[:, :, 2], out=x[:, :, 2])
+
+
+# What the cases above leave out of the rules that pick a kernel.  Questions of a usual prompt without padding (two groups of waves, and one), heads
+# of 64 with biases in two groups; rows of more than 16 sequences' tokens over row blocks with the own keys by workgroup; steps over a long prefix with
+# heads of 64; many sequences without a prefix.
+@pytest.mark.parametrize("B,Nq,P,Nk,H,hd,kind", [
+    (1, 37, 352, 37, 32, 128, None), (4, 64, 352, 64, 8, 128, None), (8, 128, 352, 128, 32, 128, None), (1, 64, 352, 64, 16, 64, "add"), (3, 130, 352, 130, 8, 64, "left"), (2, 257, 64, 257, 3, 64, "left"),
+    (8, 130, 200, 130, 2, 64, "add"), (3, 33, 200, 33, 3, 128, None), (2, 257, 0, 257, 70, 128, None), (1, 100, 0, 500, 4, 64, "all"), (2, 200, 2000, 200, 2, 64, None), (32, 16, 1600, 40, 4, 128, None), (32, 16, 1600, 40, 4, 128, "left"), (16, 32, 1600, 40, 6, 128, None),
+    (16, 32, 1600, 40, 6, 128, "holes"), (32, 16, 2100, 130, 8, 64, None), (32, 16, 2100, 130, 8, 64, "add"), (16, 25, 3000, 200, 8, 64, None), (16, 25, 3000, 200, 8, 64, "all"),
+    (40, 16, 1300, 30, 26, 64, None), (40, 16, 1300, 30, 26, 64, "left"), (40, 16, 600, 30, 26, 128, None), (33, 17, 800, 17, 20, 128, None), (5, 3, 1500, 40, 6, 64, None),
+    (5, 3, 1500, 40, 6, 64, "left"), (40, 1, 0, 40, 30, 128, "all"), (40, 1, 0, 90, 30, 128, None), (60, 3, 0, 33, 20, 64, "left"), (60, 1, 0, 33, 20, 64, None),
+    (40, 5, 0, 500, 20, 64, "holes"), (3, 1, 1500, 40, 8, 128, None)])
+def test_prefix_attention_by_every_rule(B, Nq, P, Nk, H, hd, kind):
+    test_prefix_attention_matches_its_definition(B, Nq, P, Nk, H, hd, kind)
+
+
+@pytest.mark.parametrize("B,Nq,Nk,H,hd,causal,kind", [      # without biases: two launches of one group and of two, chunks, one launch of up to 256 keys
+    (2, 450, 450, 45, 128, True, None), (2, 450, 450, 45, 64, True, None), (1, 1000, 1000, 2, 64, True, None), (2, 40, 3000, 2, 64, True, None), (1, 600, 600, 4, 64, False, None),
+    (2, 200, 250, 2, 128, True, None), (1, 256, 256, 3, 64, True, None), (64, 400, 400, 8, 128, True, None)])
+def test_attn_key_weights_without_biases(B, Nq, Nk, H, hd, causal, kind):
+    test_attn_key_weights_matches_its_definition(B, Nq, Nk, H, hd, causal, kind)
+
+
+@pytest.mark.parametrize("B,n,budget,recent,H,hd,masked", [      # many rows per workgroup: several ordered steps, where more than 32 pairs move them in place
+    (2, 576, 512, 128, 20, 128, True), (2, 576, 512, 128, 20, 128, False), (1, 2048, 1900, 5, 34, 64, True), (2, 600, 200, 9, 2, 128, True), (2, 1000, 500, 3, 3, 64, False), (2, 512, 400, 3, 3, 64, True),
+    (2, 2500, 1500, 7, 20, 128, True), (2, 2500, 200, 7, 2, 128, False), (1, 3000, 2500, 0, 3, 64, False), (1, 5000, 3000, 7, 34, 64, False), (1, 6000, 4500, 100, 33, 128, True),
+    (1, 13000, 200, 9, 2, 128, True), (1, 9000, 4000, 0, 3, 128, False)])
+@pytest.mark.parametrize("inplace", [False, True])
+def test_cache_evict_of_many_rows(B, n, budget, recent, H, hd, masked, inplace):
+    test_cache_evict_keeps_the_heaviest_rows(B, n, budget, recent, H, hd, masked, inplace)
+
+
+@pytest.mark.parametrize("B,n,budget,recent,H,hd,masked,inplace", [(1, 16500, 3000, 7, 34, 64, False, True), (1, 16400, 2100, 0, 33, 128, True, True)])
+def test_cache_evict_of_many_rows_of_many_long_caches(B, n, budget, recent, H, hd, masked, inplace):
+    test_cache_evict_keeps_the_heaviest_rows(B, n, budget, recent, H, hd, masked, inplace)
+
+
+def test_prefix_attention_in_a_workspace_of_the_callers():
+    """Of exactly the size asked for, between guards; too small, of another type, strided: refused."""
+    for B, Nq, P, Nk, H, hd in ((16, 1, 1985, 61, 4, 128), (7, 37, 1201, 37, 8, 128), (32, 16, 1600, 40, 4, 128), (5, 3, 1500, 40, 6, 64)):
+        need = ops.prefix_attention_ws(B, H, Nq, P, Nk, hd)
+        assert need > 64
+        q, kp, vp = _rand((B, Nq, H, hd), 1, 0.1), _rand((P, H, hd), 2), _rand((P, H, hd), 3)
+        k, v = _rand((B, Nk, H, hd), 4), _rand((B, Nk, H, hd), 5)
+        buf = torch.full((need + 512,), 255, dtype=torch.uint8, device=DEV)                   # (as floats: NaN)
+        want = ops.prefix_attention(q, kp, vp, k, v)
+        for _ in range(2):
+            assert torch.equal(ops.prefix_attention(q, kp, vp, k, v, ws=buf[256:256 + need]), want)
+            assert bool((buf[:256] == 255).all()) and bool((buf[256 + need:] == 255).all())
+        with pytest.raises(RuntimeError, match="workspace"):
+            ops.prefix_attention(q, kp, vp, k, v, ws=buf[256:256 + need - 1])
+        with pytest.raises(RuntimeError, match="uint8"):
+            ops.prefix_attention(q, kp, vp, k, v, ws=torch.empty((need,), device=DEV))
+        with pytest.raises(RuntimeError, match="uint8"):
+            ops.prefix_attention(q, kp, vp, k, v, ws=torch.empty((2 * need,), dtype=torch.uint8, device=DEV)[::2])
+    q = _rand((4, 1, 4, 128), 1, 0.1)
+    kp, k = _rand((300, 4, 128), 2), _rand((4, 20, 4, 128), 4)                                # one launch: whatever is passed is left alone
+    buf = torch.full((64,), 255, dtype=torch.uint8, device=DEV)
+    assert torch.equal(ops.prefix_attention(q, kp, kp, k, k, ws=buf), ops.prefix_attention(q, kp, kp, k, k)) and bool((buf == 255).all())
