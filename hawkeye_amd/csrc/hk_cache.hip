@@ -850,7 +850,8 @@ int launch_evict(const EvictParams& p, hipStream_t s) {
 }
 template <int HD, bool MOVE>
 int launch_evict_any(const EvictParams& p, hipStream_t s) {
-    if (p.n <= 512) return launch_evict<256, 2, HD, MOVE>(p, s);
+    if constexpr (MOVE || HD == 128)       // (heads of 64 move so few rows in the same launch, always)
+        if (p.n <= 512) return launch_evict<256, 2, HD, MOVE>(p, s);
     // moving rows wants more in flight than selecting them: 500 of 1000 keys, 256 : 512 threads 11.9 : 8.9 us (32 pairs, in place), 20.1 : 17.3 (128 pairs)
     if (p.n <= 2048) return launch_evict<MOVE ? 512 : 256, MOVE ? 4 : 8, HD, MOVE>(p, s);
     if (p.n <= 4096) return launch_evict<512, 8, HD, MOVE>(p, s);
