@@ -22,6 +22,7 @@
 // stay in LDS.  Bound by latency (a chain of dependent tiles per wave): one sequence over 353 keys 8 us, and the host needs 10 for the call.
 #include <type_traits>
 #include "hk_common.h"
+#include "hk_overlap.h"
 
 namespace {
 

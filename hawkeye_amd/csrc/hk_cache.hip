@@ -2,6 +2,7 @@
 // of the keys with the most weight to the front of the cache.
 #include <type_traits>
 #include "hk_common.h"
+#include "hk_overlap.h"
 
 namespace {
 

@@ -226,22 +226,27 @@ def load() -> C.CDLL:
     return lib
 
 
-def source_digest() -> str:
-    """sha1 over the kernel sources and the header the library is built from, comments and white space removed:
-    profiles taken with another kernel tree (profiles/traffic.json) are recognised as stale by it, while a note added
-    to a comment does not orphan them."""
-    import glob
+# what encode_img's kernels are compiled from
+ENCODE_SOURCES = ("hk_attn.hip", "hk_common.h", "hk_gemm.hip", "hk_input.hip", "hk_norm.hip")
+
+
+def source_digest(csrc: str = os.path.join(_HERE, "csrc")) -> str:
+    """sha1 over the sources of encode_img's kernels, comments and white space removed, and the flags they are compiled with: profiles of
+    that path taken with other kernels (profiles/traffic.json) are recognised as stale by it, while a note added to a comment
+    or another path's kernel does not orphan them."""
     import hashlib
     import re
     h = hashlib.sha1()
-    files = sorted(glob.glob(os.path.join(_HERE, "csrc", "*.hip")) + glob.glob(os.path.join(_HERE, "csrc", "*.h")))
-    files.append(os.path.join(os.path.dirname(_HERE), "include", "hawkeye_hip.h"))
-    for f in files:
-        text = open(f, "r", errors="replace").read()
+    for name in ENCODE_SOURCES:
+        text = open(os.path.join(csrc, name), "r", errors="replace").read()
         text = re.sub(r"/\*.*?\*/", " ", text, flags=re.S)      # block comments
         text = re.sub(r"//[^\n]*", " ", text)                   # line comments (no '//' occurs inside a string here)
-        h.update(os.path.basename(f).encode())
+        h.update(name.encode())
         h.update(" ".join(text.split()).encode())
+    objs = [n.replace(".hip", ".o") for n in ENCODE_SOURCES]
+    for line in open(os.path.join(csrc, "Makefile")):
+        if re.match(r"(ARCH|CXXFLAGS)\s*\??=", line) or ("CXXFLAGS +=" in line and any(o in line.split(":")[0].split() for o in objs)):
+            h.update(" ".join(line.split()).encode())
     return h.hexdigest()[:16]
 
 
