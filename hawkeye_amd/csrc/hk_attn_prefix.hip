@@ -416,6 +416,9 @@ __global__ __launch_bounds__(NW * 64, HD == 128 && RT == 1 && !BIAS && !ONE ? 3 
 // GRP = 2: two such groups of waves share a workgroup, each with stages of its own, and take every other tile; the second's (m, l, o) joins the
 // first's through LDS at the end (where CUs would be idle: make_plan).
 // A tile with nothing to mask goes by halves, the second half's products among the first half's exponentials.
+// TWO: P as two bf16 numbers, as in hk_prefix_part_kernel, for steps (MIXED, Nq = 1), which reading bounds: one : two (us, in a graph), 64 sequences
+// over 16384 + 333 keys 129.3 : 130.2, 128 over 2000 + 20 32.1 : 33.8.  One, off by 2^-8, for questions, as in hk_flash_attn_bf16: the feed of the
+// matrix unit bounds those (32 x 16 tokens over 1600 39.2 : 44.4).
 // Measured (32 heads of 128): 8 sequences of 512 rows over 1400 shared keys and their own 120 us, 930 TFLOP/s; the matrix unit is busy half of
 // the time.  Copies of the loop without one part, in-bounds and for timing only: without LDS-DMA and barriers 107-116 us, without the reads of
 // K from LDS 84, without those of V too 79, without exp2 101: bound by feeding the matrix unit from LDS (each wave reads every tile), at the clock that the
@@ -438,7 +441,7 @@ __device__ __forceinline__ float half_max(float x) {    // the larger of the two
     return fmaxf(a, b);
 }
 
-template <int HD, bool BIAS, int GRP>
+template <int HD, bool BIAS, int GRP, bool TWO>
 __global__ __launch_bounds__(GRP * 256, 2) void hk_prefix_rows_kernel(const PrefixParams p, const RowsParams q) {
     constexpr int ROWB = HD * 2, CH = HD / 8, NKS = HD / 16, NDT = HD / 32;
     constexpr int STAGE = 2 * KT * ROWB;
@@ -598,6 +601,14 @@ __global__ __launch_bounds__(GRP * 256, 2) void hk_prefix_rows_kernel(const Pref
                 }
                 return vf;
             };
+            auto rest = [&](int s, bf16x8 hi) __attribute__((always_inline)) {      // what rounding left of the values in piece s of P
+                const u32x4 w = __builtin_bit_cast(u32x4, hi);
+                u32x4 x;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    x[j] = pack_bf16x2(st[s >> 1][8 * (s & 1) + 2 * j] - bf16_lo(w[j]), st[s >> 1][8 * (s & 1) + 2 * j + 1] - bf16_hi(w[j]));
+                return __builtin_bit_cast(bf16x8, x);
+            };
             const bool plain = !pending && !edge && !(BIAS && (biased || gone));
             int from = 0;                                  // the tile's keys from here on are left to the general form below
             if (plain) {
@@ -640,12 +651,14 @@ __global__ __launch_bounds__(GRP * 256, 2) void hk_prefix_rows_kernel(const Pref
                 };
                 if (__builtin_amdgcn_ballot_w64(!(e0 <= OVERFLOW_SUM)) == 0) {
                     l += e0;
-                    bf16x8 pf[2] = {pack(0), pack(1)};
+                    bf16x8 pf[2] = {pack(0), pack(1)}, pl[2];
+                    if (TWO) pl[0] = rest(0, pf[0]), pl[1] = rest(1, pf[1]);
                     __builtin_amdgcn_s_setprio(2);
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int j = 0; j < 2 * NDT; ++j) {
                         ot[j % NDT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[j & 3], pf[j / NDT], ot[j % NDT], 0, 0, 0);
+                        if (TWO) ot[j % NDT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[j & 3], pl[j / NDT], ot[j % NDT], 0, 0, 0);
                         if (j + 4 < 4 * NDT) vf[j & 3] = vread(j + 4);
 #pragma unroll
                         for (int y = 16 * j / (2 * NDT); y < 16 * (j + 1) / (2 * NDT); ++y) {
@@ -659,10 +672,12 @@ __global__ __launch_bounds__(GRP * 256, 2) void hk_prefix_rows_kernel(const Pref
                         l += e1;
                         pf[0] = pack(2);
                         pf[1] = pack(3);
+                        if (TWO) pl[0] = rest(2, pf[0]), pl[1] = rest(3, pf[1]);
                         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                         for (int j = 2 * NDT; j < 4 * NDT; ++j) {
                             ot[j % NDT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[j & 3], pf[j / NDT - 2], ot[j % NDT], 0, 0, 0);
+                            if (TWO) ot[j % NDT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[j & 3], pl[j / NDT - 2], ot[j % NDT], 0, 0, 0);
                             if (j + 4 < 4 * NDT) vf[j & 3] = vread(j + 4);
                             __builtin_amdgcn_sched_barrier(0);
                         }
@@ -737,7 +752,7 @@ __global__ __launch_bounds__(GRP * 256, 2) void hk_prefix_rows_kernel(const Pref
 #pragma unroll
                         for (int i = 0; i < 16; ++i) ot[d][i] *= a;
                 };
-                auto pv = [&](const bf16x8* pf, auto masked_c) __attribute__((always_inline)) {
+                auto pv = [&](const bf16x8* pf, const bf16x8* pl, auto masked_c) __attribute__((always_inline)) {
 #pragma unroll
                     for (int s = 0; s < 4; ++s) {
                         u32x4 keep = {~0u, ~0u, ~0u, ~0u};
@@ -754,6 +769,7 @@ __global__ __launch_bounds__(GRP * 256, 2) void hk_prefix_rows_kernel(const Pref
                             bf16x8 vf = vread(s * NDT + d);
                             if (decltype(masked_c)::value) vf = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, vf) & keep);
                             ot[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[s], ot[d], 0, 0, 0);
+                            if (TWO) ot[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pl[s], ot[d], 0, 0, 0);
                         }
                     }
                 };
@@ -774,16 +790,17 @@ __global__ __launch_bounds__(GRP * 256, 2) void hk_prefix_rows_kernel(const Pref
                     if (take || __builtin_amdgcn_ballot_w64(!(rs <= OVERFLOW_SUM)) == 0) break;
                 }
                 l += rs;
-                bf16x8 pf[4];                                  // P in bf16, the matrix instruction's operand; l sums the unrounded values
+                bf16x8 pf[4], pl[4];                           // P in bf16, the matrix instruction's operand; l sums the unrounded values
 #pragma unroll
                 for (int s = 0; s < 4; ++s) {
                     u32x4 w;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(st[s >> 1][8 * (s & 1) + 2 * j], st[s >> 1][8 * (s & 1) + 2 * j + 1]);
                     pf[s] = __builtin_bit_cast(bf16x8, w);
+                    if (TWO) pl[s] = rest(s, pf[s]);
                 }
-                if (BIAS && gone) pv(pf, std::true_type{});
-                else pv(pf, std::false_type{});
+                if (BIAS && gone) pv(pf, pl, std::true_type{});
+                else pv(pf, pl, std::false_type{});
             }
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the next tile's LDS-DMA, unknown to the compiler
@@ -1095,21 +1112,21 @@ void launch_once(const PrefixParams& p, const StepWeights& sw, hipStream_t s) {
     if (p.bias) hipLaunchKernelGGL((hk_prefix_part_kernel<HD, 1, true, RAW, 8, true>), grid, dim3(512), 0, s, p, sw);
     else hipLaunchKernelGGL((hk_prefix_part_kernel<HD, 1, false, RAW, 8, true>), grid, dim3(512), 0, s, p, sw);
 }
-template <int HD, bool BIAS, int GRP>
+template <int HD, bool BIAS, int GRP, bool TWO>
 int launch_rows_groups(const PrefixParams& p, const Plan& m, hipStream_t s) {
     constexpr int LDS = GRP * (2 * 2 * KT * HD * 2 + (BIAS ? 2 * KT * 4 : 0));
     static std::atomic<unsigned long long> attr_done{0};   // per device
-    const hipError_t e = hk_lds_attr_once(attr_done, reinterpret_cast<const void*>(&hk_prefix_rows_kernel<HD, BIAS, GRP>), LDS);
+    const hipError_t e = hk_lds_attr_once(attr_done, reinterpret_cast<const void*>(&hk_prefix_rows_kernel<HD, BIAS, GRP, TWO>), LDS);
     if (e != hipSuccess) {
         hk_set_error("hk_prefix_attn_bf16: hipFuncSetAttribute(%d B LDS): %s", LDS, hipGetErrorString(e));
         return HK_ELAUNCH;
     }
-    hipLaunchKernelGGL((hk_prefix_rows_kernel<HD, BIAS, GRP>), dim3((unsigned)rows_grid(p, m)), dim3(GRP * 256), LDS, s, p, m.rows);
+    hipLaunchKernelGGL((hk_prefix_rows_kernel<HD, BIAS, GRP, TWO>), dim3((unsigned)rows_grid(p, m)), dim3(GRP * 256), LDS, s, p, m.rows);
     return HK_OK;
 }
 template <int HD, bool BIAS>
 int launch_rows(const PrefixParams& p, const Plan& m, hipStream_t s) {
-    return m.groups == 2 ? launch_rows_groups<HD, BIAS, 2>(p, m, s) : launch_rows_groups<HD, BIAS, 1>(p, m, s);
+    return m.groups == 2 ? launch_rows_groups<HD, BIAS, 2, false>(p, m, s) : launch_rows_groups<HD, BIAS, 1, false>(p, m, s);
 }
 template <int HD, int SG>
 void launch_join(const PrefixParams& p, hipStream_t s) {
@@ -1124,7 +1141,9 @@ int launch_prefix(const PrefixParams& p, const Plan& m, hipStream_t s) {
     }
     if (m.mode != SMALL) {
         // MIXED: the rows kernel reads the prefix only, which has no bias
-        const int rc = p.bias && m.mode != MIXED ? launch_rows<HD, true>(p, m, s) : launch_rows<HD, false>(p, m, s);
+        const int rc = m.mode == MIXED && p.Nq == 1 ? launch_rows_groups<HD, false, 1, true>(p, m, s)
+                       : p.bias && m.mode != MIXED  ? launch_rows<HD, true>(p, m, s)
+                                                    : launch_rows<HD, false>(p, m, s);
         if (rc != HK_OK || m.mode == FUSED) return rc;
     }
     if (m.mode != PACKED) {

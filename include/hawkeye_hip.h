@@ -425,7 +425,7 @@ int hk_qformer_embed_bwd(const float* dz, const int64_t* input_ids, float* dquer
  *   O = softmax over the P prefix keys, all visible, and the sequence's own keys j <= i + (Nk - Nq)      (Nk >= Nq >= 1, P >= 0)
  * The prefix's K and V exist once and are read once for the rows of all sequences.  Prompts (Nq > 1: the questions) and single tokens
  * (Nq = 1: the decode step) alike.  bf16 in and out, fp32 softmax; the probabilities enter the second product as two bf16 numbers (2^-16 of
- * themselves) in steps and calls of a few tokens, as one (2^-8, as in hk_flash_attn_bf16) where rows fill blocks of 128.
+ * themselves) in steps and calls of a few tokens, as one (2^-8, as in hk_flash_attn_bf16) where the rows of questions (Nq > 1) fill blocks of 128.
  *   Q [B,Nq,H,hd] carries softmax_scale * log2(e); KP / VP [P,H,hd]; K / V [B,Nk,H,hd]; O [B,Nq,H,hd]: token strides ld*, batch strides
  *   bs* in elements, head h at column h * hd.  key_bias: optional fp32, own key j of sequence b adds key_bias[b * bias_bs + j] (natural-log
  *   units); a key whose bias is -1e4 or less (hk_qformer_key_bias's mask value, -inf) is removed: its K and V rows may hold anything.

@@ -757,3 +757,9 @@ def test_prefix_attention_in_a_workspace_of_the_callers():
     kp, k = _rand((300, 4, 128), 2), _rand((4, 20, 4, 128), 4)                                # one launch: whatever is passed is left alone
     buf = torch.full((64,), 255, dtype=torch.uint8, device=DEV)
     assert torch.equal(ops.prefix_attention(q, kp, kp, k, k, ws=buf), ops.prefix_attention(q, kp, kp, k, k)) and bool((buf == 255).all())
+
+
+@pytest.mark.parametrize("B,Nq,P,Nk,H,hd,kind", [           # the prefix by blocks of 128 rows
+    (64, 1, 5000, 40, 16, 128, None), (64, 1, 5000, 140, 16, 128, "left"), (130, 1, 2600, 20, 32, 64, None), (130, 1, 2600, 20, 32, 64, "add"), (256, 1, 200, 30, 64, 128, None)])
+def test_steps_of_many_sequences_keep_the_bits_of_their_probabilities(B, Nq, P, Nk, H, hd, kind):
+    test_steps_keep_the_bits_of_their_probabilities(B, Nq, P, Nk, H, hd, kind)
