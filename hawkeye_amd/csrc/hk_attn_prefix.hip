@@ -5,7 +5,7 @@
 //
 // over the prefix's keys and the row's own; softmax sums are associative, so the keys are cut into chunks, a chunk leaves
 // (m, l, o) = (its maximum, sum_j 2^(s_j - m), sum_j 2^(s_j - m) v_j) in 32 bits, and a second launch joins the chunks of a
-// row in index order (bit-reproducible).
+// row.  Tiles go to waves, and chunks to groups of threads, in turn; every sum's order follows from the sizes alone (bit-reproducible).
 //
 // hk_prefix_part_kernel: a workgroup = one (head, key chunk, group of query rows).  Prefix chunks take rows of ALL
 // sequences (row r = sequence r / Nq, token r % Nq), a sequence's own chunks take its Nq rows.  Its four waves walk 32-key tiles

@@ -78,8 +78,8 @@ struct GemmParams {
 // Exact-erf GELU (nn.GELU default, vit.py:44; ACT2FN["gelu"], Qformer.py:383) to fp32 rounding noise:
 // erfc(t) = exp2(t * p(t)) on t in [0, 6], |err| <= 3.2e-7 (degree-5 fit), and
 //     gelu(x) = 0.5 x + 0.5 |x| (1 - erfc(|x| / sqrt 2))
-// which needs no sign select.  Written on float2 so hipcc emits v_pk_fma_f32 / v_pk_mul_f32: 8 VALU
-// instructions per element instead of 14.
+// which needs no sign select: 13 VALU instructions per element.  (On pairs of elements, but packed fp32 instructions are
+// off for all kernels: the Makefile says why.)
 typedef __attribute__((ext_vector_type(2))) float f32x2;
 __device__ __forceinline__ f32x2 gelu_erf2(const f32x2 x) {
     const f32x2 a = __builtin_elementwise_max(x, -x);

@@ -433,7 +433,9 @@ int hk_qformer_embed_bwd(const float* dz, const int64_t* input_ids, float* dquer
  * ws: hk_prefix_attn_ws bytes of the caller's, 16-byte aligned, for this call alone (calls in flight together need one each); where that is
  * HK_NO_WS, one launch does it all and ws may be NULL.  out may not overlap an input or ws; strides are multiples of 8 elements (4: O's),
  * token strides of K and V below 2^25.
- * Bit-reproducible: chunks are joined in index order. */
+ * Scores are held in 32 bits with the bias in them: where all that a row sees carries a bias b, they are good to 2^-24 |b|.  Own rows of V that only
+ * later queries see must be finite (0 times infinity is not).
+ * Bit-reproducible: the order of every sum follows from the sizes alone. */
 #define HK_NO_WS 16
 typedef struct hk_prefix_attn_desc {
     const void* Q;
@@ -476,8 +478,8 @@ size_t hk_decode_attn_weights_ws(int32_t B, int32_t H, int32_t head_dim, int32_t
  *   w_out[b][h][j] = w_in[b][h][j] + sum over i of softmax_j(q_i . k_j + bias_j),   causal: query i sees keys <= i + (Nk - Nq)
  * Q [B,Nq,H,hd] (carrying softmax_scale * log2(e)) and K [B,Nk,H,hd] bf16 through strides as in hk_attn_desc; weights fp32 with strides
  * (*_bs, *_hs), w_in NULL = zeros, may be w_out; key_bias[b * bias_bs + j] as in hk_prefix_attn_desc; a query that sees no key adds nothing.
- * ws: hk_attn_key_weights_ws bytes of the caller's, 16-byte aligned (the rows' log2 sums; few queries take theirs in chunks of keys, joined in
- * index order; HK_NO_WS: few keys, one launch, ws may be NULL).  Strides as in hk_prefix_attn_desc.  Else two or three launches: row sums, their
+ * ws: hk_attn_key_weights_ws bytes of the caller's, 16-byte aligned (the rows' log2 sums, one 32-bit number each; few queries take theirs in chunks of keys;
+ * HK_NO_WS: few keys, one launch, ws may be NULL).  Strides as in hk_prefix_attn_desc.  Else two or three launches: row sums, their
  * join, weights.  Bit-reproducible. */
 typedef struct hk_key_weights_desc {
     const void* Q;
