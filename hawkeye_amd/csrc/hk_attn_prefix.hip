@@ -16,10 +16,10 @@
 // K goes from memory straight to the A operand's registers, V through 32 keys of LDS that belong to the wave (no barrier in
 // the loop).  The next tile's K is requested as soon as this one's scores stand, its V as soon as this one's is in LDS: a
 // wave keeps about 16 KB in flight, 8 waves per CU.  Bound by memory: 16 sequences' step over 1500 own keys each (398 MB) 80 us, 5.0 TB/s;
-// 64 sequences' over 512 own keys each beside the prefix 66 us.
+// 64 sequences' over 333 own keys each beside the prefix (350 MB) 67 us.
 // Many sequences with few own keys each: a wave takes a sequence's keys alone (by_wave).
 // ONE: a workgroup of eight waves per (sequence, head) for all its keys, the prefix's tiles first; no chunks, no second launch, a step's scores
-// stay in LDS.  Bound by latency (a chain of dependent tiles per wave): one sequence over 353 keys 8 us, and the host needs 10 for the call.
+// stay in LDS.  Bound by latency (a chain of dependent tiles per wave): one sequence over 353 keys 7.7 us, and the host needs 10 for the call.
 #include <type_traits>
 #include "hk_common.h"
 #include "hk_overlap.h"
@@ -419,12 +419,12 @@ __global__ __launch_bounds__(NW * 64, HD == 128 && RT == 1 && !BIAS && !ONE ? 3 
 // TWO: P as two bf16 numbers, as in hk_prefix_part_kernel, for steps (MIXED, Nq = 1), which reading bounds: one : two (us, in a graph), 64 sequences
 // over 16384 + 333 keys 129.3 : 130.2, 128 over 2000 + 20 32.1 : 33.8.  One, off by 2^-8, for questions, as in hk_flash_attn_bf16: the feed of the
 // matrix unit bounds those (32 x 16 tokens over 1600 39.2 : 44.4).
-// Measured (32 heads of 128): 8 sequences of 512 rows over 1400 shared keys and their own 120 us, 930 TFLOP/s; the matrix unit is busy half of
+// Measured (32 heads of 128): 8 sequences of 512 rows over 1400 shared keys and their own 116-125 us, 890-960 TFLOP/s; the matrix unit is busy half of
 // the time.  Copies of the loop without one part, in-bounds and for timing only: without LDS-DMA and barriers 107-116 us, without the reads of
 // K from LDS 84, without those of V too 79, without exp2 101: bound by feeding the matrix unit from LDS (each wave reads every tile), at the clock that the
 // card holds under it.  Slower: 32-key tiles at 3-4 waves per SIMD (10-40 %), LDS-DMA spread over the matrix steps (141), K read before
 // the LDS-DMA is issued (130), four stages instead of two (10-40 % where a CU holds two workgroups, the same elsewhere).  64 sequences' single rows over 16384 shared keys
-// (268 MB, one workgroup per CU): 54-59 us, 4.5-5.0 TB/s.
+// (268 MB, one workgroup per CU): 59-69 us, 3.9-4.5 TB/s, P as two numbers (54-59 as one).
 struct RowsParams {
     int packed;                      // prefix by packed row blocks and key chunks, own keys apart; else both in one workgroup
     int npb, nob;                    // row blocks: of all rows (packed prefix), of a sequence

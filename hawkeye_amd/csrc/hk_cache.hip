@@ -18,7 +18,7 @@ constexpr float REMOVED = -1.0e4f;   // a key whose bias is at or below this doe
 //   SUMS:  keys stay, queries pass: 2^(s - z) added up in 16 registers per lane, over the 32 lanes at the end.
 // GRP = 2: two such groups of four waves share a workgroup, each with stages of its own, and take every other tile; the second's sums
 // join the first's through LDS at the end.  Chunks of keys (key_chunks) leave (m, sum) for a small launch that joins them: every order is fixed.
-// Measured: 2 x 2047 tokens, 32 heads of 128, padded 77-89 us for both launches (clock), 770-890 TFLOP/s of the products they make (each makes them
+// Measured: 2 x 2047 tokens, 32 heads of 128, padded 75-86 us for both launches (clock), 800-910 TFLOP/s of the products they make (each makes them
 // all).  The matrix unit is busy 21 % of the time, the vector unit 38 %, 1.8 waves per SIMD on average: bound by the chain of a tile within a wave
 // (LDS, 16 matrix instructions, 32 exp2: about 2000 cycles) and the uneven lengths of causal blocks.  No gain: 128-row tiles, their products
 // spread among the exponentials, fragments read 2-8 steps ahead, starting values kept in registers, long and short blocks paired on a CU by

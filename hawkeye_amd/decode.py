@@ -233,7 +233,8 @@ class LlamaGenerator:
         read once for the batch, in the prefill and in every step; src then holds what follows it.
         cache_budget: the sequences' caches are cut to this many rows per layer and head whenever they have outgrown it by ROW_GRANULE (the
         prompt's at once): the last cache_recent rows (default: half of the budget) and those that have collected the most attention
-        weight stay.  Not together with prefix (cut the prefix itself: make_prefix(budget=)).
+        weight stay.  Steps get cheaper, not longer dialogues possible: positions go on and end at max_position_embeddings.  Not together with
+        prefix (cut the prefix itself: make_prefix(budget=)).
         Returns {"tokens": int64 [B, T] (T <= max_new_tokens), "logits": fp32 [T, B, V] if return_logits}."""
         cfg = self.cfg
         if max_new_tokens < 1:
